@@ -439,6 +439,101 @@ int scn_scatter_columns_axpy(float *d_W, int K, int N, const int *d_idx, int n, 
 int scn_sgemm_rowmajor(int transA, int transB, const float *d_A, const float *d_B, float *d_C, int l, int m, int r,
                        float alpha, float beta, scn_stream_t stream);
 
+/* ------------------------------------------------------------------ embedding table (no counterpart in the reference)
+ * Sites that carry a code (a pen stroke's kind, a material, a label) instead of real features: a table
+ * [vocab x C] in front of the first layer turns each row's code into C features, and learns. */
+
+/* Types of the arrays passed as void pointers. */
+enum scn_type { SCN_F32 = 0, SCN_BF16 = 1, SCN_F16 = 2 };
+
+/* Bit that the embedding calls may set in *d_errors (which they never clear): SCN_DEV_ERR_KEY, a token at or above vocab. */
+
+/* out[i][c] = scale * table[tokens[i]][c], computed in 32 bits and rounded once to out_type.  A negative token (a
+ * sample's background row, say) gives a zero row, as a negative rule does in scn_gather_forward; so does a token at or
+ * above vocab, which also sets SCN_DEV_ERR_KEY in *d_errors if that is not NULL.
+ *   d_table     [vocab x C] of table_type
+ *   d_out       n rows of C values of out_type, out_stride (>= C) values apart: a column range of a wider feature
+ *               matrix can be written; what lies between the rows is left as it is.  It must not overlap the table. */
+int scn_embedding_forward(const void *d_table, int table_type, int vocab, int C, const int *d_tokens, long long n, float scale,
+                          void *d_out, int out_type, long long out_stride, int *d_errors, scn_stream_t stream);
+
+/* The table's gradient: dtable[t][c] = scale * sum of dout[i][c] over the rows i with tokens[i] == t, in 32 bits.  The
+ * rows are sorted by token (stably), each token's rows are added in an order that depends on the tokens alone: the
+ * same call gives the same bits.  Without `accumulate` all vocab rows are written (zeros where no token points); with
+ * it the sums are added onto what is there and rows without a token are left as they are.  Negative tokens and tokens at
+ * or above vocab (these set SCN_DEV_ERR_KEY in *d_errors if not NULL) contribute nothing.
+ *   d_dout      n rows of C values of dout_type, dout_stride (>= C) values apart
+ *   d_workspace scn_embedding_backward_workspace_bytes(n, vocab, C) bytes (0: bad sizes), 16-byte aligned, nothing kept
+ *               in it between calls; calls that can overlap on the GPU need a workspace each. */
+size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C);
+int scn_embedding_backward(const int *d_tokens, long long n, const void *d_dout, int dout_type, long long dout_stride, int vocab, int C,
+                           float scale, int accumulate, float *d_dtable, int *d_errors, void *d_workspace, size_t workspace_bytes,
+                           scn_stream_t stream);
+
+/* ------------------------------------------------------------------ AdamW (no counterpart in the reference)
+ * One step of Adam with decoupled weight decay over a list of tensors in one launch (one more for every further
+ * SCN_ADAMW_MAX_TENSORS tensors, and for a list that mixes 8-bit and 32-bit states).  For every value, at step t:
+ *     g' = g * grad_scale * clip               clip: 1, or max_norm / norm where that is smaller (see d_norm)
+ *     m  = beta1 m + (1 - beta1) g'
+ *     v  = beta2 v + (1 - beta2) g' g'
+ *     w  = max(w_min, w - lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay w))
+ * in 32 bits; w_min = -INFINITY: no bound. */
+#define SCN_ADAMW_MAX_TENSORS 320
+#define SCN_ADAMW_BLOCK 256
+
+/* One tensor of the list.  32-bit states: d_m, d_v are float[n], the scales NULL.  8-bit states: blocks of
+ * SCN_ADAMW_BLOCK consecutive values (the last one shorter) share a scale s, a power of two, in
+ * d_m_scale / d_v_scale [ceil(n / SCN_ADAMW_BLOCK)]; d_m is int8_t[n], a code q standing for q |q| s (-127 <= q <= 127);
+ * d_v is uint8_t[n], a code q standing for q^4 s.  All bytes zero: m = v = 0, where a run starts.  A value between two
+ * codes goes up or down by a number drawn from (seed, its position in the call's list), so that the code's mean is
+ * the value: a moving average whose change is a fraction of a code would else stand still.  v > 0 is never
+ * stored as 0.  A block with a value that is not finite gets a NaN scale: all its states read as NaN from then on.
+ * Tensors must not overlap, and each pointer is aligned to its own type. */
+typedef struct {
+  float *d_w;          /* [n] the parameters, updated in place                                         */
+  const void *d_g;     /* [n] their gradient, of g_type                                                */
+  void *d_m, *d_v;     /* [n] the moments                                                              */
+  float *d_m_scale, *d_v_scale;
+  void *d_w16;         /* NULL, or [n]: the updated parameters rounded to w16_type (SCN_BF16, SCN_F16) */
+  long long n;
+  float weight_decay, w_min;
+  int g_type, w16_type;
+} scn_adamw_tensor_t;
+
+typedef struct {
+  double lr, beta1, beta2, eps; /* 0 <= beta < 1, eps > 0                                             */
+  double grad_scale;            /* 1 / batch size for the sums over a batch that the layers give, say */
+  double max_norm;              /* > 0: clip to this norm (needs d_norm); 0: no clipping              */
+  long long step;               /* t >= 1                                                             */
+  unsigned seed;                /* of the 8-bit states' rounding: another one each step               */
+} scn_adamw_t;
+
+/* The same as the kernel reads it (48 bytes).  A step captured into a CUDA graph takes its numbers from device memory instead
+ * (d_scalars), where the caller puts the next step's before each replay. */
+typedef struct {
+  float lr, beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
+  float bias1, bias2;           /* 1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t) */
+  float grad_scale, max_norm;
+  unsigned seed, reserved;
+} scn_adamw_scalars_t;
+int scn_adamw_scalars(const scn_adamw_t *h, scn_adamw_scalars_t *out); /* on the host */
+
+/* *d_norm = the 2-norm of all the list's gradients together (grad_scale not applied), summed in 64 bits in a fixed
+ * order.  Reads d_g, g_type and n only.  Workspace: scn_grad_norm_workspace_bytes() bytes, 8-byte aligned, nothing kept
+ * in it between calls. */
+size_t scn_grad_norm_workspace_bytes(void);
+int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float *d_norm, void *d_workspace, size_t workspace_bytes,
+                  scn_stream_t stream);
+
+/* The step.  `tensors` and `h` are host arrays, read before the call returns.  d_scalars: NULL, or a device copy of the
+ * scalars to use instead of h's (h may then be NULL).  d_norm: NULL, or the norm of all gradients on the device
+ * (scn_grad_norm's): needed for max_norm, and a norm that is not finite makes the step change nothing at all. */
+int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, const scn_adamw_t *h, const scn_adamw_scalars_t *d_scalars,
+                   const float *d_norm, scn_stream_t stream);
+
+/* What 8-bit states stand for: d_out[n] from d_codes[n] and d_scale[ceil(n / SCN_ADAMW_BLOCK)]; second: codes of v, else of m. */
+int scn_adamw_decode(const void *d_codes, const float *d_scale, long long n, int second, float *d_out, scn_stream_t stream);
+
 /* ------------------------------------------------------------------ result exchange between the GPUs of one node
  * The reference runs on one GPU (SparseConvNetCUDA.cu:43-71 picks a single device).  Sharded by sample over several
  * GPUs, the path has one exchange step: every rank's [rows x nClasses] block of probabilities (what

@@ -26,6 +26,8 @@ EXPORTS = [
     "scn_exchange_buffer_bytes", "scn_exchange_set_timeout_ms", "scn_exchange_alloc", "scn_exchange_free", "scn_exchange_open", "scn_exchange_close", "scn_exchange_publish", "scn_exchange_collect", "scn_exchange_step",
     "scn_mask_columns", "scn_sgd_update_masked", "scn_gather_columns", "scn_scatter_columns_axpy", "scn_sgemm_rowmajor", "scn_softmax_nll_backward", "scn_activation_backward", "scn_conv_nin_backward_weights", "scn_conv_nin_backward_weights_tc_bytes", "scn_conv_nin_backward_weights_tc", "scn_transpose_weights", "scn_gather_backward",
     "scn_maxpool_backward", "scn_terminal_pool_backward", "scn_sgd_update",
+    "scn_embedding_forward", "scn_embedding_backward_workspace_bytes", "scn_embedding_backward",
+    "scn_adamw_scalars", "scn_grad_norm_workspace_bytes", "scn_grad_norm", "scn_adamw_step", "scn_adamw_decode",
 ]
 
 
@@ -36,6 +38,26 @@ class Regions(ctypes.Structure):
 class ChainLayer(ctypes.Structure):
     _fields_ = [("regions", Regions), ("d_out_keys", c_p), ("d_out_off", c_p), ("d_out_bg", c_p), ("d_rules", c_p),
                 ("rows_out_capacity", c_int), ("d_result", c_p)]
+
+
+F32, BF16, F16 = 0, 1, 2
+ADAMW_BLOCK = 256
+_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("d_w", c_p), ("d_g", c_p), ("d_m", c_p), ("d_v", c_p), ("d_m_scale", c_p), ("d_v_scale", c_p), ("d_w16", c_p),
+                ("n", c_ll), ("weight_decay", c_f), ("w_min", c_f), ("g_type", c_int), ("w16_type", c_int)]
+
+
+class AdamWParameters(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("grad_scale", ctypes.c_double), ("max_norm", ctypes.c_double), ("step", c_ll), ("seed", ctypes.c_uint)]
+
+
+class AdamWScalars(ctypes.Structure):
+    _fields_ = [(n, c_f) for n in ("lr", "beta1", "beta2", "one_minus_beta1", "one_minus_beta2", "eps", "bias1", "bias2", "grad_scale",
+                                   "max_norm")] + [("seed", ctypes.c_uint), ("reserved", ctypes.c_uint)]
 
 
 class ScnError(RuntimeError):
@@ -101,6 +123,15 @@ def lib():
         L.scn_top_indices.argtypes = [c_p, c_int, c_int, c_int, c_p, c_p]
         L.scn_activation_forward.argtypes = [c_p, c_p, c_int, c_int, c_int, c_p, c_p]
         L.scn_background_rows.argtypes = [c_p, c_p, c_int, c_p, c_p]
+        L.scn_embedding_forward.argtypes = [c_p, c_int, c_int, c_int, c_p, c_ll, c_f, c_p, c_int, c_ll, c_p, c_p]
+        L.scn_embedding_backward_workspace_bytes.restype = c_sz
+        L.scn_embedding_backward_workspace_bytes.argtypes = [c_ll, c_int, c_int]
+        L.scn_embedding_backward.argtypes = [c_p, c_ll, c_p, c_int, c_ll, c_int, c_int, c_f, c_int, c_p, c_p, c_p, c_sz, c_p]
+        L.scn_adamw_scalars.argtypes = [c_p, c_p]
+        L.scn_grad_norm_workspace_bytes.restype = c_sz
+        L.scn_grad_norm.argtypes = [c_p, c_int, c_p, c_p, c_sz, c_p]
+        L.scn_adamw_step.argtypes = [c_p, c_int, c_p, c_p, c_p, c_p]
+        L.scn_adamw_decode.argtypes = [c_p, c_p, c_ll, c_int, c_p, c_p]
         _lib = L
     return _lib
 
@@ -537,6 +568,201 @@ def sgd_update_masked(w, m, d, row_mask, row_period, col_mask, lr, momentum, kee
 def sgemm_rowmajor(A, B, C, l, m, r, alpha=1.0, beta=0.0, trans_a=False, trans_b=False):
     """C[l x r] = alpha * op(A) op(B) + beta * C (in place on C)."""
     check(lib().scn_sgemm_rowmajor(int(trans_a), int(trans_b), _ptr(_f32(A)), _ptr(_f32(B)), _ptr(_f32(C)), l, m, r, c_f(alpha), c_f(beta), _stream()))
+
+
+# ---------------------------------------------------------------------------------------------- embedding table
+def _here(device):
+    """The current device's index, if `device` is it: kernels run on the current device's current stream."""
+    if device.type != "cuda":
+        raise ScnError("invalid argument: CUDA tensors are needed, not tensors on %s" % device)
+    if device.index != torch.cuda.current_device():
+        raise ScnError("invalid argument: tensors on %s, the current device is cuda:%d" % (device, torch.cuda.current_device()))
+
+
+def _rows_of(t, n, C, what):
+    """(pointer, type, row stride) of a 2-d tensor [n, C] whose rows may lie further apart than C."""
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != C or t.dtype not in _TYPES or not t.is_cuda:
+        raise ScnError("invalid argument: %s must be a CUDA tensor [%d, %d] of float32, bfloat16 or float16" % (what, n, C))
+    stride = t.stride(0) if n > 1 else C
+    if (C > 1 and t.stride(1) != 1) or stride < C:
+        raise ScnError("invalid argument: %s: the values of a row must lie together and rows must not overlap" % what)
+    return t.data_ptr(), _TYPES[t.dtype], stride
+
+
+def _tokens_of(tokens, device):
+    if tokens.dtype != torch.int32 or tokens.dim() != 1 or not tokens.is_contiguous() or tokens.device != device:
+        raise ScnError("invalid argument: tokens must be a contiguous 1-d int32 tensor on the other arguments' device")
+    return tokens.data_ptr(), tokens.numel()
+
+
+def _optional_i32(t, device, what):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() < 1 or not t.is_contiguous() or t.device != device:
+        raise ScnError("invalid argument: %s must be an int32 tensor on the other arguments' device" % what)
+    return t.data_ptr()
+
+
+def embedding_forward(table, tokens, scale=1.0, out=None, out_dtype=torch.float32, errors=None):
+    """scn_embedding_forward: scale * table[tokens] as a new tensor [n, C] of out_dtype, or into `out` (a view with a row
+    stride is fine).  errors: int32 tensor that gets DEV_ERR_KEY or-ed in where a token is not below the table's rows."""
+    dev = table.device
+    _here(dev)
+    if table.dim() != 2 or table.dtype not in _TYPES or not table.is_contiguous():
+        raise ScnError("invalid argument: the table must be a contiguous 2-d tensor of float32, bfloat16 or float16")
+    V, C = table.shape
+    ptr, n = _tokens_of(tokens, dev)
+    if out is None:
+        out = torch.empty((n, C), dtype=out_dtype, device=dev)
+    elif out.device != dev:
+        raise ScnError("invalid argument: out is on another device")
+    optr, otype, stride = _rows_of(out, n, C, "out")
+    check(lib().scn_embedding_forward(table.data_ptr(), _TYPES[table.dtype], V, C, ptr, n, scale, optr, otype, stride,
+                                      _optional_i32(errors, dev, "errors"), torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def embedding_backward_workspace(n, vocab, C, device):
+    nbytes = lib().scn_embedding_backward_workspace_bytes(n, vocab, C)
+    if not nbytes:
+        raise ScnError("invalid argument: bad embedding sizes")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def embedding_backward(dout, tokens, dtable, scale=1.0, accumulate=False, workspace=None, errors=None):
+    """scn_embedding_backward: the gradient of embedding_forward's table into the float32 tensor dtable [vocab, C] (added
+    onto it with `accumulate`); returns dtable.  workspace: embedding_backward_workspace(n, vocab, C, device), to keep."""
+    dev = dtable.device
+    _here(dev)
+    if dtable.dim() != 2 or dtable.dtype != torch.float32 or not dtable.is_contiguous():
+        raise ScnError("invalid argument: dtable must be a contiguous 2-d float32 tensor")
+    V, C = dtable.shape
+    ptr, n = _tokens_of(tokens, dev)
+    if dout.device != dev:
+        raise ScnError("invalid argument: dout is on another device")
+    dptr, dtype, stride = _rows_of(dout, n, C, "dout")
+    if workspace is None:
+        workspace = embedding_backward_workspace(n, V, C, dev)
+    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ScnError("invalid argument: the workspace must be a uint8 tensor on the other arguments' device")
+    check(lib().scn_embedding_backward(ptr, n, dptr, dtype, stride, V, C, scale, int(accumulate), dtable.data_ptr(),
+                                       _optional_i32(errors, dev, "errors"), workspace.data_ptr(), workspace.numel(),
+                                       torch.cuda.current_stream().cuda_stream))
+    return dtable
+
+
+# ---------------------------------------------------------------------------------------------- AdamW
+def adamw_states(n, device, bits=8):
+    """Moments of n values as a run starts, as keyword arguments of an AdamW entry: {"m", "v"} or {"m", "v", "m_scale", "v_scale"}."""
+    if bits == 32:
+        return dict(m=torch.zeros(n, device=device), v=torch.zeros(n, device=device))
+    if bits != 8:
+        raise ScnError("invalid argument: states have 8 or 32 bits")
+    blocks = -(-n // ADAMW_BLOCK)
+    return dict(m=torch.zeros(n, dtype=torch.int8, device=device), v=torch.zeros(n, dtype=torch.uint8, device=device),
+                m_scale=torch.zeros(blocks, device=device), v_scale=torch.zeros(blocks, device=device))
+
+
+def adamw_scalars(lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, max_norm=0.0, seed=None):
+    """scn_adamw_scalars as a CPU int32 tensor [12]: what AdamW.step(scalars=...) reads from device memory."""
+    h = AdamWParameters(lr, beta1, beta2, eps, grad_scale, max_norm, step, (step if seed is None else seed) & 0xFFFFFFFF)
+    out = torch.empty(12, dtype=torch.int32)
+    check(lib().scn_adamw_scalars(ctypes.byref(h), out.data_ptr()))
+    return out
+
+
+class AdamW:
+    """scn_adamw_step / scn_grad_norm over a fixed list of tensors.  Each entry is a dict of contiguous CUDA tensors: w (float32),
+    g (float32, bfloat16 or float16), m and v (float32; or int8 and uint8 with float32 m_scale and v_scale, see
+    adamw_states), optionally w16 (bfloat16 or float16, receives the updated w), and numbers weight_decay and w_min.
+    The object keeps references to the tensors; their memory must stay where it is."""
+
+    def __init__(self, tensors):
+        self.tensors = [dict(t) for t in tensors]
+        self.count = len(self.tensors)
+        self.list = (AdamWTensor * max(self.count, 1))()
+        self.device = self.tensors[0]["w"].device if self.tensors else torch.device("cuda", torch.cuda.current_device())
+        spans = []
+        for i, t in enumerate(self.tensors):
+            n = t["w"].numel()
+            eight = t.get("m_scale") is not None or t.get("v_scale") is not None
+            blocks = -(-n // ADAMW_BLOCK)
+            want = dict(w=(n, (torch.float32,)), g=(n, tuple(_TYPES)), m=(n, (torch.int8 if eight else torch.float32,)),
+                        v=(n, (torch.uint8 if eight else torch.float32,)))
+            if eight:
+                want.update(m_scale=(blocks, (torch.float32,)), v_scale=(blocks, (torch.float32,)))
+            if t.get("w16") is not None:
+                want["w16"] = (n, (torch.bfloat16, torch.float16))
+            unknown = set(t) - set(want) - {"weight_decay", "w_min", "w16", "m_scale", "v_scale"}
+            if unknown:
+                raise ScnError("invalid argument: AdamW tensor %d: unknown entries %s" % (i, sorted(unknown)))
+            e = self.list[i]
+            for k, (size, types) in want.items():
+                x = t.get(k)
+                if x is None or x.numel() != size or x.dtype not in types or not x.is_contiguous() or x.device != self.device or not x.is_cuda:
+                    raise ScnError("invalid argument: AdamW tensor %d: %s must be a contiguous tensor of %d values of %s on %s" % (
+                        i, k, size, " or ".join(str(y) for y in types), self.device))
+                setattr(e, "d_" + k, x.data_ptr())
+                if size:
+                    spans.append((x.data_ptr(), x.data_ptr() + size * x.element_size(), k == "g"))
+            e.n, e.weight_decay, e.w_min = n, t.get("weight_decay", 0.0), t.get("w_min", float("-inf"))
+            e.g_type = _TYPES[t["g"].dtype]
+            e.w16_type = _TYPES[t["w16"].dtype] if t.get("w16") is not None else F32
+        written, read = 0, 0  # ends of what is written and of what is only read so far, in the order of the addresses
+        for first, last, only_read in sorted(spans):
+            if first < written or (first < read and not only_read):
+                raise ScnError("invalid argument: AdamW: a tensor that the step writes overlaps another one")
+            if only_read:
+                read = max(read, last)
+            else:
+                written = max(written, last)
+        self.h = AdamWParameters()
+        self._h = ctypes.byref(self.h)
+        self._norm = torch.empty(1, device=self.device)
+        self._workspace = torch.empty(lib().scn_grad_norm_workspace_bytes(), dtype=torch.uint8, device=self.device)
+
+    def grad_norm(self):
+        """The 2-norm of all gradients as a float32 tensor [1] that this object owns."""
+        _here(self.device)
+        check(lib().scn_grad_norm(self.list, self.count, self._norm.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(),
+                                  torch.cuda.current_stream().cuda_stream))
+        return self._norm
+
+    def step(self, lr=None, step=None, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, seed=None, norm=None, max_norm=0.0, scalars=None):
+        """Step number `step` (from 1).  seed: of the 8-bit states' rounding (the step number unless given).  norm: what
+        grad_norm() returned, for max_norm > 0.  scalars: a CUDA copy of adamw_scalars(...) instead of the numbers, for a
+        captured step."""
+        _here(self.device)
+        if scalars is not None:
+            if lr is not None or step is not None:
+                raise ScnError("invalid argument: pass the numbers or the scalars, not both")
+            if scalars.dtype != torch.int32 or scalars.numel() != 12 or scalars.device != self.device or not scalars.is_contiguous():
+                raise ScnError("invalid argument: scalars must be a CUDA copy of adamw_scalars(...)")
+            h, sp = None, scalars.data_ptr()
+        else:
+            if lr is None or step is None:
+                raise ScnError("invalid argument: a step needs lr and its number")
+            p = self.h
+            p.lr, p.beta1, p.beta2, p.eps, p.grad_scale, p.max_norm, p.step = lr, beta1, beta2, eps, grad_scale, max_norm, step
+            p.seed = (step if seed is None else seed) & 0xFFFFFFFF
+            h, sp = self._h, None
+        if norm is not None and (norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != self.device):
+            raise ScnError("invalid argument: norm must be a float32 tensor of one value on the tensors' device")
+        check(lib().scn_adamw_step(self.list, self.count, h, sp, None if norm is None else norm.data_ptr(),
+                                   torch.cuda.current_stream().cuda_stream))
+
+
+def adamw_decode(codes, scale):
+    """What 8-bit moments stand for, as a new float32 tensor: codes int8 (first moment) or uint8 (second)."""
+    n = codes.numel()
+    if codes.dtype not in (torch.int8, torch.uint8) or not codes.is_contiguous() or scale.dtype != torch.float32 or not scale.is_contiguous() \
+            or scale.numel() != -(-n // ADAMW_BLOCK) or scale.device != codes.device:
+        raise ScnError("invalid argument: codes must be int8 or uint8 with a float32 scale for each %d of them" % ADAMW_BLOCK)
+    _here(codes.device)
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    check(lib().scn_adamw_decode(codes.data_ptr(), scale.data_ptr(), n, int(codes.dtype == torch.uint8), out.data_ptr(),
+                                 torch.cuda.current_stream().cuda_stream))
+    return out
 
 
 class ExchangeBuffer:

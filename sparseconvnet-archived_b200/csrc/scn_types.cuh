@@ -1,0 +1,28 @@
+// Values held as float, bfloat16 or IEEE half (enum scn_type), read and written as float.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "scn_common.cuh"
+
+namespace scn {
+
+inline bool type_known(int type) { return type == SCN_F32 || type == SCN_BF16 || type == SCN_F16; }
+inline int type_bytes(int type) { return type == SCN_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v); // rounded to nearest, ties to even
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// CALL with T naming the C++ type of a run-time scn_type.
+#define SCN_DISPATCH_TYPE(type, T, CALL)                                                    \
+  switch (type) {                                                                           \
+  case SCN_BF16: { using T = __nv_bfloat16; CALL; } break;                                  \
+  case SCN_F16: { using T = __half; CALL; } break;                                          \
+  default: { using T = float; CALL; } break;                                                \
+  }
+
+} // namespace scn
