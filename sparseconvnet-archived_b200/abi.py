@@ -718,11 +718,11 @@ class AdamW:
                 written = max(written, last)
         self.h = AdamWParameters()
         self._h = ctypes.byref(self.h)
-        self._norm = torch.empty(1, device=self.device)
+        self._norm = torch.empty((), device=self.device)
         self._workspace = torch.empty(lib().scn_grad_norm_workspace_bytes(), dtype=torch.uint8, device=self.device)
 
     def grad_norm(self):
-        """The 2-norm of all gradients as a float32 tensor [1] that this object owns."""
+        """The 2-norm of all gradients as a float32 tensor of no dimensions that this object owns."""
         _here(self.device)
         check(lib().scn_grad_norm(self.list, self.count, self._norm.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(),
                                   torch.cuda.current_stream().cuda_stream))

@@ -5,24 +5,73 @@
 namespace scn {
 namespace {
 
-// out[i][c] = scale * table[tokens[i]][c]; no row for a token outside [0, vocab).
-template <class T, class O>
-__global__ void k_embedding_forward(const T *table, int vocab, int C, const int *tokens, long long n, float scale, O *out, long long stride, int *errors) {
-  const long long total = n * C;
-  for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
-    const long long i = e / C;
-    const int c = (int)(e - i * C), t = tokens[i];
-    float v = 0.f;
-    if (t >= 0 && t < vocab) v = to_float(table[(long long)t * C + c]) * scale;
-    else if (t >= vocab && errors && c == 0) atomicOr(errors, SCN_DEV_ERR_KEY);
-    out[i * stride + c] = from_float<O>(v);
+constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_LANES = 64;
+
+// out[i][c] = scale * table[tokens[i]][c]; a zero row for a token outside [0, vocab).  Groups of `lanes` threads take a row, W
+// columns a thread at a time, LOOKUP_ROWS rows at once so that as many table rows are on their way; the output, which is
+// not read again here, is stored past the caches' reach of the table.
+constexpr int LOOKUP_ROWS = 4;
+template <class T, class O, int W>
+__global__ void __launch_bounds__(THREADS) k_embedding_forward(const T *__restrict__ table, int vocab, int C, const int *__restrict__ tokens, long long n, float scale,
+                                                               O *__restrict__ out, long long stride, int lanes, int groups, int *errors) {
+  constexpr int V = W * sizeof(O) > 16 ? 16 / (int)sizeof(O) : W; // values a store
+  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = C / W;
+  if (group >= groups) return;
+  const long long step = (long long)gridDim.x * groups * LOOKUP_ROWS;
+  for (long long i = (long long)blockIdx.x * groups * LOOKUP_ROWS + group; i < n; i += step) {
+    int t[LOOKUP_ROWS];
+#pragma unroll
+    for (int u = 0; u < LOOKUP_ROWS; ++u) {
+      t[u] = i + u * groups < n ? __ldg(tokens + i + u * groups) : -1;
+      if (t[u] >= vocab) {
+        if (lane == 0 && errors) atomicOr(errors, SCN_DEV_ERR_KEY);
+        t[u] = -1;
+      }
+    }
+    for (int v = lane; v < vectors; v += lanes) {
+      Pack<T, W> from[LOOKUP_ROWS];
+#pragma unroll
+      for (int u = 0; u < LOOKUP_ROWS; ++u)
+        if (t[u] >= 0) from[u] = load_pack<T, W>(table + (long long)t[u] * C + v * W);
+#pragma unroll
+      for (int u = 0; u < LOOKUP_ROWS; ++u) {
+        if (i + u * groups >= n) break;
+        O *to = out + (i + u * groups) * stride + v * W;
+#pragma unroll
+        for (int w = 0; w < W; w += V) {
+          Pack<O, V> o;
+#pragma unroll
+          for (int k = 0; k < V; ++k) o.v[k] = from_float<O>(t[u] >= 0 ? to_float(from[u].v[w + k]) * scale : 0.f);
+          __stcs((typename Raw<V * (int)sizeof(O)>::type *)(to + w), o.raw);
+        }
+      }
+    }
   }
+}
+// Threads of a group for rows of so many W-value pieces: all of them at once up to MAX_LANES, else in equal turns.
+int lanes_for(int vectors) {
+  const int turns = (vectors + MAX_LANES - 1) / MAX_LANES;
+  return (vectors + turns - 1) / turns;
+}
+template <class T, class O> void launch_forward(const T *table, int vocab, int C, const int *tokens, long long n, float scale, O *out, long long stride,
+                                                int *errors, cudaStream_t s) {
+  // the widest access that addresses, width and stride allow: at most 16 bytes of the table
+  constexpr int MOST = 16 / (int)sizeof(T);
+  int W = MOST;
+  while (W > 1 && !(C % W == 0 && stride % W == 0 && (uintptr_t)table % (W * sizeof(T)) == 0 && (uintptr_t)out % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
+  const int lanes = lanes_for(C / W), groups = THREADS / lanes;
+  const long long rows = (long long)groups * LOOKUP_ROWS;
+  const int grid = (int)std::min((n + rows - 1) / rows, 64ll * sm_count());
+  if (W == MOST) k_embedding_forward<T, O, MOST><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+  else if (W == 1) k_embedding_forward<T, O, 1><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+  else if (W == MOST / 2) k_embedding_forward<T, O, MOST / 2><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+  else k_embedding_forward<T, O, 2><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
 }
 
 // ------------------------------------------------------------------ stable radix sort of (token, row)
 // Digits of at most MAX_DIGIT bits, least significant first; per pass: digit counts of each tile, their running sums
 // over the tiles, and the scatter.  A tile is TILE consecutive entries, a warp of it WARP_ITEMS consecutive ones.
-constexpr int THREADS = 256, WARPS = THREADS / 32, ROUNDS = 16, TILE = THREADS * ROUNDS, WARP_ITEMS = 32 * ROUNDS, MAX_DIGIT = 10;
+constexpr int ROUNDS = 16, TILE = THREADS * ROUNDS, WARP_ITEMS = 32 * ROUNDS, MAX_DIGIT = 10;
 
 struct Pass {
   const int *tokens;         // first pass: the caller's tokens (row = index), else null
@@ -127,35 +176,159 @@ __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
   }
 }
 
-// One warp a table row: its tokens' rows lie together in the sorted order.
-__device__ __forceinline__ int lower_bound(const unsigned *keys, int n, unsigned t) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (keys[mid] < t) lo = mid + 1; else hi = mid;
+// ------------------------------------------------------------------ sums of the sorted rows
+// A tile of the sorted entries goes to one CTA (times column slabs): groups of `lanes` threads, W columns a thread, take
+// equal runs of it one after the other and add the rows up in registers.  A run's tokens that lie between its first and
+// its last are complete and go straight to the table; what is left of its first and last token is joined over the CTA in
+// shared memory, and what is left of the tile's first and last token over the tiles by k_embedding_join.  So a token's
+// rows are added in an order that depends on the sorted tokens alone, a token on most of the rows costs no more than
+// others, and each table row is written once.
+constexpr int SUM_UNROLL = 8, MAX_TILE = 2048;
+struct Sums {
+  const unsigned *keys, *rows; // sorted
+  int n, vocab, C, tile;       // tile: entries a CTA
+  long long stride;            // of dout's rows
+  int lanes, groups;           // threads of a group, groups of a CTA; a slab is lanes * W columns
+  float scale;
+  int accumulate;
+  float *dtable;
+  float *head, *tail;          // [tiles][C]: the part of a tile's first (last) token, where that began (goes on) in another tile
+};
+template <int W> __device__ __forceinline__ void write_row(const Sums &p, unsigned key, int c, const float (&sum)[W]) {
+  float *to = p.dtable + (long long)key * p.C + c;
+#pragma unroll
+  for (int w = 0; w < W; w += (W < 4 ? W : 4)) {
+    constexpr int V = W < 4 ? W : 4;
+    Pack<float, V> o;
+    if (p.accumulate) o.raw = *(typename Raw<V * 4>::type *)(to + w);
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = p.accumulate ? o.v[k] + p.scale * sum[w + k] : p.scale * sum[w + k];
+    *(typename Raw<V * 4>::type *)(to + w) = o.raw;
   }
-  return lo;
 }
-template <class T>
-__global__ void __launch_bounds__(THREADS) k_embedding_backward(const unsigned *keys, const unsigned *rows, int n, const T *dout, long long stride, int vocab,
-                                                                int C, float scale, int accumulate, float *dtable) {
-  const int t = blockIdx.x * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= vocab) return;
-  const int first = lower_bound(keys, n, t), last = lower_bound(keys, n, t + 1u);
-  if (accumulate && first == last) return;
-  for (int c = lane; c < C; c += 32) {
-    float sum = 0.f;
-    for (int i = first; i < last; ++i) sum += to_float(dout[rows[i] * stride + c]);
-    float *to = dtable + (long long)t * C + c;
-    *to = accumulate ? *to + scale * sum : scale * sum;
+template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding_sums(const Sums p, const T *dout) {
+  extern __shared__ unsigned mem[];
+  unsigned *key = mem, *row = key + p.tile, *itemKey = row + p.tile; // items: each group's first and last token's sums
+  float *item = (float *)(itemKey + 2 * p.groups);
+  const int first = blockIdx.x * p.tile, count = min(p.tile, p.n - first), width = p.lanes * W, column0 = blockIdx.y * width;
+  for (int i = threadIdx.x; i < count; i += THREADS) { key[i] = p.keys[first + i]; row[i] = p.rows[first + i]; }
+  const unsigned none = p.vocab; // the key of rows without a token: behind all others
+  for (int i = threadIdx.x; i < 2 * p.groups; i += THREADS) itemKey[i] = none;
+  __syncthreads();
+  const int group = threadIdx.x / p.lanes, lane = threadIdx.x - group * p.lanes, c = column0 + lane * W;
+  if (group < p.groups && c < p.C) {
+    const int each = (count + p.groups - 1) / p.groups, begin = min(group * each, count), end = min(begin + each, count);
+    float sum[W];
+    unsigned now = begin < end ? key[begin] : none;
+    bool atHead = true;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum[w] = 0.f;
+    for (int i = begin; i < end && key[i] != none; i += SUM_UNROLL) {
+      Pack<T, W> v[SUM_UNROLL];
+      unsigned k[SUM_UNROLL];
+#pragma unroll
+      for (int u = 0; u < SUM_UNROLL; ++u) {
+        k[u] = i + u < end ? key[i + u] : none;
+        if (k[u] != none) v[u] = load_pack<T, W>(dout + row[i + u] * p.stride + c);
+      }
+#pragma unroll
+      for (int u = 0; u < SUM_UNROLL; ++u) {
+        if (k[u] == none) break;
+        if (k[u] != now) {
+          if (atHead) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) item[2 * group * width + lane * W + w] = sum[w];
+            if (lane == 0) itemKey[2 * group] = now;
+            atHead = false;
+          } else write_row<W>(p, now, c, sum);
+          now = k[u];
+#pragma unroll
+          for (int w = 0; w < W; ++w) sum[w] = 0.f;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum[w] += to_float(v[u].v[w]);
+      }
+    }
+    if (now != none) {
+      const int at = 2 * group + (atHead ? 0 : 1);
+#pragma unroll
+      for (int w = 0; w < W; ++w) item[at * width + lane * W + w] = sum[w];
+      if (lane == 0) itemKey[at] = now;
+    }
   }
+  __syncthreads();
+  if (count <= 0) return;
+  const unsigned before = first > 0 ? p.keys[first - 1] : none, after = first + count < p.n ? p.keys[first + count] : none;
+  for (int x = threadIdx.x; x < width && column0 + x < p.C; x += THREADS) {
+    unsigned now = none;
+    float sum[1] = {0.f};
+    for (int j = 0; j <= 2 * p.groups; ++j) {
+      const unsigned k = j < 2 * p.groups ? itemKey[j] : none;
+      if (k == none && j < 2 * p.groups) continue;
+      if (k != now) {
+        if (now != none) {
+          if (now == before) p.head[(long long)blockIdx.x * p.C + column0 + x] = sum[0];
+          else if (now == after) p.tail[(long long)blockIdx.x * p.C + column0 + x] = sum[0];
+          else write_row<1>(p, now, column0 + x, sum);
+        }
+        now = k;
+        sum[0] = 0.f;
+      }
+      if (j < 2 * p.groups) sum[0] += item[j * width + x];
+    }
+  }
+}
+// One CTA a tile (times 32-column slabs): if the tile's last token begins in it and goes on, its parts are added up, every
+// WARPS-th one by a warp, then over the warps.
+__global__ void __launch_bounds__(THREADS) k_embedding_join(const Sums p, int tiles) {
+  const int b = blockIdx.x, first = b * p.tile, end = first + p.tile;
+  if (end >= p.n) return;
+  const unsigned k = p.keys[end - 1];
+  if (k == (unsigned)p.vocab || p.keys[end] != k || (first > 0 && p.keys[first - 1] == k)) return;
+  __shared__ float part[WARPS][32];
+  int last = b + 1; // the first tile behind that does not begin with k
+  for (;;) {
+    const int t = last + threadIdx.x;
+    const int off = __syncthreads_count(t < tiles && p.keys[(long long)t * p.tile] == k);
+    last += off;
+    if (off < THREADS) break;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int c0 = blockIdx.y * 32; c0 < p.C; c0 += gridDim.y * 32) {
+    float sum[1] = {0.f};
+    if (c0 + lane < p.C) {
+#pragma unroll 8
+      for (int t = b + warp; t < last; t += WARPS) sum[0] += (t == b ? p.tail : p.head)[(long long)t * p.C + c0 + lane];
+    }
+    part[warp][lane] = sum[0];
+    __syncthreads();
+    if (warp == 0 && c0 + lane < p.C) {
+      for (int w = 1; w < WARPS; ++w) sum[0] += part[w][lane];
+      write_row<1>(p, k, c0 + lane, sum);
+    }
+    __syncthreads();
+  }
+}
+
+// Values a thread takes at once: what the addresses, widths and strides of dout and the table allow, up to 16 bytes of dout.
+int pack_width(int type, const void *dout, long long stride, const float *dtable, int C) {
+  const int size = type_bytes(type);
+  for (int W = 16 / size; W > 1; W /= 2)
+    if (C % W == 0 && stride % W == 0 && (uintptr_t)dout % (W * size) == 0 && (uintptr_t)dtable % (4 * std::min(W, 4)) == 0) return W;
+  return 1;
+}
+// Entries a CTA sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than four CTAs each.
+int sum_tile(long long n) {
+  int tile = MAX_TILE;
+  while (tile > 64 && n / tile < 4 * 148) tile /= 2;
+  return tile;
 }
 
 struct SortPlan {
   int tiles, passes, digit;           // digit: bits a pass (the last one may have fewer)
-  size_t array, counts, totals, total; // bytes
+  size_t array, counts, totals, parts, total; // bytes
 };
-SortPlan plan_sort(long long n, int vocab) {
+SortPlan plan_sort(long long n, int vocab, int C) {
   SortPlan p;
   int bits = 1;
   while (bits < 31 && ((long long)vocab >> bits) > 0) ++bits; // keys 0..vocab
@@ -165,7 +338,8 @@ SortPlan plan_sort(long long n, int vocab) {
   p.array = align_up(sizeof(unsigned) * (size_t)n, 256);
   p.counts = align_up(sizeof(unsigned) * ((size_t)p.tiles << p.digit), 256);
   p.totals = align_up(sizeof(unsigned) << p.digit, 256);
-  p.total = 4 * p.array + p.counts + p.totals + 256;
+  p.parts = align_up(sizeof(float) * (size_t)((n + sum_tile(n) - 1) / sum_tile(n)) * (size_t)C, 256); // of each tile's first and last token
+  p.total = 4 * p.array + p.counts + p.totals + 2 * p.parts + 256;
   return p;
 }
 
@@ -182,16 +356,15 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
   if (!type_known(table_type) || !type_known(out_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (n == 0) return SCN_OK;
   if (!d_table || !d_tokens || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
-  const int grid = grid_for(n * C, 256);
-  SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, (k_embedding_forward<T, O><<<grid, 256, 0, (cudaStream_t)stream>>>(
-                    (const T *)d_table, vocab, C, d_tokens, n, scale, (O *)d_out, out_stride, d_errors))));
+  SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, launch_forward((const T *)d_table, vocab, C, d_tokens, n, scale, (O *)d_out, out_stride,
+                                                                                 d_errors, (cudaStream_t)stream)));
   SCN_LAUNCH_CHECK("k_embedding_forward");
   return SCN_OK;
 }
 
 extern "C" size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C) {
   if (n < 0 || n > 0x7fffffffll - TILE || vocab < 1 || C < 1) return 0;
-  return plan_sort(n, vocab).total;
+  return plan_sort(n, vocab, C).total;
 }
 
 extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const void *d_dout, int dout_type, long long dout_stride, int vocab, int C,
@@ -203,7 +376,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   if (!type_known(dout_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (!d_dtable || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
   if (n && (!d_tokens || !d_dout)) return fail(SCN_ERR_INVALID, "null pointer");
-  const SortPlan sp = plan_sort(n, vocab);
+  const SortPlan sp = plan_sort(n, vocab, C);
   if (workspace_bytes < sp.total) return fail(SCN_ERR_WORKSPACE, "workspace smaller than scn_embedding_backward_workspace_bytes()");
   if ((uintptr_t)d_workspace & 15) return fail(SCN_ERR_INVALID, "embedding: the workspace must be 16-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
@@ -232,8 +405,32 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     k_radix_scatter<<<p.tiles, THREADS, sizeof(unsigned) * digits * WARPS, s>>>(p);
     SCN_LAUNCH_CHECK("k_radix_scatter");
   }
-  SCN_DISPATCH_TYPE(dout_type, T, (k_embedding_backward<T><<<(vocab + WARPS - 1) / WARPS, THREADS, 0, s>>>(p.keysOut, p.rowsOut, (int)n, (const T *)d_dout,
-                    dout_stride, vocab, C, scale, accumulate, d_dtable)));
-  SCN_LAUNCH_CHECK("k_embedding_backward");
+  const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W, slabs = (vectors + MAX_LANES - 1) / MAX_LANES;
+  Sums q = {};
+  q.keys = p.keysOut; q.rows = p.rowsOut;
+  q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = dout_stride;
+  q.lanes = lanes_for(vectors);
+  q.groups = THREADS / q.lanes;
+  q.tile = sum_tile(n);
+  q.scale = scale; q.accumulate = accumulate; q.dtable = d_dtable;
+  q.head = (float *)(w + 4 * sp.array + sp.counts + sp.totals);
+  q.tail = (float *)(w + 4 * sp.array + sp.counts + sp.totals + sp.parts);
+  const int tiles = (int)((n + q.tile - 1) / q.tile);
+  if (!accumulate) SCN_CUDA_TRY(cudaMemsetAsync(d_dtable, 0, sizeof(float) * (size_t)vocab * C, s));
+  const size_t smem = 4ull * (2 * q.tile + 2 * q.groups) + 4ull * 2 * q.groups * q.lanes * W;
+  const dim3 grid(tiles, slabs);
+  SCN_DISPATCH_TYPE(dout_type, T, {
+    constexpr int MOST = 16 / (int)sizeof(T);
+    const T *from = (const T *)d_dout;
+    if (W == MOST) k_embedding_sums<T, MOST><<<grid, THREADS, smem, s>>>(q, from);
+    else if (W == MOST / 2) k_embedding_sums<T, MOST / 2><<<grid, THREADS, smem, s>>>(q, from);
+    else if (W == 1) k_embedding_sums<T, 1><<<grid, THREADS, smem, s>>>(q, from);
+    else k_embedding_sums<T, 2><<<grid, THREADS, smem, s>>>(q, from);
+  });
+  SCN_LAUNCH_CHECK("k_embedding_sums");
+  if (tiles > 1) {
+    k_embedding_join<<<dim3(tiles, std::min((C + 31) / 32, 8)), THREADS, 0, s>>>(q, tiles);
+    SCN_LAUNCH_CHECK("k_embedding_join");
+  }
   return SCN_OK;
 }

@@ -17,12 +17,29 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// CALL with T naming the C++ type of a run-time scn_type.
-#define SCN_DISPATCH_TYPE(type, T, CALL)                                                    \
+// W consecutive values as one access of W * sizeof(T) bytes (at most 16), which their address has to be a multiple of.
+template <int BYTES> struct Raw;
+template <> struct Raw<2> { using type = unsigned short; };
+template <> struct Raw<4> { using type = unsigned; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<16> { using type = uint4; };
+template <class T, int W> union Pack {
+  typename Raw<W * (int)sizeof(T)>::type raw;
+  T v[W];
+  __device__ Pack() {}
+};
+template <class T, int W> __device__ __forceinline__ Pack<T, W> load_pack(const T *p) {
+  Pack<T, W> r;
+  r.raw = __ldg((const typename Raw<W * (int)sizeof(T)>::type *)p);
+  return r;
+}
+
+// The statements with T naming the C++ type of a run-time scn_type.
+#define SCN_DISPATCH_TYPE(type, T, ...)                                                     \
   switch (type) {                                                                           \
-  case SCN_BF16: { using T = __nv_bfloat16; CALL; } break;                                  \
-  case SCN_F16: { using T = __half; CALL; } break;                                          \
-  default: { using T = float; CALL; } break;                                                \
+  case SCN_BF16: { using T = __nv_bfloat16; __VA_ARGS__; } break;                                  \
+  case SCN_F16: { using T = __half; __VA_ARGS__; } break;                                          \
+  default: { using T = float; __VA_ARGS__; } break;                                                \
   }
 
 } // namespace scn
