@@ -34,6 +34,28 @@ template <class T, int W> __device__ __forceinline__ Pack<T, W> load_pack(const 
   return r;
 }
 
+// Eight consecutive values, 32-byte (float), 16-byte (16-bit) aligned, as one access.
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]),
+               "f"(x[6]), "f"(x[7]) : "memory");
+}
+template <class T> __device__ __forceinline__ void load8_16(const T *p, float (&x)[8]) {
+  Pack<T, 8> r;
+  r.raw = *(const uint4 *)p;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = to_float(r.v[k]);
+}
+template <class T> __device__ __forceinline__ void store8_16(T *p, const float (&x)[8]) {
+  Pack<T, 8> r;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) r.v[k] = from_float<T>(x[k]);
+  *(uint4 *)p = r.raw;
+}
+
 // The statements with T naming the C++ type of a run-time scn_type.
 #define SCN_DISPATCH_TYPE(type, T, ...)                                                     \
   switch (type) {                                                                           \
