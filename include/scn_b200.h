@@ -477,7 +477,7 @@ int scn_embedding_backward(const int *d_tokens, long long n, const void *d_dout,
  *     m  = beta1 m + (1 - beta1) g'
  *     v  = beta2 v + (1 - beta2) g' g'
  *     w  = max(w_min, w - lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay w))
- * in 32 bits; w_min = -INFINITY: no bound. */
+ * in 32 bits; w_min = -INFINITY: no bound.  The root of a v below 2^-126 (gradients around 1e-18 and less) counts as 0. */
 #define SCN_ADAMW_MAX_TENSORS 320
 #define SCN_ADAMW_BLOCK 256
 
@@ -501,7 +501,7 @@ typedef struct {
 } scn_adamw_tensor_t;
 
 typedef struct {
-  double lr, beta1, beta2, eps; /* 0 <= beta < 1, eps > 0                                             */
+  double lr, beta1, beta2, eps; /* 0 <= beta < 1, eps >= 2^-126                                       */
   double grad_scale;            /* 1 / batch size for the sums over a batch that the layers give, say */
   double max_norm;              /* > 0: clip to this norm (needs d_norm); 0: no clipping              */
   long long step;               /* t >= 1                                                             */

@@ -147,7 +147,13 @@ def _ptr(t):
 
 
 def _stream():
-    return c_p(torch.cuda.current_stream().cuda_stream)
+    return c_p(_raw_stream())
+
+
+def _raw_stream():
+    """The current stream of the current device as an integer (what torch.cuda.current_stream().cuda_stream gives, without making the
+    Stream object, which takes longer than a kernel launch)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _i32(t):
@@ -618,7 +624,7 @@ def embedding_forward(table, tokens, scale=1.0, out=None, out_dtype=torch.float3
         raise ScnError("invalid argument: out is on another device")
     optr, otype, stride = _rows_of(out, n, C, "out")
     check(lib().scn_embedding_forward(table.data_ptr(), _TYPES[table.dtype], V, C, ptr, n, scale, optr, otype, stride,
-                                      _optional_i32(errors, dev, "errors"), torch.cuda.current_stream().cuda_stream))
+                                      _optional_i32(errors, dev, "errors"), _raw_stream()))
     return out
 
 
@@ -647,7 +653,7 @@ def embedding_backward(dout, tokens, dtable, scale=1.0, accumulate=False, worksp
         raise ScnError("invalid argument: the workspace must be a uint8 tensor on the other arguments' device")
     check(lib().scn_embedding_backward(ptr, n, dptr, dtype, stride, V, C, scale, int(accumulate), dtable.data_ptr(),
                                        _optional_i32(errors, dev, "errors"), workspace.data_ptr(), workspace.numel(),
-                                       torch.cuda.current_stream().cuda_stream))
+                                       _raw_stream()))
     return dtable
 
 
@@ -725,7 +731,7 @@ class AdamW:
         """The 2-norm of all gradients as a float32 tensor of no dimensions that this object owns."""
         _here(self.device)
         check(lib().scn_grad_norm(self.list, self.count, self._norm.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(),
-                                  torch.cuda.current_stream().cuda_stream))
+                                  _raw_stream()))
         return self._norm
 
     def step(self, lr=None, step=None, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, seed=None, norm=None, max_norm=0.0, scalars=None):
@@ -749,7 +755,7 @@ class AdamW:
         if norm is not None and (norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != self.device):
             raise ScnError("invalid argument: norm must be a float32 tensor of one value on the tensors' device")
         check(lib().scn_adamw_step(self.list, self.count, h, sp, None if norm is None else norm.data_ptr(),
-                                   torch.cuda.current_stream().cuda_stream))
+                                   _raw_stream()))
 
 
 def adamw_decode(codes, scale):
@@ -761,7 +767,7 @@ def adamw_decode(codes, scale):
     _here(codes.device)
     out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
     check(lib().scn_adamw_decode(codes.data_ptr(), scale.data_ptr(), n, int(codes.dtype == torch.uint8), out.data_ptr(),
-                                 torch.cuda.current_stream().cuda_stream))
+                                 _raw_stream()))
     return out
 
 

@@ -8,7 +8,7 @@ namespace scn {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, BLOCK = SCN_ADAMW_BLOCK;
-constexpr int CHUNK = WARPS * BLOCK; // values a CTA takes at a time: one block of 8-bit states a warp
+constexpr int TURN = WARPS * BLOCK; // values a CTA takes at a time: eight a thread, one block of 8-bit states a warp
 constexpr float TOP_M = 127.f * 127.f, TOP_V = 4228250624.f; // the largest codes' values over the scale: 127^2, 255^4 in 32 bits
 
 // The list as the kernel takes it, by value: nothing has to be copied to the device before the launch, and a captured
@@ -29,9 +29,10 @@ struct Tensor {
 template <int CAP> struct List {
   static constexpr int capacity = CAP;
   int count, chunks;
+  int turns; // of a chunk: its CTA takes turns * TURN values
   Tensor t[CAP];
 };
-constexpr int CAP_SMALL = 16, CAP_LARGE = SCN_ADAMW_MAX_TENSORS;
+constexpr int CAP_SMALL = 16, CAP_MEDIUM = 64, CAP_LARGE = SCN_ADAMW_MAX_TENSORS;
 static_assert(sizeof(List<CAP_LARGE>) <= 32000, "a launch takes at most 32764 bytes of parameters");
 
 // The tensor that owns a chunk (tensors without values own none).
@@ -68,17 +69,19 @@ template <int CAP> __global__ void __launch_bounds__(THREADS) k_grad_norm_partia
   double sum = 0;
   for (int chunk = blockIdx.x; chunk < l.chunks; chunk += gridDim.x) {
     const Tensor &t = l.t[owner(l, chunk)];
-    const long long first = (long long)(chunk - t.chunk) * CHUNK;
-    if (t.wide && first + CHUNK <= t.n) {
-      float g[8];
-      load8_typed(t.g, t.gtype, first + threadIdx.x * 8, g);
+    long long first = (long long)(chunk - t.chunk) * l.turns * TURN;
+    for (int turn = 0; turn < l.turns && first < t.n; ++turn, first += TURN) {
+      if (t.wide && first + TURN <= t.n) {
+        float g[8];
+        load8_typed(t.g, t.gtype, first + threadIdx.x * 8, g);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += (double)g[k] * g[k];
-      continue;
-    }
-    for (int j = threadIdx.x; j < CHUNK && first + j < t.n; j += THREADS) {
-      const double g = load_typed(t.g, t.gtype, first + j);
-      sum += g * g;
+        for (int k = 0; k < 8; ++k) sum += (double)g[k] * g[k];
+        continue;
+      }
+      for (int j = threadIdx.x; j < TURN && first + j < t.n; j += THREADS) {
+        const double g = load_typed(t.g, t.gtype, first + j);
+        sum += g * g;
+      }
     }
   }
   dependents_may_launch();
@@ -114,56 +117,82 @@ __device__ __forceinline__ float gradient_scale(const scn_adamw_scalars_t &h, co
   const float clip = h.max_norm > 0.f && total > h.max_norm ? __fdiv_rn(h.max_norm, total) : 1.f;
   return __fmul_rn(h.grad_scale, clip);
 }
+// Two values in one instruction each, as far as there is one: the 8-bit step is bound by the instructions it issues.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 sub(float2 a, float2 b) { return __ffma2_rn(b, both(-1.f), a); }
+__device__ __forceinline__ float root(float x) { // an ulp or so off; 0 below 2^-126
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) { // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // The moments.  Every operation is one rounding (no fused multiply-add), so that the 8-bit codes, which are compared
 // against these values, come out the same in any program that computes the formula in 32 bits.
-__device__ __forceinline__ void moments(const scn_adamw_scalars_t &h, float g, float &m, float &v) {
-  m = __fadd_rn(__fmul_rn(m, h.beta1), __fmul_rn(g, h.one_minus_beta1));
-  v = __fadd_rn(__fmul_rn(v, h.beta2), __fmul_rn(__fmul_rn(g, g), h.one_minus_beta2));
+__device__ __forceinline__ void moments(const scn_adamw_scalars_t &h, float gs, float2 g, float2 &m, float2 &v) {
+  g = mul(g, both(gs));
+  m = add(mul(m, both(h.beta1)), mul(g, both(h.one_minus_beta1)));
+  v = add(mul(v, both(h.beta2)), mul(mul(g, g), both(h.one_minus_beta2)));
 }
-// The parameter's step may use the hardware's approximate root and quotient (an ulp or two of 32 bits): unlike the states it
-// is compared with nothing.  max.NaN keeps a NaN.
-__device__ __forceinline__ float updated(const scn_adamw_scalars_t &h, float w, float m, float v, float decay, float least) {
-  float root, to;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  const float step = fmaf(decay, w, __fdividef(m * h.bias1, fmaf(root, h.bias2, h.eps)));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(to) : "f"(fmaf(-h.lr, step, w)), "f"(least));
-  return to;
+// The parameter's step may use the hardware's approximate root and reciprocal (an ulp or two of 32 bits): unlike the states it
+// is compared with nothing.
+__device__ __forceinline__ float2 updated(const scn_adamw_scalars_t &h, float2 w, float2 m, float2 v, float decay, float least) {
+  const float2 den = __ffma2_rn(make_float2(root(v.x), root(v.y)), both(h.bias2), both(h.eps));
+  const float2 hat = mul(mul(m, both(h.bias1)), make_float2(reciprocal(den.x), reciprocal(den.y)));
+  w = __ffma2_rn(both(-h.lr), __ffma2_rn(both(decay), w, hat), w);
+  return make_float2(max_nan(w.x, least), max_nan(w.y, least));
 }
-// A CTA takes one chunk, a thread eight values of it: everything it reads is on its way before the first is used.
+// A CTA takes one chunk, a thread eight values a turn: everything it reads is on its way before the first is used.
 template <int CAP>
 __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   const Tensor &t = l.t[owner(l, blockIdx.x)];
-  const long long first = (long long)((int)blockIdx.x - t.chunk) * CHUNK;
+  long long first = (long long)((int)blockIdx.x - t.chunk) * l.turns * TURN;
   float *ms = (float *)t.m, *vs = (float *)t.v;
   wait_for_prior_grids();
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
-  if (t.wide && first + CHUNK <= t.n) {
-    const long long i = first + threadIdx.x * 8;
-    float w[8], g[8], m[8], v[8];
-    load8_typed(t.g, t.gtype, i, g);
-    load8(ms + i, m);
-    load8(vs + i, v);
-    load8(t.w + i, w);
+  for (int turn = 0; turn < l.turns && first < t.n; ++turn, first += TURN) {
+    if (t.wide && first + TURN <= t.n) {
+      const long long i = first + threadIdx.x * 8;
+      float w[8], g[8], m[8], v[8];
+      load8_typed(t.g, t.gtype, i, g);
+      load8(ms + i, m);
+      load8(vs + i, v);
+      load8(t.w + i, w);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      moments(h, __fmul_rn(g[k], gs), m[k], v[k]);
-      w[k] = updated(h, w[k], m[k], v[k], t.decay, t.least);
+      for (int k = 0; k < 8; k += 2) {
+        float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
+        moments(h, gs, make_float2(g[k], g[k + 1]), m2, v2);
+        const float2 w2 = updated(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
+        m[k] = m2.x; m[k + 1] = m2.y;
+        v[k] = v2.x; v[k + 1] = v2.y;
+        w[k] = w2.x; w[k + 1] = w2.y;
+      }
+      store8(ms + i, m);
+      store8(vs + i, v);
+      store8(t.w + i, w);
+      if (t.w16) store8_typed(t.w16, t.w16type, i, w);
+      continue;
     }
-    store8(ms + i, m);
-    store8(vs + i, v);
-    store8(t.w + i, w);
-    if (t.w16) store8_typed(t.w16, t.w16type, i, w);
-    return;
-  }
-  for (int j = threadIdx.x; j < CHUNK && first + j < t.n; j += THREADS) {
-    const long long i = first + j;
-    float m = ms[i], v = vs[i];
-    moments(h, __fmul_rn(load_typed(t.g, t.gtype, i), gs), m, v);
-    const float w = updated(h, t.w[i], m, v, t.decay, t.least);
-    ms[i] = m; vs[i] = v; t.w[i] = w;
-    if (t.w16) store_16(t.w16, t.w16type, i, w);
+    for (int j = threadIdx.x; j < TURN && first + j < t.n; j += THREADS) {
+      const long long i = first + j;
+      float2 m = both(ms[i]), v = both(vs[i]);
+      moments(h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
+      const float w = updated(h, both(t.w[i]), m, v, t.decay, t.least).x;
+      ms[i] = m.x; vs[i] = v.x; t.w[i] = w;
+      if (t.w16) store_16(t.w16, t.w16type, i, w);
+    }
   }
 }
 
@@ -177,28 +206,31 @@ __device__ __forceinline__ int scale_exponent(float most, float top, int bits) {
   e = max(e, -126);
   return most > top * power_of_two(e) ? e + 1 : e;
 }
-__device__ __forceinline__ float square(float q) { return __fmul_rn(q, q); }
-__device__ __forceinline__ float fourth(float q) { return square(square(q)); }
-__device__ __forceinline__ float root(float x) {
-  float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // floor(r) for 0 <= r < 2^22, of an r made a little smaller first, so that an approximate root never comes out too large:
 // adding 2^23 with rounding down leaves the whole part.
-__device__ __forceinline__ float floor_below(float r) { return __fadd_rd(r * (1.f - 0x1p-20f), 8388608.f) - 8388608.f; }
-// Largest whole q with power(q) <= x (the comparison decides; floor_below is right or one too small), then one more where
-// the dither says so.
-__device__ __forceinline__ float code_m(float x, float u) {
-  float q = floor_below(root(x));
-  if (square(q + 1.f) <= x) q += 1.f;
-  return __fsub_rn(x, square(q)) > __fmul_rn(u, 2.f * q + 1.f) ? q + 1.f : q;
+__device__ __forceinline__ float2 floor_below(float2 r) { return add(__fadd2_rd(mul(r, both(1.f - 0x1p-20f)), both(8388608.f)), both(-8388608.f)); }
+// Largest whole q with q^2 <= x (the comparison decides; floor_below is right or one too small), then one more where
+// the dither says so.  (x - q^2 and 2 q + 1 are exact.)
+__device__ __forceinline__ float2 code_m(float2 x, float2 u) {
+  float2 q = floor_below(make_float2(root(x.x), root(x.y)));
+  const float2 next = add(q, both(1.f)), square = mul(next, next);
+  q.x = square.x <= x.x ? next.x : q.x;
+  q.y = square.y <= x.y ? next.y : q.y;
+  const float2 over = sub(x, mul(q, q)), limit = mul(u, __ffma2_rn(q, both(2.f), both(1.f)));
+  if (over.x > limit.x) q.x += 1.f;
+  if (over.y > limit.y) q.y += 1.f;
+  return q;
 }
-__device__ __forceinline__ float code_v(float y, float u) {
-  float q = floor_below(root(root(y)));
-  if (fourth(q + 1.f) <= y) q += 1.f;
-  const float low = fourth(q);
-  return __fsub_rn(y, low) > __fmul_rn(u, __fsub_rn(fourth(q + 1.f), low)) ? q + 1.f : q;
+__device__ __forceinline__ float2 fourth(float2 q) { q = mul(q, q); return mul(q, q); }
+__device__ __forceinline__ float2 code_v(float2 y, float2 u) {
+  float2 q = floor_below(make_float2(root(root(y.x)), root(root(y.y))));
+  const float2 next = add(q, both(1.f)), power = fourth(next);
+  q.x = power.x <= y.x ? next.x : q.x;
+  q.y = power.y <= y.y ? next.y : q.y;
+  const float2 low = fourth(q), over = sub(y, low), limit = mul(u, sub(fourth(add(q, both(1.f))), low));
+  if (over.x > limit.x) q.x += 1.f;
+  if (over.y > limit.y) q.y += 1.f;
+  return q;
 }
 // A 32-bit mix of a position and the seed: multiplications by odd numbers (the fractional bits of the square roots of 2, 3,
 // 5 and 7) between shifts that bring the high bits down.
@@ -210,20 +242,21 @@ __device__ __forceinline__ unsigned mix(unsigned at, unsigned key) {
   h *= 0x3C6EF373u;
   return h ^ h >> 16;
 }
-// (b + 1/2) / 2^16 of the 16 bits at bit 7 of x: they become the upper bits of a fraction of 1.
-__device__ __forceinline__ float dither(unsigned x) { return __uint_as_float((x & 0x7FFF80u) | 0x3F800000u) - (1.f - 0x1p-17f); }
-__device__ __forceinline__ float decode_m(int q, float s) { return __fmul_rn((float)(q * abs(q)), s); }
-__device__ __forceinline__ float decode_v(int q, float s) { return __fmul_rn(fourth((float)q), s); }
-// Byte k of a word as a float: the byte in the low bits of 2^23, less 2^23.
-template <int K> __device__ __forceinline__ float byte_of(unsigned word) { return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + K)) - 8388608.f; }
-template <int K> __device__ __forceinline__ float signed_byte_of(unsigned word) { // word: with every sign bit turned over
-  return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + K)) - 8388736.f;
+// (b + 1/2) / 2^16 of the 16 bits at bit 7 of x and of y: they become the upper bits of fractions of 1.
+__device__ __forceinline__ float2 dither(unsigned x, unsigned y) {
+  return add(make_float2(__uint_as_float((x & 0x7FFF80u) | 0x3F800000u), __uint_as_float((y & 0x7FFF80u) | 0x3F800000u)), both(0x1p-17f - 1.f));
 }
-template <int K> __device__ __forceinline__ void decode4(unsigned mq, unsigned vq, float sm, float sv, float *m, float *v) {
-  const float a = signed_byte_of<K>(mq), b = byte_of<K>(vq);
-  m[K] = __fmul_rn(__fmul_rn(a, fabsf(a)), sm);
-  v[K] = __fmul_rn(fourth(b), sv);
+// Bytes K and K + 1 of a word as floats: the byte in the low bits of 2^23, less 2^23 (less 2^23 + 128 where every sign bit
+// has been turned over).
+template <int K> __device__ __forceinline__ float2 bytes_of(unsigned word, float base) {
+  return add(make_float2(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + K)), __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7651 + K))), both(-base));
 }
+constexpr float UNSIGNED = 8388608.f, SIGNED = 8388736.f;
+template <int K> __device__ __forceinline__ float2 decode_m(unsigned word, float s) {
+  const float2 q = bytes_of<K>(word, SIGNED);
+  return mul(make_float2(__fmul_rn(q.x, fabsf(q.x)), __fmul_rn(q.y, fabsf(q.y))), both(s));
+}
+template <int K> __device__ __forceinline__ float2 decode_v(unsigned word, float s) { return mul(fourth(bytes_of<K>(word, UNSIGNED)), both(s)); }
 
 // A warp takes one block, a lane eight consecutive values of it.  Values behind the end of the tensor count as zeros.
 // The largest |m| and v are found as whole numbers: the bits of floats that are not negative are in the floats' order, and what
@@ -233,92 +266,102 @@ template <int CAP>
 __global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   const Tensor &t = l.t[owner(l, blockIdx.x)];
   const int lane = threadIdx.x & 31;
-  const long long block = (long long)((int)blockIdx.x - t.chunk) * WARPS + (threadIdx.x >> 5), i = block * BLOCK + lane * 8;
-  if (block * BLOCK >= t.n) return;
+  long long block = (long long)((int)blockIdx.x - t.chunk) * l.turns * WARPS + (threadIdx.x >> 5);
   signed char *mq = (signed char *)t.m;
   unsigned char *vq = (unsigned char *)t.v;
   wait_for_prior_grids();
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
-  const bool wide = t.wide && (block + 1) * BLOCK <= t.n;
-  float w[8], g[8], m[8], v[8];
-  uint2 mw = {0, 0}, vw = {0, 0};
-  const float sm = t.ms[block], sv = t.vs[block];
-  if (wide) {
-    load8_typed(t.g, t.gtype, i, g);
-    mw = *(const uint2 *)(mq + i);
-    vw = *(const uint2 *)(vq + i);
-    load8(t.w + i, w);
-  } else {
+  for (int turn = 0; turn < l.turns && block * BLOCK < t.n; ++turn, block += WARPS) {
+    const long long i = block * BLOCK + lane * 8;
+    const bool wide = t.wide && (block + 1) * BLOCK <= t.n;
+    float w[8], g[8];
+    unsigned mw[2], vw[2];
+    const float sm = t.ms[block], sv = t.vs[block];
+    if (wide) {
+      load8_typed(t.g, t.gtype, i, g);
+      const uint2 a = *(const uint2 *)(mq + i), b = *(const uint2 *)(vq + i);
+      load8(t.w + i, w);
+      mw[0] = a.x; mw[1] = a.y; vw[0] = b.x; vw[1] = b.y;
+    } else {
+      mw[0] = mw[1] = vw[0] = vw[1] = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = i + k < t.n;
+        g[k] = in ? load_typed(t.g, t.gtype, i + k) : 0.f;
+        w[k] = in ? t.w[i + k] : 0.f;
+        mw[k / 4] |= (in ? (unsigned)(unsigned char)mq[i + k] : 0u) << (k % 4 * 8);
+        vw[k / 4] |= (in ? (unsigned)vq[i + k] : 0u) << (k % 4 * 8);
+      }
+    }
+    float2 m[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned turned = mw[k] ^ 0x80808080u;
+      m[2 * k] = decode_m<0>(turned, sm); m[2 * k + 1] = decode_m<2>(turned, sm);
+      v[2 * k] = decode_v<0>(vw[k], sv); v[2 * k + 1] = decode_v<2>(vw[k], sv);
+    }
+    unsigned mostM = 0, mostV = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      moments(h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
+      const float2 to = updated(h, make_float2(w[2 * k], w[2 * k + 1]), m[k], v[k], t.decay, t.least);
+      w[2 * k] = to.x; w[2 * k + 1] = to.y;
+      if (!wide) { // (a NaN scale would reach the values behind the end)
+        if (i + 2 * k >= t.n) m[k].x = v[k].x = 0.f;
+        if (i + 2 * k + 1 >= t.n) m[k].y = v[k].y = 0.f;
+      }
+      mostM = max(mostM, max(__float_as_uint(fabsf(m[k].x)), __float_as_uint(fabsf(m[k].y))));
+      mostV = max(mostV, max(__float_as_uint(v[k].x), __float_as_uint(v[k].y)));
+    }
+    if (wide) {
+      store8(t.w + i, w);
+      if (t.w16) store8_typed(t.w16, t.w16type, i, w);
+    }
+    mostM = __reduce_max_sync(~0u, mostM);
+    mostV = __reduce_max_sync(~0u, mostV);
+    const bool lost = max(mostM, mostV) >= NOT_FINITE;
+    const int em = lost ? 0 : scale_exponent(__uint_as_float(mostM), TOP_M, 13), ev = lost ? 0 : scale_exponent(__uint_as_float(mostV), TOP_V, 31);
+    if (lane == 0) {
+      t.ms[block] = lost ? __uint_as_float(0x7FFFFFFFu) : mostM ? power_of_two(em) : 0.f;
+      t.vs[block] = lost ? __uint_as_float(0x7FFFFFFFu) : mostV ? power_of_two(ev) : 0.f;
+    }
+    const float im = power_of_two(-em), iv = power_of_two(-ev);
+    const unsigned long long at0 = (t.block + block) * BLOCK;
+    const unsigned at = (unsigned)at0 + lane * 8, key = h.seed * 0xBB67AE85u + (unsigned)(at0 >> 32) * 0xA54FF53Bu;
     unsigned mb[8], vb[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool in = i + k < t.n;
-      g[k] = in ? load_typed(t.g, t.gtype, i + k) : 0.f;
-      w[k] = in ? t.w[i + k] : 0.f;
-      mb[k] = in ? (unsigned char)mq[i + k] : 0u;
-      vb[k] = in ? vq[i + k] : 0u;
+    for (int k = 0; k < 4; ++k) {
+      const unsigned r = mix(at + 2 * k, key), s = mix(at + 2 * k + 1, key);
+      float2 qm = code_m(make_float2(__fmul_rn(fabsf(m[k].x), im), __fmul_rn(fabsf(m[k].y), im)), dither(r << 7, s << 7));
+      float2 qv = code_v(mul(v[k], both(iv)), dither(r >> 9, s >> 9));
+      if (v[k].x > 0.f) qv.x = fmaxf(qv.x, 1.f);
+      if (v[k].y > 0.f) qv.y = fmaxf(qv.y, 1.f);
+      qm = add(make_float2(copysignf(qm.x, m[k].x), copysignf(qm.y, m[k].y)), both(SIGNED)); // the bytes in the low bits again
+      qv = add(qv, both(UNSIGNED));
+      mb[2 * k] = __float_as_uint(qm.x); mb[2 * k + 1] = __float_as_uint(qm.y);
+      vb[2 * k] = __float_as_uint(qv.x); vb[2 * k + 1] = __float_as_uint(qv.y);
     }
-    mw = make_uint2(mb[0] | mb[1] << 8 | mb[2] << 16 | mb[3] << 24, mb[4] | mb[5] << 8 | mb[6] << 16 | mb[7] << 24);
-    vw = make_uint2(vb[0] | vb[1] << 8 | vb[2] << 16 | vb[3] << 24, vb[4] | vb[5] << 8 | vb[6] << 16 | vb[7] << 24);
-  }
-  mw.x ^= 0x80808080u; mw.y ^= 0x80808080u;
-  decode4<0>(mw.x, vw.x, sm, sv, m, v); decode4<1>(mw.x, vw.x, sm, sv, m, v);
-  decode4<2>(mw.x, vw.x, sm, sv, m, v); decode4<3>(mw.x, vw.x, sm, sv, m, v);
-  decode4<0>(mw.y, vw.y, sm, sv, m + 4, v + 4); decode4<1>(mw.y, vw.y, sm, sv, m + 4, v + 4);
-  decode4<2>(mw.y, vw.y, sm, sv, m + 4, v + 4); decode4<3>(mw.y, vw.y, sm, sv, m + 4, v + 4);
-  unsigned mostM = 0, mostV = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    moments(h, __fmul_rn(g[k], gs), m[k], v[k]);
-    w[k] = updated(h, w[k], m[k], v[k], t.decay, t.least);
-    if (wide || i + k < t.n) { // (a NaN scale would reach the values behind the end)
-      mostM = max(mostM, __float_as_uint(fabsf(m[k])));
-      mostV = max(mostV, __float_as_uint(v[k]));
-    }
-  }
-  mostM = __reduce_max_sync(~0u, mostM);
-  mostV = __reduce_max_sync(~0u, mostV);
-  const bool lost = max(mostM, mostV) >= NOT_FINITE;
-  const float topM = __uint_as_float(mostM), topV = __uint_as_float(mostV);
-  const int em = lost ? 0 : scale_exponent(topM, TOP_M, 13), ev = lost ? 0 : scale_exponent(topV, TOP_V, 31);
-  if (lane == 0) {
-    t.ms[block] = lost ? __uint_as_float(0x7FFFFFFFu) : mostM ? power_of_two(em) : 0.f;
-    t.vs[block] = lost ? __uint_as_float(0x7FFFFFFFu) : mostV ? power_of_two(ev) : 0.f;
-  }
-  const float im = power_of_two(-em), iv = power_of_two(-ev);
-  const unsigned long long at0 = (t.block + block) * BLOCK;
-  const unsigned at = (unsigned)at0 + lane * 8, key = h.seed * 0xBB67AE85u + (unsigned)(at0 >> 32) * 0xA54FF53Bu;
-  unsigned mb[8], vb[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const unsigned r = mix(at + k, key);
-    float qm = code_m(__fmul_rn(fabsf(m[k]), im), dither(r << 7)), qv = code_v(__fmul_rn(v[k], iv), dither(r >> 9));
-    if (v[k] > 0.f) qv = fmaxf(qv, 1.f);
-    qm = m[k] < 0.f ? -qm : qm;
-    mb[k] = __float_as_uint(qm + 8388736.f) ^ 0x80u; // the byte in the low bits again
-    vb[k] = __float_as_uint(qv + 8388608.f);
-  }
-  if (lost) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) mb[k] = vb[k] = 0;
-  }
-  if (wide) {
     const auto pack = [](const unsigned *b) { return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410); };
-    store8(t.w + i, w);
-    if (t.w16) store8_typed(t.w16, t.w16type, i, w);
-    *(uint2 *)(mq + i) = make_uint2(pack(mb), pack(mb + 4));
-    *(uint2 *)(vq + i) = make_uint2(pack(vb), pack(vb + 4));
-    return;
-  }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (i + k >= t.n) break;
-    t.w[i + k] = w[k];
-    if (t.w16) store_16(t.w16, t.w16type, i + k, w[k]);
-    mq[i + k] = (signed char)mb[k];
-    vq[i + k] = (unsigned char)vb[k];
+    for (int k = 0; k < 2; ++k) {
+      mw[k] = lost ? 0u : pack(mb + 4 * k) ^ 0x80808080u;
+      vw[k] = lost ? 0u : pack(vb + 4 * k);
+    }
+    if (wide) {
+      *(uint2 *)(mq + i) = make_uint2(mw[0], mw[1]);
+      *(uint2 *)(vq + i) = make_uint2(vw[0], vw[1]);
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i + k >= t.n) break;
+      t.w[i + k] = w[k];
+      if (t.w16) store_16(t.w16, t.w16type, i + k, w[k]);
+      mq[i + k] = (signed char)(mw[k / 4] >> (k % 4 * 8));
+      vq[i + k] = (unsigned char)(vw[k / 4] >> (k % 4 * 8));
+    }
   }
 }
 // Four codes a thread where the arrays are aligned for it (`wide`: so many values are), then one by one.
@@ -327,18 +370,13 @@ __global__ void __launch_bounds__(THREADS) k_adamw_decode(const unsigned char *c
   for (long long j = self; j < wide / 4; j += step) {
     const unsigned q = ((const unsigned *)codes)[j];
     const float s = scale[j / (BLOCK / 4)];
-    float4 o;
-    if (second) {
-      o = make_float4(__fmul_rn(fourth(byte_of<0>(q)), s), __fmul_rn(fourth(byte_of<1>(q)), s), __fmul_rn(fourth(byte_of<2>(q)), s), __fmul_rn(fourth(byte_of<3>(q)), s));
-    } else {
-      const unsigned t = q ^ 0x80808080u;
-      const float a = signed_byte_of<0>(t), b = signed_byte_of<1>(t), c = signed_byte_of<2>(t), d = signed_byte_of<3>(t);
-      o = make_float4(__fmul_rn(a * fabsf(a), s), __fmul_rn(b * fabsf(b), s), __fmul_rn(c * fabsf(c), s), __fmul_rn(d * fabsf(d), s));
-    }
-    ((float4 *)out)[j] = o;
+    float2 a, b;
+    if (second) { a = decode_v<0>(q, s); b = decode_v<2>(q, s); }
+    else { a = decode_m<0>(q ^ 0x80808080u, s); b = decode_m<2>(q ^ 0x80808080u, s); }
+    ((float4 *)out)[j] = make_float4(a.x, a.y, b.x, b.y);
   }
   for (long long i = wide + self; i < n; i += step)
-    out[i] = second ? decode_v(codes[i], scale[i / BLOCK]) : decode_m(((const signed char *)codes)[i], scale[i / BLOCK]);
+    out[i] = second ? decode_v<0>(codes[i], scale[i / BLOCK]).x : decode_m<0>(codes[i] ^ 0x80u, scale[i / BLOCK]).x;
 }
 
 // ------------------------------------------------------------------ host side
@@ -366,22 +404,23 @@ bool wide(const scn_adamw_tensor_t &t) {
   const uintptr_t states = (uintptr_t)t.d_m | (uintptr_t)t.d_v;
   return !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 7 : 31));
 }
-// LAUNCH(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.
+// launch(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.  Where one turn a
+// chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes four: it finds its tensor once for all of them.
 template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, Take take, Launch launch) {
   List<CAP> l;
+  long long all = 0;
+  for (int i = 0; i < count; ++i) all += take(t[i]) ? (t[i].n + TURN - 1) / TURN : 0;
+  l.turns = all > 100ll * 148 ? 4 : 1;
+  const long long size = (long long)l.turns * TURN;
   l.count = l.chunks = 0;
   unsigned long long block = 0;
-  auto flush = [&]() -> int {
-    const int rc = l.count ? launch(l) : (int)SCN_OK;
-    l.count = l.chunks = 0;
-    return rc;
-  };
   for (int i = 0; i < count; ++i) {
-    const long long blocks = (t[i].n + BLOCK - 1) / BLOCK, chunks = (t[i].n + CHUNK - 1) / CHUNK;
+    const long long blocks = (t[i].n + BLOCK - 1) / BLOCK, chunks = (t[i].n + size - 1) / size;
     if (t[i].n > 0 && take(t[i])) {
       if (l.count == CAP || l.chunks + chunks > 0x7fffffffll) {
-        const int rc = flush();
+        const int rc = launch(l);
         if (rc != SCN_OK) return rc;
+        l.count = l.chunks = 0;
       }
       l.t[l.count++] = Tensor{t[i].d_w, t[i].d_g, t[i].d_m, t[i].d_v, t[i].d_m_scale, t[i].d_v_scale, t[i].d_w16, t[i].n, block,
                               t[i].weight_decay, t[i].w_min, l.chunks, (short)t[i].g_type, (short)t[i].w16_type, wide(t[i])};
@@ -389,10 +428,13 @@ template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tenso
     }
     block += blocks;
   }
-  return flush();
+  return l.count ? launch(l) : (int)SCN_OK;
 }
+// The parameters' bytes are copied at every launch: the smallest list that holds them all.
 template <class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, Take take, Launch launch) {
-  return count <= CAP_SMALL ? for_lists<CAP_SMALL>(t, count, take, launch) : for_lists<CAP_LARGE>(t, count, take, launch);
+  if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, take, launch);
+  if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, take, launch);
+  return for_lists<CAP_LARGE>(t, count, take, launch);
 }
 int norm_ctas() { return 4 * sm_count(); }
 
@@ -406,7 +448,7 @@ extern "C" int scn_adamw_scalars(const scn_adamw_t *h, scn_adamw_scalars_t *out)
   if (!h || !out) return fail(SCN_ERR_INVALID, "null pointer");
   if (!(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1)) return fail(SCN_ERR_INVALID, "AdamW: beta1 and beta2 must be in [0, 1)");
   if (!std::isfinite(h->lr) || !std::isfinite(h->grad_scale)) return fail(SCN_ERR_INVALID, "AdamW: lr and grad_scale must be finite");
-  if (!(std::isfinite(h->eps) && (float)h->eps > 0.f)) return fail(SCN_ERR_INVALID, "AdamW: eps must be positive in 32 bits");
+  if (!(std::isfinite(h->eps) && (float)h->eps >= 1.17549435e-38f)) return fail(SCN_ERR_INVALID, "AdamW: eps must be a positive normal 32-bit number");
   if (!(std::isfinite(h->max_norm) && h->max_norm >= 0)) return fail(SCN_ERR_INVALID, "AdamW: max_norm must be finite and not negative");
   if (h->step < 1) return fail(SCN_ERR_INVALID, "AdamW: steps count from 1");
   out->lr = (float)h->lr;
@@ -435,7 +477,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
   cudaStream_t s = (cudaStream_t)stream;
   double *partial = (double *)d_workspace;
   const int most = (int)(scn_grad_norm_workspace_bytes() / sizeof(double));
-  int used = 0, launches = (count + (count <= CAP_SMALL ? CAP_SMALL : CAP_LARGE) - 1) / (count <= CAP_SMALL ? CAP_SMALL : CAP_LARGE);
+  int used = 0, launches = (count + CAP_LARGE - 1) / CAP_LARGE;
   if (launches > most) return fail(SCN_ERR_UNSUPPORTED, "AdamW: list too long");
   const int each = std::min(norm_ctas(), most / std::max(launches, 1));
   const int rc = for_lists(tensors, count, [](const scn_adamw_tensor_t &) { return true; }, [&](const auto &l) -> int {

@@ -10,31 +10,35 @@ constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_LANES = 64;
 // out[i][c] = scale * table[tokens[i]][c]; a zero row for a token outside [0, vocab).  Groups of `lanes` threads take a row, W
 // columns a thread at a time, LOOKUP_ROWS rows at once so that as many table rows are on their way; the output, which is
 // not read again here, is stored past the caches' reach of the table.
-constexpr int LOOKUP_ROWS = 4;
-template <class T, class O, int W>
+template <class T, class O, int W, int ROWS>
 __global__ void __launch_bounds__(THREADS) k_embedding_forward(const T *__restrict__ table, int vocab, int C, const int *__restrict__ tokens, long long n, float scale,
                                                                O *__restrict__ out, long long stride, int lanes, int groups, int *errors) {
   constexpr int V = W * sizeof(O) > 16 ? 16 / (int)sizeof(O) : W; // values a store
   const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = C / W;
   if (group >= groups) return;
-  const long long step = (long long)gridDim.x * groups * LOOKUP_ROWS;
-  for (long long i = (long long)blockIdx.x * groups * LOOKUP_ROWS + group; i < n; i += step) {
-    int t[LOOKUP_ROWS];
+  const long long step = (long long)gridDim.x * groups * ROWS;
+  long long i = (long long)blockIdx.x * groups * ROWS + group;
+  int next[ROWS];
 #pragma unroll
-    for (int u = 0; u < LOOKUP_ROWS; ++u) {
-      t[u] = i + u * groups < n ? __ldg(tokens + i + u * groups) : -1;
+  for (int u = 0; u < ROWS; ++u) next[u] = i + u * groups < n ? __ldg(tokens + i + u * groups) : -1;
+  for (; i < n; i += step) {
+    int t[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      t[u] = next[u];
       if (t[u] >= vocab) {
         if (lane == 0 && errors) atomicOr(errors, SCN_DEV_ERR_KEY);
         t[u] = -1;
       }
+      next[u] = i + step + u * groups < n ? __ldg(tokens + i + step + u * groups) : -1; // the next turn's, while this one's rows travel
     }
     for (int v = lane; v < vectors; v += lanes) {
-      Pack<T, W> from[LOOKUP_ROWS];
+      Pack<T, W> from[ROWS];
 #pragma unroll
-      for (int u = 0; u < LOOKUP_ROWS; ++u)
+      for (int u = 0; u < ROWS; ++u)
         if (t[u] >= 0) from[u] = load_pack<T, W>(table + (long long)t[u] * C + v * W);
 #pragma unroll
-      for (int u = 0; u < LOOKUP_ROWS; ++u) {
+      for (int u = 0; u < ROWS; ++u) {
         if (i + u * groups >= n) break;
         O *to = out + (i + u * groups) * stride + v * W;
 #pragma unroll
@@ -60,97 +64,74 @@ template <class T, class O> void launch_forward(const T *table, int vocab, int C
   int W = MOST;
   while (W > 1 && !(C % W == 0 && stride % W == 0 && (uintptr_t)table % (W * sizeof(T)) == 0 && (uintptr_t)out % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
   const int lanes = lanes_for(C / W), groups = THREADS / lanes;
-  const long long rows = (long long)groups * LOOKUP_ROWS;
-  const int grid = (int)std::min((n + rows - 1) / rows, 64ll * sm_count());
-  if (W == MOST) k_embedding_forward<T, O, MOST><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
-  else if (W == 1) k_embedding_forward<T, O, 1><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
-  else if (W == MOST / 2) k_embedding_forward<T, O, MOST / 2><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
-  else k_embedding_forward<T, O, 2><<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+  const auto launch = [&](auto kernel, int rows) {
+    const int grid = (int)std::min((n + groups * rows - 1) / (groups * rows), 16ll * sm_count());
+    kernel<<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+  };
+  // narrow accesses: more rows at once, for as many bytes on their way
+  if (W == MOST) launch(k_embedding_forward<T, O, MOST, 4>, 4);
+  else if (W == 1) launch(k_embedding_forward<T, O, 1, 8>, 8);
+  else if (W == MOST / 2) launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
+  else launch(k_embedding_forward<T, O, 2, 8>, 8);
 }
 
 // ------------------------------------------------------------------ stable radix sort of (token, row)
 // Digits of at most MAX_DIGIT bits, least significant first; per pass: digit counts of each tile, their running sums
-// over the tiles, and the scatter.  A tile is TILE consecutive entries, a warp of it WARP_ITEMS consecutive ones.
-constexpr int ROUNDS = 16, TILE = THREADS * ROUNDS, WARP_ITEMS = 32 * ROUNDS, MAX_DIGIT = 10;
-
+// over the tiles, and the scatter.  A tile is THREADS * ROUNDS consecutive entries, a warp of it 32 * ROUNDS consecutive ones.
+constexpr int MAX_DIGIT = 9;
 struct Pass {
-  const int *tokens;         // first pass: the caller's tokens (row = index), else null
-  const unsigned *keys, *rows;
-  unsigned *keysOut, *rowsOut;
+  const int *tokens;  // first pass: the caller's tokens (row = index), else null
+  const uint2 *in;    // (key, row)
+  uint2 *out;
   int n, vocab, tiles, shift, bits;
-  unsigned *counts;          // [2^bits][tiles]
-  unsigned *totals;          // [2^bits]
+  unsigned *counts;   // [2^bits][tiles]
+  unsigned *totals;   // [2^bits]
   int *errors;
+  float *clear;       // first pass: clearN values to set to zero on the side, or null
+  long long clearN;
 };
 // The token, or vocab (sorted behind all tokens) where it names no row.
-__device__ __forceinline__ unsigned key_of(const Pass &p, int i) {
-  if (!p.tokens) return p.keys[i];
-  const int t = p.tokens[i];
-  return t >= 0 && t < p.vocab ? (unsigned)t : (unsigned)p.vocab;
+__device__ __forceinline__ unsigned key_of(int token, int vocab) { return token >= 0 && token < vocab ? (unsigned)token : (unsigned)vocab; }
+__device__ void clear_floats(float *p, long long n, long long self, long long step) {
+  const long long before = min(n, (long long)(((16 - ((uintptr_t)p & 15)) & 15) / 4)), whole = (n - before) / 4;
+  for (long long i = self; i < whole; i += step) ((float4 *)(p + before))[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (long long i = self; i < n; i += step)
+    if (i >= before && i < before + 4 * whole) i += (before + 4 * whole - i - 1) / step * step; // (only the ends are left)
+    else p[i] = 0.f;
 }
-__global__ void __launch_bounds__(THREADS) k_radix_count(const Pass p) {
+template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_count(const Pass p) {
   extern __shared__ unsigned hist[];
+  wait_for_prior_grids();
+  dependents_may_launch();
+  if ((int)blockIdx.x >= p.tiles) { // the table's zeros, written while the sort's kernels wait for one another
+    clear_floats(p.clear, p.clearN, (long long)(blockIdx.x - p.tiles) * THREADS + threadIdx.x, (long long)(gridDim.x - p.tiles) * THREADS);
+    return;
+  }
   const int digits = 1 << p.bits;
+  const long long first = (long long)blockIdx.x * (THREADS * ROUNDS);
+  unsigned key[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const long long i = first + r * THREADS + threadIdx.x;
+    key[r] = i >= p.n ? 0u : p.tokens ? (unsigned)p.tokens[i] : p.in[i].x;
+  }
   for (int d = threadIdx.x; d < digits; d += THREADS) hist[d] = 0;
   __syncthreads();
-  const int first = blockIdx.x * TILE, last = min(p.n - first, TILE);
-  for (int j = threadIdx.x; j < last; j += THREADS) {
-    if (p.tokens && p.errors && p.tokens[first + j] >= p.vocab) atomicOr(p.errors, SCN_DEV_ERR_KEY);
-    atomicAdd(&hist[(key_of(p, first + j) >> p.shift) & (digits - 1)], 1u);
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    if (first + r * THREADS + threadIdx.x >= p.n) break;
+    if (p.tokens) {
+      if (p.errors && (int)key[r] >= p.vocab) atomicOr(p.errors, SCN_DEV_ERR_KEY);
+      key[r] = key_of((int)key[r], p.vocab);
+    }
+    atomicAdd(&hist[(key[r] >> p.shift) & (digits - 1)], 1u);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += THREADS) p.counts[(long long)d * p.tiles + blockIdx.x] = hist[d];
 }
-// One CTA a digit: counts[d][*] becomes its exclusive running sum, totals[d] its sum.
-__global__ void __launch_bounds__(THREADS) k_radix_scan(const Pass p) {
-  __shared__ unsigned warpSum[WARPS];
-  unsigned *row = p.counts + (long long)blockIdx.x * p.tiles;
+// Running sum over the CTA's threads: what the threads before this one hold; `all`: what all of them hold.
+__device__ __forceinline__ unsigned sum_before(unsigned own, unsigned *warpSum, unsigned &all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned before = 0;
-  for (int base = 0; base < p.tiles; base += THREADS) {
-    const int j = base + threadIdx.x;
-    const unsigned own = j < p.tiles ? row[j] : 0u;
-    unsigned sum = own;
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned v = __shfl_up_sync(~0u, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (lane == 31) warpSum[warp] = sum;
-    __syncthreads();
-    unsigned all = 0, mine = 0;
-    for (int w = 0; w < WARPS; ++w) { if (w == warp) mine = all; all += warpSum[w]; }
-    if (j < p.tiles) row[j] = before + mine + sum - own;
-    before += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) p.totals[blockIdx.x] = before;
-}
-__global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
-  extern __shared__ unsigned mem[];
-  const int digits = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned *count = mem; // [warp][digit]
-  __shared__ unsigned warpSum[WARPS];
-  for (int d = threadIdx.x; d < WARPS * digits; d += THREADS) count[d] = 0;
-  __syncthreads();
-  const int first = blockIdx.x * TILE + warp * WARP_ITEMS;
-  unsigned key[ROUNDS], rank[ROUNDS];
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int i = first + r * 32 + lane;
-    const bool in = i < p.n;
-    key[r] = in ? key_of(p, i) : 0u;
-    const unsigned d = (key[r] >> p.shift) & (digits - 1);
-    const unsigned peers = __match_any_sync(~0u, in ? d : (unsigned)digits);
-    if (in) rank[r] = count[warp * digits + d] + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (in && (peers >> lane) == 1u) count[warp * digits + d] += __popc(peers); // the group's last lane
-    __syncwarp();
-  }
-  __syncthreads();
-  // count becomes each warp's own start: behind the smaller digits, this digit in earlier tiles and in earlier warps
-  const int per = (digits + THREADS - 1) / THREADS, d0 = threadIdx.x * per;
-  unsigned own = 0;
-  for (int d = d0; d < min(digits, d0 + per); ++d) own += p.totals[d];
   unsigned sum = own;
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned v = __shfl_up_sync(~0u, sum, o);
@@ -158,21 +139,115 @@ __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
   }
   if (lane == 31) warpSum[warp] = sum;
   __syncthreads();
-  unsigned at = sum - own;
-  for (int w = 0; w < warp; ++w) at += warpSum[w];
-  for (int d = d0; d < min(digits, d0 + per); ++d) {
-    unsigned s = at + p.counts[(long long)d * p.tiles + blockIdx.x];
-    at += p.totals[d];
-    for (int w = 0; w < WARPS; ++w) { const unsigned c = count[w * digits + d]; count[w * digits + d] = s; s += c; }
+  unsigned before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) { if (w == warp) before = all; all += warpSum[w]; }
+  __syncthreads();
+  return before + sum - own;
+}
+// One CTA a digit: counts[d][*] becomes its exclusive running sum, totals[d] its sum.
+__global__ void __launch_bounds__(THREADS) k_radix_scan(const Pass p) {
+  __shared__ unsigned warpSum[WARPS];
+  wait_for_prior_grids();
+  dependents_may_launch();
+  unsigned *row = p.counts + (long long)blockIdx.x * p.tiles;
+  unsigned before = 0, all;
+  for (int base = 0; base < p.tiles; base += THREADS) {
+    const int j = base + threadIdx.x;
+    const unsigned own = j < p.tiles ? row[j] : 0u, at = sum_before(own, warpSum, all);
+    if (j < p.tiles) row[j] = before + at;
+    before += all;
+  }
+  if (threadIdx.x == 0) p.totals[blockIdx.x] = before;
+}
+// Places of a tile's entries in its order by digit: place[r] of the entry that this thread holds in round r (a warp's entries
+// lie one after the other, a round's in the order of the lanes).  count[WARPS][digits]: scratch; start(d, at, n) is called once
+// for each digit with the place `at` of its first entry and their number n.  Ranks within a round come from one ballot a bit.
+template <int ROUNDS, class Start>
+__device__ __forceinline__ void places_by_digit(const unsigned (&key)[ROUNDS], int inTile, int shift, int bits, unsigned short *count, unsigned *warpSum,
+                                                unsigned (&place)[ROUNDS], Start start) {
+  const int digits = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int d = threadIdx.x; d < WARPS * digits / 2; d += THREADS) ((unsigned *)count)[d] = 0;
+  __syncthreads();
+  unsigned short *own = count + warp * digits;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool in = (warp * ROUNDS + r) * 32 + lane < inTile;
+    const unsigned d = (key[r] >> shift) & (digits - 1);
+    unsigned peers = __ballot_sync(~0u, in);
+    for (int b = 0; b < bits; ++b) {
+      const bool set = d >> b & 1;
+      const unsigned votes = __ballot_sync(~0u, set);
+      peers &= set ? votes : ~votes;
+    }
+    if (in) {
+      const unsigned n = own[d];
+      place[r] = n + __popc(peers & ((1u << lane) - 1));
+      __syncwarp(peers);
+      if (peers >> lane == 1u) own[d] = (unsigned short)(n + __popc(peers)); // the last of the lanes with this digit
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  const int per = (digits + THREADS - 1) / THREADS, d0 = threadIdx.x * per, d1 = min(digits, d0 + per);
+  unsigned sum = 0, all;
+  for (int d = d0; d < d1; ++d)
+    for (int w = 0; w < WARPS; ++w) sum += count[w * digits + d];
+  unsigned at = sum_before(sum, warpSum, all);
+  for (int d = d0; d < d1; ++d) {
+    const unsigned first = at;
+    for (int w = 0; w < WARPS; ++w) {
+      const unsigned n = count[w * digits + d];
+      count[w * digits + d] = (unsigned short)at;
+      at += n;
+    }
+    start(d, first, at - first);
   }
   __syncthreads();
 #pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if ((warp * ROUNDS + r) * 32 + lane < inTile) place[r] += own[(key[r] >> shift) & (digits - 1)];
+}
+// A tile is put in order in shared memory first, so that entries of one digit leave side by side.
+template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
+  extern __shared__ uint2 stage[];
+  constexpr int TILE = THREADS * ROUNDS;
+  const int digits = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned *shift = (unsigned *)(stage + TILE); // [digits]: place in the output less place in the tile
+  unsigned short *count = (unsigned short *)(shift + digits);
+  __shared__ unsigned warpSum[WARPS];
+  wait_for_prior_grids();
+  dependents_may_launch();
+  const long long first = (long long)blockIdx.x * TILE;
+  const int inTile = (int)min((long long)TILE, p.n - first);
+  unsigned key[ROUNDS], row[ROUNDS], place[ROUNDS];
+#pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const int i = first + r * 32 + lane;
-    if (i >= p.n) continue;
-    const unsigned dst = count[warp * digits + ((key[r] >> p.shift) & (digits - 1))] + rank[r];
-    p.keysOut[dst] = key[r];
-    p.rowsOut[dst] = p.tokens ? (unsigned)i : p.rows[i];
+    const int j = (warp * ROUNDS + r) * 32 + lane;
+    key[r] = 0; row[r] = (unsigned)(first + j);
+    if (j < inTile) {
+      if (p.tokens) key[r] = key_of(p.tokens[first + j], p.vocab);
+      else { const uint2 e = p.in[first + j]; key[r] = e.x; row[r] = e.y; }
+    }
+  }
+  // entries of smaller digits, plus those of the digit in earlier tiles
+  const int per = (digits + THREADS - 1) / THREADS, d0 = threadIdx.x * per, d1 = min(digits, d0 + per);
+  unsigned sum = 0, all;
+  for (int d = d0; d < d1; ++d) sum += p.totals[d];
+  unsigned at = sum_before(sum, warpSum, all);
+  for (int d = d0; d < d1; ++d) {
+    shift[d] = at + p.counts[(long long)d * p.tiles + blockIdx.x];
+    at += p.totals[d];
+  }
+  places_by_digit<ROUNDS>(key, inTile, p.shift, p.bits, count, warpSum, place, [&](int d, unsigned start, unsigned) { shift[d] -= start; });
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if ((warp * ROUNDS + r) * 32 + lane < inTile) stage[place[r]] = make_uint2(key[r], row[r]);
+  __syncthreads();
+  for (int j = threadIdx.x; j < inTile; j += THREADS) {
+    const uint2 e = stage[j];
+    p.out[shift[(e.x >> p.shift) & (digits - 1)] + j] = e;
   }
 }
 
@@ -185,7 +260,7 @@ __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
 // others, and each table row is written once.
 constexpr int SUM_UNROLL = 8, MAX_TILE = 2048;
 struct Sums {
-  const unsigned *keys, *rows; // sorted
+  const uint2 *entries;        // (token, row), sorted
   int n, vocab, C, tile;       // tile: entries a CTA
   long long stride;            // of dout's rows
   int lanes, groups;           // threads of a group, groups of a CTA; a slab is lanes * W columns
@@ -206,30 +281,29 @@ template <int W> __device__ __forceinline__ void write_row(const Sums &p, unsign
     *(typename Raw<V * 4>::type *)(to + w) = o.raw;
   }
 }
-template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding_sums(const Sums p, const T *dout) {
-  extern __shared__ unsigned mem[];
-  unsigned *key = mem, *row = key + p.tile, *itemKey = row + p.tile; // items: each group's first and last token's sums
-  float *item = (float *)(itemKey + 2 * p.groups);
-  const int first = blockIdx.x * p.tile, count = min(p.tile, p.n - first), width = p.lanes * W, column0 = blockIdx.y * width;
-  for (int i = threadIdx.x; i < count; i += THREADS) { key[i] = p.keys[first + i]; row[i] = p.rows[first + i]; }
+// The sums of `count` sorted entries in shared memory; before, after: the tokens around them.  items: 2 * groups keys and as
+// many rows of a slab's width.
+template <class T, int W>
+__device__ __forceinline__ void sum_entries(const Sums &p, const T *dout, const uint2 *entry, int count, unsigned before, unsigned after, unsigned *itemKey, float *item) {
   const unsigned none = p.vocab; // the key of rows without a token: behind all others
+  const int width = p.lanes * W, column0 = blockIdx.y * width, group = threadIdx.x / p.lanes, lane = threadIdx.x - group * p.lanes, c = column0 + lane * W;
   for (int i = threadIdx.x; i < 2 * p.groups; i += THREADS) itemKey[i] = none;
   __syncthreads();
-  const int group = threadIdx.x / p.lanes, lane = threadIdx.x - group * p.lanes, c = column0 + lane * W;
   if (group < p.groups && c < p.C) {
     const int each = (count + p.groups - 1) / p.groups, begin = min(group * each, count), end = min(begin + each, count);
     float sum[W];
-    unsigned now = begin < end ? key[begin] : none;
+    unsigned now = begin < end ? entry[begin].x : none;
     bool atHead = true;
 #pragma unroll
     for (int w = 0; w < W; ++w) sum[w] = 0.f;
-    for (int i = begin; i < end && key[i] != none; i += SUM_UNROLL) {
+    for (int i = begin; i < end && entry[i].x != none; i += SUM_UNROLL) {
       Pack<T, W> v[SUM_UNROLL];
       unsigned k[SUM_UNROLL];
 #pragma unroll
       for (int u = 0; u < SUM_UNROLL; ++u) {
-        k[u] = i + u < end ? key[i + u] : none;
-        if (k[u] != none) v[u] = load_pack<T, W>(dout + row[i + u] * p.stride + c);
+        const uint2 e = i + u < end ? entry[i + u] : make_uint2(none, 0u);
+        k[u] = e.x;
+        if (k[u] != none) v[u] = load_pack<T, W>(dout + e.y * p.stride + c);
       }
 #pragma unroll
       for (int u = 0; u < SUM_UNROLL; ++u) {
@@ -257,8 +331,6 @@ template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding
     }
   }
   __syncthreads();
-  if (count <= 0) return;
-  const unsigned before = first > 0 ? p.keys[first - 1] : none, after = first + count < p.n ? p.keys[first + count] : none;
   for (int x = threadIdx.x; x < width && column0 + x < p.C; x += THREADS) {
     unsigned now = none;
     float sum[1] = {0.f};
@@ -278,18 +350,84 @@ template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding
     }
   }
 }
+template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding_sums(const Sums p, const T *dout) {
+  extern __shared__ uint2 entry[];
+  unsigned *itemKey = (unsigned *)(entry + p.tile);
+  wait_for_prior_grids();
+  dependents_may_launch();
+  const long long first = (long long)blockIdx.x * p.tile;
+  const int count = (int)min((long long)p.tile, p.n - first);
+  for (int i = threadIdx.x; i < count; i += THREADS) entry[i] = p.entries[first + i];
+  const unsigned none = p.vocab;
+  const unsigned before = first > 0 ? p.entries[first - 1].x : none, after = first + count < p.n ? p.entries[first + count].x : none;
+  sum_entries<T, W>(p, dout, entry, count, before, after, itemKey, (float *)(itemKey + 2 * p.groups));
+}
+// The whole gradient of at most SMALL rows in one launch: the first CTAs (one a slab) sort the entries in shared memory and
+// add them up; the others write the zeros of the rows that no token names, each for a range of `range` rows.
+constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
+template <class T, int W>
+__global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums p, const T *dout, const int *tokens, int bits, int range, int *errors) {
+  extern __shared__ uint2 entry[]; // two copies of SMALL entries, then the items; the digit counts lie where the items go
+  __shared__ unsigned warpSum[WARPS], named[MOST_RANGE / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  wait_for_prior_grids();
+  dependents_may_launch();
+  if (blockIdx.x > 0) {
+    if (blockIdx.y > 0) return;
+    const int first = (int)(blockIdx.x - 1) * range, rows = min(range, p.vocab - first);
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += THREADS) named[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.n; i += THREADS) {
+      const int t = tokens[i] - first;
+      if (tokens[i] >= first && t < rows) atomicOr(&named[t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+    for (int r = warp; r < rows; r += WARPS)
+      if (!(named[r >> 5] >> (r & 31) & 1)) clear_floats(p.dtable + (long long)(first + r) * p.C, p.C, lane, 32);
+    return;
+  }
+  uint2 *now = entry, *other = entry + SMALL;
+  unsigned *itemKey = (unsigned *)(entry + 2 * SMALL);
+  for (int i = threadIdx.x; i < p.n; i += THREADS) {
+    const int t = tokens[i];
+    if (t >= p.vocab && errors && blockIdx.y == 0) atomicOr(errors, SCN_DEV_ERR_KEY);
+    now[i] = make_uint2(key_of(t, p.vocab), i);
+  }
+  __syncthreads();
+  const int passes = (bits + SMALL_DIGIT - 1) / SMALL_DIGIT, each = (bits + passes - 1) / passes;
+  for (int k = 0; k < passes; ++k) {
+    unsigned key[SMALL_ROUNDS], row[SMALL_ROUNDS], place[SMALL_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < SMALL_ROUNDS; ++r) {
+      const int j = (warp * SMALL_ROUNDS + r) * 32 + lane;
+      const uint2 e = j < p.n ? now[j] : make_uint2(0u, 0u);
+      key[r] = e.x; row[r] = e.y;
+    }
+    places_by_digit<SMALL_ROUNDS>(key, p.n, k * each, each, (unsigned short *)itemKey, warpSum, place, [](int, unsigned, unsigned) {});
+#pragma unroll
+    for (int r = 0; r < SMALL_ROUNDS; ++r)
+      if ((warp * SMALL_ROUNDS + r) * 32 + lane < p.n) other[place[r]] = make_uint2(key[r], row[r]);
+    __syncthreads();
+    uint2 *t = now; now = other; other = t;
+  }
+  const unsigned none = p.vocab;
+  sum_entries<T, W>(p, dout, now, p.n, none, none, itemKey, (float *)(itemKey + 2 * p.groups));
+}
 // One CTA a tile (times 32-column slabs): if the tile's last token begins in it and goes on, its parts are added up, every
 // WARPS-th one by a warp, then over the warps.
 __global__ void __launch_bounds__(THREADS) k_embedding_join(const Sums p, int tiles) {
-  const int b = blockIdx.x, first = b * p.tile, end = first + p.tile;
+  wait_for_prior_grids();
+  dependents_may_launch();
+  const int b = blockIdx.x;
+  const long long first = (long long)b * p.tile, end = first + p.tile;
   if (end >= p.n) return;
-  const unsigned k = p.keys[end - 1];
-  if (k == (unsigned)p.vocab || p.keys[end] != k || (first > 0 && p.keys[first - 1] == k)) return;
+  const unsigned k = p.entries[end - 1].x, after = p.entries[end].x, before = first > 0 ? p.entries[first - 1].x : (unsigned)p.vocab;
+  if (k == (unsigned)p.vocab || after != k || before == k) return;
   __shared__ float part[WARPS][32];
   int last = b + 1; // the first tile behind that does not begin with k
   for (;;) {
     const int t = last + threadIdx.x;
-    const int off = __syncthreads_count(t < tiles && p.keys[(long long)t * p.tile] == k);
+    const int off = __syncthreads_count(t < tiles && p.entries[(long long)t * p.tile].x == k);
     last += off;
     if (off < THREADS) break;
   }
@@ -324,23 +462,36 @@ int sum_tile(long long n) {
   return tile;
 }
 
+int sort_rounds(long long n) { return n > (1 << 20) ? 16 : 4; } // large tiles: longer runs of a digit; small ones: work for every SM
 struct SortPlan {
-  int tiles, passes, digit;           // digit: bits a pass (the last one may have fewer)
+  int tiles, passes, bits, digit;            // digit: bits a pass
   size_t array, counts, totals, parts, total; // bytes
 };
 SortPlan plan_sort(long long n, int vocab, int C) {
   SortPlan p;
-  int bits = 1;
-  while (bits < 31 && ((long long)vocab >> bits) > 0) ++bits; // keys 0..vocab
-  p.passes = (bits + MAX_DIGIT - 1) / MAX_DIGIT;
-  p.digit = (bits + p.passes - 1) / p.passes;
-  p.tiles = (int)((n + TILE - 1) / TILE);
-  p.array = align_up(sizeof(unsigned) * (size_t)n, 256);
+  p.bits = 1;
+  while (p.bits < 31 && ((long long)vocab >> p.bits) > 0) ++p.bits; // keys 0..vocab
+  p.passes = (p.bits + MAX_DIGIT - 1) / MAX_DIGIT;
+  p.digit = (p.bits + p.passes - 1) / p.passes;
+  const long long tile = THREADS * sort_rounds(n);
+  p.tiles = (int)((n + tile - 1) / tile);
+  p.array = align_up(sizeof(uint2) * (size_t)n, 256);
   p.counts = align_up(sizeof(unsigned) * ((size_t)p.tiles << p.digit), 256);
   p.totals = align_up(sizeof(unsigned) << p.digit, 256);
   p.parts = align_up(sizeof(float) * (size_t)((n + sum_tile(n) - 1) / sum_tile(n)) * (size_t)C, 256); // of each tile's first and last token
-  p.total = 4 * p.array + p.counts + p.totals + 2 * p.parts + 256;
+  p.total = 2 * p.array + p.counts + p.totals + 2 * p.parts + 256;
   return p;
+}
+template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
+  const int digits = 1 << p.bits, clearing = p.clear ? 2 * sm_count() : 0;
+  SCN_CUDA_TRY(launch_dependent(k_radix_count<ROUNDS>, dim3(p.tiles + clearing), dim3(THREADS), sizeof(unsigned) * digits, s, p));
+  SCN_LAUNCH_CHECK("k_radix_count");
+  SCN_CUDA_TRY(launch_dependent(k_radix_scan, dim3(digits), dim3(THREADS), 0, s, p));
+  SCN_LAUNCH_CHECK("k_radix_scan");
+  const size_t smem = sizeof(uint2) * THREADS * ROUNDS + sizeof(unsigned) * digits + sizeof(unsigned short) * WARPS * digits;
+  SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS>, dim3(p.tiles), dim3(THREADS), smem, s, p));
+  SCN_LAUNCH_CHECK("k_radix_scatter");
+  return SCN_OK;
 }
 
 } // namespace
@@ -363,7 +514,7 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
 }
 
 extern "C" size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C) {
-  if (n < 0 || n > 0x7fffffffll - TILE || vocab < 1 || C < 1) return 0;
+  if (n < 0 || n > 0x7fff0000ll || vocab < 1 || C < 1) return 0;
   return plan_sort(n, vocab, C).total;
 }
 
@@ -371,7 +522,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
                                       float scale, int accumulate, float *d_dtable, int *d_errors, void *d_workspace, size_t workspace_bytes,
                                       scn_stream_t stream) {
   clear_error();
-  if (vocab < 1 || C < 1 || n < 0 || n > 0x7fffffffll - TILE) return fail(SCN_ERR_INVALID, "bad embedding sizes");
+  if (vocab < 1 || C < 1 || n < 0 || n > 0x7fff0000ll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (dout_stride < C) return fail(SCN_ERR_INVALID, "embedding: the gradient's row stride is below the number of features");
   if (!type_known(dout_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (!d_dtable || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
@@ -385,51 +536,56 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     return SCN_OK;
   }
   char *w = (char *)d_workspace;
-  unsigned *array[4];
-  for (int i = 0; i < 4; ++i) array[i] = (unsigned *)(w + i * sp.array);
-  Pass p = {};
-  p.n = (int)n; p.vocab = vocab; p.tiles = sp.tiles; p.bits = sp.digit;
-  p.counts = (unsigned *)(w + 4 * sp.array);
-  p.totals = (unsigned *)(w + 4 * sp.array + sp.counts);
-  p.errors = d_errors;
-  for (int k = 0; k < sp.passes; ++k) {
-    p.tokens = k == 0 ? d_tokens : nullptr;
-    p.keys = array[2 * ((k + 1) & 1)]; p.rows = array[2 * ((k + 1) & 1) + 1];
-    p.keysOut = array[2 * (k & 1)]; p.rowsOut = array[2 * (k & 1) + 1];
-    p.shift = k * sp.digit;
-    const int digits = 1 << p.bits;
-    k_radix_count<<<p.tiles, THREADS, sizeof(unsigned) * digits, s>>>(p);
-    SCN_LAUNCH_CHECK("k_radix_count");
-    k_radix_scan<<<digits, THREADS, 0, s>>>(p);
-    SCN_LAUNCH_CHECK("k_radix_scan");
-    k_radix_scatter<<<p.tiles, THREADS, sizeof(unsigned) * digits * WARPS, s>>>(p);
-    SCN_LAUNCH_CHECK("k_radix_scatter");
-  }
   const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W, slabs = (vectors + MAX_LANES - 1) / MAX_LANES;
   Sums q = {};
-  q.keys = p.keysOut; q.rows = p.rowsOut;
   q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = dout_stride;
   q.lanes = lanes_for(vectors);
   q.groups = THREADS / q.lanes;
   q.tile = sum_tile(n);
   q.scale = scale; q.accumulate = accumulate; q.dtable = d_dtable;
-  q.head = (float *)(w + 4 * sp.array + sp.counts + sp.totals);
-  q.tail = (float *)(w + 4 * sp.array + sp.counts + sp.totals + sp.parts);
+  q.head = (float *)(w + 2 * sp.array + sp.counts + sp.totals);
+  q.tail = (float *)(w + 2 * sp.array + sp.counts + sp.totals + sp.parts);
+  const size_t items = 4ull * 2 * q.groups * (1 + q.lanes * W);
+  // F<T, W> for dout's type and the width
+#define SCN_SUMS(F, ...)                                                                                              \
+  SCN_DISPATCH_TYPE(dout_type, T, {                                                                                   \
+    constexpr int MOST = 16 / (int)sizeof(T);                                                                         \
+    if (W == MOST) SCN_CUDA_TRY(launch_dependent(F<T, MOST>, __VA_ARGS__));                                           \
+    else if (W == MOST / 2) SCN_CUDA_TRY(launch_dependent(F<T, MOST / 2>, __VA_ARGS__));                              \
+    else if (W == 1) SCN_CUDA_TRY(launch_dependent(F<T, 1>, __VA_ARGS__));                                            \
+    else SCN_CUDA_TRY(launch_dependent(F<T, 2>, __VA_ARGS__));                                                        \
+  })
+  if (n <= SMALL) {
+    const size_t counts = sizeof(unsigned short) * WARPS << SMALL_DIGIT;
+    const int range = std::max(32, std::min(MOST_RANGE, (vocab + 4 * sm_count() - 1) / (4 * sm_count()))), clearing = accumulate ? 0 : (vocab + range - 1) / range;
+    SCN_SUMS(k_embedding_backward_small, dim3(1 + clearing, slabs), dim3(THREADS), sizeof(uint2) * 2 * SMALL + std::max(items, counts), s, q, (const T *)d_dout,
+             d_tokens, sp.bits, range, d_errors);
+    SCN_LAUNCH_CHECK("k_embedding_backward_small");
+    return SCN_OK;
+  }
+  uint2 *const array[2] = {(uint2 *)w, (uint2 *)(w + sp.array)};
+  Pass p = {};
+  p.n = (int)n; p.vocab = vocab; p.tiles = sp.tiles; p.bits = sp.digit;
+  p.counts = (unsigned *)(w + 2 * sp.array);
+  p.totals = (unsigned *)(w + 2 * sp.array + sp.counts);
+  p.errors = d_errors;
+  for (int k = 0; k < sp.passes; ++k) {
+    p.tokens = k == 0 ? d_tokens : nullptr;
+    p.in = array[(k + 1) & 1];
+    p.out = array[k & 1];
+    p.shift = k * sp.digit;
+    p.clear = k == 0 && !accumulate ? d_dtable : nullptr;
+    p.clearN = (long long)vocab * C;
+    const int rc = sort_rounds(n) == 16 ? sort_pass<16>(p, s) : sort_pass<4>(p, s);
+    if (rc != SCN_OK) return rc;
+  }
+  q.entries = p.out;
   const int tiles = (int)((n + q.tile - 1) / q.tile);
-  if (!accumulate) SCN_CUDA_TRY(cudaMemsetAsync(d_dtable, 0, sizeof(float) * (size_t)vocab * C, s));
-  const size_t smem = 4ull * (2 * q.tile + 2 * q.groups) + 4ull * 2 * q.groups * q.lanes * W;
-  const dim3 grid(tiles, slabs);
-  SCN_DISPATCH_TYPE(dout_type, T, {
-    constexpr int MOST = 16 / (int)sizeof(T);
-    const T *from = (const T *)d_dout;
-    if (W == MOST) k_embedding_sums<T, MOST><<<grid, THREADS, smem, s>>>(q, from);
-    else if (W == MOST / 2) k_embedding_sums<T, MOST / 2><<<grid, THREADS, smem, s>>>(q, from);
-    else if (W == 1) k_embedding_sums<T, 1><<<grid, THREADS, smem, s>>>(q, from);
-    else k_embedding_sums<T, 2><<<grid, THREADS, smem, s>>>(q, from);
-  });
+  SCN_SUMS(k_embedding_sums, dim3(tiles, slabs), dim3(THREADS), sizeof(uint2) * q.tile + items, s, q, (const T *)d_dout);
+#undef SCN_SUMS
   SCN_LAUNCH_CHECK("k_embedding_sums");
   if (tiles > 1) {
-    k_embedding_join<<<dim3(tiles, std::min((C + 31) / 32, 8)), THREADS, 0, s>>>(q, tiles);
+    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(tiles, std::min((C + 31) / 32, 8)), dim3(THREADS), 0, s, q, tiles));
     SCN_LAUNCH_CHECK("k_embedding_join");
   }
   return SCN_OK;

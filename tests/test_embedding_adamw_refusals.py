@@ -81,7 +81,7 @@ def test_step_refuses_bad_tensors(a, change, text):
 
 @pytest.mark.parametrize("change,text", [
     (dict(lr=math.nan), "finite"), (dict(lr=math.inf), "finite"), (dict(grad_scale=math.nan), "finite"), (dict(beta1=1.0), "beta"), (dict(beta1=-0.1), "beta"),
-    (dict(beta2=1.0), "beta"), (dict(beta2=math.nan), "beta"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=-1.0), "eps"), (dict(step=0), "steps"),
+    (dict(beta2=1.0), "beta"), (dict(beta2=math.nan), "beta"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=1e-39), "eps"), (dict(eps=-1.0), "eps"), (dict(step=0), "steps"),
     (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=math.nan), "max_norm"), (dict(max_norm=1.0), "needs the gradients' norm"),
 ])
 def test_step_refuses_bad_parameters(a, change, text):
