@@ -405,12 +405,12 @@ bool wide(const scn_adamw_tensor_t &t) {
   return !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 7 : 31));
 }
 // launch(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.  Where one turn a
-// chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes four: it finds its tensor once for all of them.
-template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, Take take, Launch launch) {
+// chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes `most`: it finds its tensor once for all of them.
+template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Launch launch) {
   List<CAP> l;
   long long all = 0;
   for (int i = 0; i < count; ++i) all += take(t[i]) ? (t[i].n + TURN - 1) / TURN : 0;
-  l.turns = all > 100ll * 148 ? 4 : 1;
+  l.turns = all > 100ll * 148 ? most : 1;
   const long long size = (long long)l.turns * TURN;
   l.count = l.chunks = 0;
   unsigned long long block = 0;
@@ -431,10 +431,10 @@ template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tenso
   return l.count ? launch(l) : (int)SCN_OK;
 }
 // The parameters' bytes are copied at every launch: the smallest list that holds them all.
-template <class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, Take take, Launch launch) {
-  if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, take, launch);
-  if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, take, launch);
-  return for_lists<CAP_LARGE>(t, count, take, launch);
+template <class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Launch launch) {
+  if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, most, take, launch);
+  if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, most, take, launch);
+  return for_lists<CAP_LARGE>(t, count, most, take, launch);
 }
 int norm_ctas() { return 4 * sm_count(); }
 
@@ -480,7 +480,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
   int used = 0, launches = (count + CAP_LARGE - 1) / CAP_LARGE;
   if (launches > most) return fail(SCN_ERR_UNSUPPORTED, "AdamW: list too long");
   const int each = std::min(norm_ctas(), most / std::max(launches, 1));
-  const int rc = for_lists(tensors, count, [](const scn_adamw_tensor_t &) { return true; }, [&](const auto &l) -> int {
+  const int rc = for_lists(tensors, count, 4, [](const scn_adamw_tensor_t &) { return true; }, [&](const auto &l) -> int {
     const int grid = std::min(l.chunks, each);
     SCN_CUDA_TRY(launch_dependent(k_grad_norm_partial<std::decay_t<decltype(l)>::capacity>, dim3(grid), dim3(THREADS), 0, s, l, partial + used));
     SCN_LAUNCH_CHECK("k_grad_norm_partial");
@@ -505,13 +505,13 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
   }
   cudaStream_t s = (cudaStream_t)stream;
   const auto eight = [](const scn_adamw_tensor_t &t) { return t.d_m_scale != nullptr; };
-  int rc = for_lists(tensors, count, [&](const scn_adamw_tensor_t &t) { return !eight(t); }, [&](const auto &l) -> int {
+  int rc = for_lists(tensors, count, 1, [&](const scn_adamw_tensor_t &t) { return !eight(t); }, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_32<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
     SCN_LAUNCH_CHECK("k_adamw_32");
     return SCN_OK;
   });
   if (rc != SCN_OK) return rc;
-  return for_lists(tensors, count, eight, [&](const auto &l) -> int {
+  return for_lists(tensors, count, 4, eight, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_8<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
     SCN_LAUNCH_CHECK("k_adamw_8");
     return SCN_OK;

@@ -84,8 +84,8 @@ struct Pass {
   const uint2 *in;    // (key, row)
   uint2 *out;
   int n, vocab, tiles, shift, bits;
-  unsigned *counts;   // [2^bits][tiles]
-  unsigned *totals;   // [2^bits]
+  unsigned *counts;   // [tiles][2^bits]
+  unsigned *totals;   // [2^bits], or null: counts as k_radix_count left them
   int *errors;
   float *clear;       // first pass: clearN values to set to zero on the side, or null
   long long clearN;
@@ -127,7 +127,7 @@ template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_count(c
     atomicAdd(&hist[(key[r] >> p.shift) & (digits - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += THREADS) p.counts[(long long)d * p.tiles + blockIdx.x] = hist[d];
+  for (int d = threadIdx.x; d < digits; d += THREADS) p.counts[(long long)blockIdx.x * digits + d] = hist[d];
 }
 // Running sum over the CTA's threads: what the threads before this one hold; `all`: what all of them hold.
 __device__ __forceinline__ unsigned sum_before(unsigned own, unsigned *warpSum, unsigned &all) {
@@ -146,37 +146,70 @@ __device__ __forceinline__ unsigned sum_before(unsigned own, unsigned *warpSum, 
   __syncthreads();
   return before + sum - own;
 }
-// One CTA a digit: counts[d][*] becomes its exclusive running sum, totals[d] its sum.
-__global__ void __launch_bounds__(THREADS) k_radix_scan(const Pass p) {
-  __shared__ unsigned warpSum[WARPS];
+// One CTA for SCAN_DIGITS digits (so many counts of a tile fill a sector): counts[*][d] becomes its exclusive running sum over the
+// tiles, totals[d] its sum.  A thread takes one digit of a run of the tiles: it adds them up, learns what the runs before hold,
+// and writes the running sums.
+constexpr int SCAN_DIGITS = 8, SCAN_THREADS = 1024, SCAN_RUNS = SCAN_THREADS / SCAN_DIGITS;
+__global__ void __launch_bounds__(SCAN_THREADS) k_radix_scan(const Pass p) {
+  __shared__ unsigned runSum[SCAN_RUNS][SCAN_DIGITS];
   wait_for_prior_grids();
   dependents_may_launch();
-  unsigned *row = p.counts + (long long)blockIdx.x * p.tiles;
-  unsigned before = 0, all;
-  for (int base = 0; base < p.tiles; base += THREADS) {
-    const int j = base + threadIdx.x;
-    const unsigned own = j < p.tiles ? row[j] : 0u, at = sum_before(own, warpSum, all);
-    if (j < p.tiles) row[j] = before + at;
-    before += all;
+  const int digits = 1 << p.bits, d = threadIdx.x % SCAN_DIGITS, run = threadIdx.x / SCAN_DIGITS;
+  const int each = (p.tiles + SCAN_RUNS - 1) / SCAN_RUNS, begin = min(run * each, p.tiles), end = min(begin + each, p.tiles);
+  unsigned *column = p.counts + blockIdx.x * SCAN_DIGITS + d;
+  unsigned sum = 0;
+#pragma unroll 8
+  for (int t = begin; t < end; ++t) sum += column[(long long)t * digits];
+  runSum[run][d] = sum;
+  __syncthreads();
+  if (threadIdx.x < 32 * SCAN_DIGITS) { // a warp a digit: running sums over the runs
+    const int lane = threadIdx.x & 31, digit = threadIdx.x >> 5;
+    unsigned own[SCAN_RUNS / 32], all = 0;
+#pragma unroll
+    for (int r = 0; r < SCAN_RUNS / 32; ++r) { own[r] = runSum[lane * (SCAN_RUNS / 32) + r][digit]; all += own[r]; }
+    unsigned at = all;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(~0u, at, o);
+      if (lane >= o) at += v;
+    }
+    if (lane == 31) p.totals[blockIdx.x * SCAN_DIGITS + digit] = at;
+    at -= all;
+#pragma unroll
+    for (int r = 0; r < SCAN_RUNS / 32; ++r) { runSum[lane * (SCAN_RUNS / 32) + r][digit] = at; at += own[r]; }
   }
-  if (threadIdx.x == 0) p.totals[blockIdx.x] = before;
+  __syncthreads();
+  unsigned before = runSum[run][d];
+  for (int t0 = begin; t0 < end; t0 += 8) {
+    unsigned n[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) n[u] = t0 + u < end ? column[(long long)(t0 + u) * digits] : 0u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (t0 + u < end) column[(long long)(t0 + u) * digits] = before;
+      before += n[u];
+    }
+  }
 }
 // Places of a tile's entries in its order by digit: place[r] of the entry that this thread holds in round r (a warp's entries
-// lie one after the other, a round's in the order of the lanes).  count[WARPS][digits]: scratch; start(d, at, n) is called once
-// for each digit with the place `at` of its first entry and their number n.  Ranks within a round come from one ballot a bit.
-template <int ROUNDS, class Start>
-__device__ __forceinline__ void places_by_digit(const unsigned (&key)[ROUNDS], int inTile, int shift, int bits, unsigned short *count, unsigned *warpSum,
+// lie one after the other, a round's in the order of the lanes).  count[WARPS][digits]: scratch, 4-byte aligned; start(d, at) is
+// called once for each digit with the place of its first entry.  Ranks within a round come from one ballot a bit.
+template <int ROUNDS, int BITS, class Start>
+__device__ __forceinline__ void places_by_digit(const unsigned (&key)[ROUNDS], int inTile, int shift, unsigned short *count, unsigned *warpSum,
                                                 unsigned (&place)[ROUNDS], Start start) {
-  const int digits = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int d = threadIdx.x; d < WARPS * digits / 2; d += THREADS) ((unsigned *)count)[d] = 0;
+  constexpr int DIGITS = 1 << BITS, PAIRS = DIGITS / 2;
+  static_assert(PAIRS <= THREADS, "a thread takes a pair of digits");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned *pair = (unsigned *)count; // two digits' counts in a word: both stay below 2^16
+  for (int d = threadIdx.x; d < WARPS * PAIRS; d += THREADS) pair[d] = 0;
   __syncthreads();
-  unsigned short *own = count + warp * digits;
+  unsigned short *own = count + warp * DIGITS;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const bool in = (warp * ROUNDS + r) * 32 + lane < inTile;
-    const unsigned d = (key[r] >> shift) & (digits - 1);
+    const unsigned d = (key[r] >> shift) & (DIGITS - 1);
     unsigned peers = __ballot_sync(~0u, in);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
       const bool set = d >> b & 1;
       const unsigned votes = __ballot_sync(~0u, set);
       peers &= set ? votes : ~votes;
@@ -190,33 +223,34 @@ __device__ __forceinline__ void places_by_digit(const unsigned (&key)[ROUNDS], i
     __syncwarp();
   }
   __syncthreads();
-  const int per = (digits + THREADS - 1) / THREADS, d0 = threadIdx.x * per, d1 = min(digits, d0 + per);
-  unsigned sum = 0, all;
-  for (int d = d0; d < d1; ++d)
-    for (int w = 0; w < WARPS; ++w) sum += count[w * digits + d];
-  unsigned at = sum_before(sum, warpSum, all);
-  for (int d = d0; d < d1; ++d) {
-    const unsigned first = at;
+  unsigned sum = 0, all; // counts become each warp's own start
+  if (threadIdx.x < PAIRS)
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += pair[w * PAIRS + threadIdx.x];
+  unsigned at = sum_before((sum & 0xffffu) + (sum >> 16), warpSum, all);
+  if (threadIdx.x < PAIRS) {
+    start(2 * threadIdx.x, at);
+    start(2 * threadIdx.x + 1, at + (sum & 0xffffu));
+    at |= (at + (sum & 0xffffu)) << 16;
+#pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const unsigned n = count[w * digits + d];
-      count[w * digits + d] = (unsigned short)at;
+      const unsigned n = pair[w * PAIRS + threadIdx.x];
+      pair[w * PAIRS + threadIdx.x] = at;
       at += n;
     }
-    start(d, first, at - first);
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r)
-    if ((warp * ROUNDS + r) * 32 + lane < inTile) place[r] += own[(key[r] >> shift) & (digits - 1)];
+    if ((warp * ROUNDS + r) * 32 + lane < inTile) place[r] += own[(key[r] >> shift) & (DIGITS - 1)];
 }
 // A tile is put in order in shared memory first, so that entries of one digit leave side by side.
-template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
-  extern __shared__ uint2 stage[];
-  constexpr int TILE = THREADS * ROUNDS;
-  const int digits = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned *shift = (unsigned *)(stage + TILE); // [digits]: place in the output less place in the tile
-  unsigned short *count = (unsigned short *)(shift + digits);
-  __shared__ unsigned warpSum[WARPS];
+template <int ROUNDS, int BITS> __global__ void __launch_bounds__(THREADS) k_radix_scatter(const Pass p) {
+  constexpr int TILE = THREADS * ROUNDS, DIGITS = 1 << BITS, PAIRS = DIGITS / 2;
+  __shared__ uint2 stage[TILE];
+  __shared__ unsigned shift[DIGITS], warpSum[WARPS]; // shift: place in the output less place in the tile
+  __shared__ __align__(4) unsigned short count[WARPS * DIGITS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_prior_grids();
   dependents_may_launch();
   const long long first = (long long)blockIdx.x * TILE;
@@ -232,169 +266,240 @@ template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_scatter
     }
   }
   // entries of smaller digits, plus those of the digit in earlier tiles
-  const int per = (digits + THREADS - 1) / THREADS, d0 = threadIdx.x * per, d1 = min(digits, d0 + per);
-  unsigned sum = 0, all;
-  for (int d = d0; d < d1; ++d) sum += p.totals[d];
-  unsigned at = sum_before(sum, warpSum, all);
-  for (int d = d0; d < d1; ++d) {
-    shift[d] = at + p.counts[(long long)d * p.tiles + blockIdx.x];
-    at += p.totals[d];
+  unsigned all, low = 0, high = 0, lowBefore = 0, highBefore = 0;
+  if (p.totals && threadIdx.x < PAIRS) {
+    const uint2 total = ((const uint2 *)p.totals)[threadIdx.x], before = ((const uint2 *)p.counts)[(long long)blockIdx.x * PAIRS + threadIdx.x];
+    low = total.x; high = total.y; lowBefore = before.x; highBefore = before.y;
   }
-  places_by_digit<ROUNDS>(key, inTile, p.shift, p.bits, count, warpSum, place, [&](int d, unsigned start, unsigned) { shift[d] -= start; });
+  if (!p.totals && threadIdx.x < PAIRS) { // few tiles: added up here, without k_radix_scan
+#pragma unroll 16
+    for (int t = 0; t < p.tiles; ++t) {
+      const uint2 n = ((const uint2 *)p.counts)[t * PAIRS + threadIdx.x];
+      if (t == (int)blockIdx.x) { lowBefore = low; highBefore = high; }
+      low += n.x; high += n.y;
+    }
+  }
+  const unsigned at = sum_before(low + high, warpSum, all);
+  if (threadIdx.x < PAIRS) {
+    shift[2 * threadIdx.x] = at + lowBefore;
+    shift[2 * threadIdx.x + 1] = at + low + highBefore;
+  }
+  places_by_digit<ROUNDS, BITS>(key, inTile, p.shift, count, warpSum, place, [&](int d, unsigned start) { shift[d] -= start; });
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r)
     if ((warp * ROUNDS + r) * 32 + lane < inTile) stage[place[r]] = make_uint2(key[r], row[r]);
   __syncthreads();
   for (int j = threadIdx.x; j < inTile; j += THREADS) {
     const uint2 e = stage[j];
-    p.out[shift[(e.x >> p.shift) & (digits - 1)] + j] = e;
+    p.out[shift[(e.x >> p.shift) & (DIGITS - 1)] + j] = e;
   }
 }
 
 // ------------------------------------------------------------------ sums of the sorted rows
-// A tile of the sorted entries goes to one CTA (times column slabs): groups of `lanes` threads, W columns a thread, take
+// A tile of the sorted entries goes to one warp (times column slabs): groups of `lanes` threads, W columns a thread, take
 // equal runs of it one after the other and add the rows up in registers.  A run's tokens that lie between its first and
-// its last are complete and go straight to the table; what is left of its first and last token is joined over the CTA in
+// its last are complete and go straight to the table; what is left of its first and last token is joined over the warp in
 // shared memory, and what is left of the tile's first and last token over the tiles by k_embedding_join.  So a token's
 // rows are added in an order that depends on the sorted tokens alone, a token on most of the rows costs no more than
-// others, and each table row is written once.
-constexpr int SUM_UNROLL = 8, MAX_TILE = 2048;
+// others, and each table row is written once.  Warps wait for no other warp: a CTA whose warps met at its end would stand
+// idle while its last rows arrive.
+constexpr int SUM_ROWS = 8, MAX_TILE = 256, MIN_TILE = 64; // rows a thread asks for at once
 struct Sums {
   const uint2 *entries;        // (token, row), sorted
-  int n, vocab, C, tile;       // tile: entries a CTA
-  long long stride;            // of dout's rows
-  int lanes, groups;           // threads of a group, groups of a CTA; a slab is lanes * W columns
+  int n, vocab, C, tile;       // tile: entries a warp
+  unsigned stride;             // of dout's rows, in bytes
+  int lanes;                   // threads of a group in the last slab (32 in the others); a slab is lanes * W columns
   float scale;
   int accumulate;
   float *dtable;
   float *head, *tail;          // [tiles][C]: the part of a tile's first (last) token, where that began (goes on) in another tile
 };
-template <int W> __device__ __forceinline__ void write_row(const Sums &p, unsigned key, int c, const float (&sum)[W]) {
+// The running sums of W columns.
+template <int W> struct Columns {
+  float2 v[W / 2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) v[i] = make_float2(0.f, 0.f);
+  }
+  template <class T> __device__ __forceinline__ void add(const Pack<T, W> &p) {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) v[i] = __fadd2_rn(v[i], pair_of(p, i));
+  }
+  __device__ __forceinline__ float at(int w) const { return w & 1 ? v[w / 2].y : v[w / 2].x; }
+};
+template <> struct Columns<1> {
+  float v;
+  __device__ __forceinline__ void clear() { v = 0.f; }
+  template <class T> __device__ __forceinline__ void add(const Pack<T, 1> &p) { v += to_float(p.v[0]); }
+  __device__ __forceinline__ float at(int) const { return v; }
+};
+template <int W> __device__ __forceinline__ void write_row(const Sums &p, unsigned key, int c, const Columns<W> &sum) {
   float *to = p.dtable + (long long)key * p.C + c;
+  constexpr int V = W < 4 ? W : 4;
 #pragma unroll
-  for (int w = 0; w < W; w += (W < 4 ? W : 4)) {
-    constexpr int V = W < 4 ? W : 4;
+  for (int w = 0; w < W; w += V) {
     Pack<float, V> o;
-    if (p.accumulate) o.raw = *(typename Raw<V * 4>::type *)(to + w);
 #pragma unroll
-    for (int k = 0; k < V; ++k) o.v[k] = p.accumulate ? o.v[k] + p.scale * sum[w + k] : p.scale * sum[w + k];
-    *(typename Raw<V * 4>::type *)(to + w) = o.raw;
+    for (int k = 0; k < V; ++k) o.v[k] = p.scale * sum.at(w + k);
+    if (!p.accumulate) *(typename Raw<V * 4>::type *)(to + w) = o.raw;
+    else if constexpr (V == 4) atomicAdd((float4 *)(to + w), make_float4(o.v[0], o.v[1], o.v[2], o.v[3])); // (not waited for; no other
+    else if constexpr (V == 2) atomicAdd((float2 *)(to + w), make_float2(o.v[0], o.v[1]));                  //  thread adds to this row)
+    else atomicAdd(to + w, o.v[0]);
   }
 }
-// The sums of `count` sorted entries in shared memory; before, after: the tokens around them.  items: 2 * groups keys and as
-// many rows of a slab's width.
+// The sums of a warp's `count` sorted entries in shared memory, all of them of tokens, with SUM_ROWS more entries behind them that
+// name any row of dout; before, after: the tokens around them.  item[2 g], item[2 g + 1]: what group g's run holds of its first
+// and last token (0 for the last one where the run holds one token only), so that the items' tokens ascend.  head, tail: where
+// the parts go that other warps have to do with.
+template <int W> struct Items {
+  unsigned key[64];
+  float sum[64 * W];
+};
 template <class T, int W>
-__device__ __forceinline__ void sum_entries(const Sums &p, const T *dout, const uint2 *entry, int count, unsigned before, unsigned after, unsigned *itemKey, float *item) {
-  const unsigned none = p.vocab; // the key of rows without a token: behind all others
-  const int width = p.lanes * W, column0 = blockIdx.y * width, group = threadIdx.x / p.lanes, lane = threadIdx.x - group * p.lanes, c = column0 + lane * W;
-  for (int i = threadIdx.x; i < 2 * p.groups; i += THREADS) itemKey[i] = none;
-  __syncthreads();
-  if (group < p.groups && c < p.C) {
-    const int each = (count + p.groups - 1) / p.groups, begin = min(group * each, count), end = min(begin + each, count);
-    float sum[W];
-    unsigned now = begin < end ? entry[begin].x : none;
-    bool atHead = true;
+__device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const uint2 *entry, int count, unsigned before, unsigned after, Items<W> &items, float *head,
+                                          float *tail) {
+  const unsigned none = p.vocab;
+  const int lanes = blockIdx.y + 1 < gridDim.y ? 32 : p.lanes, groups = 32 / lanes, width = lanes * W, column0 = blockIdx.y * 32 * W;
+  const int lane = threadIdx.x & 31, group = lane / lanes, column = (lane - group * lanes) * W, c = column0 + column;
+  const int each = (count + groups - 1) / groups, begin = min(group * each, count), end = group < groups && c < p.C ? min(begin + each, count) : begin;
+  Columns<W> sum;
+  sum.clear();
+  unsigned now = begin < end ? entry[begin].x : none;
+  bool atHead = true;
+  const auto to_item = [&](int at) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum[w] = 0.f;
-    for (int i = begin; i < end && entry[i].x != none; i += SUM_UNROLL) {
-      Pack<T, W> v[SUM_UNROLL];
-      unsigned k[SUM_UNROLL];
+    for (int w = 0; w < W; ++w) items.sum[at * width + column + w] = sum.at(w);
+    if (column == 0) items.key[at] = now;
+  };
+  const char *from = (const char *)(dout + c);
+  for (int s = 0; s < each; s += SUM_ROWS) {
+    __syncwarp(); // the groups part where their tokens change, and ask for their next rows together
+    const int i = begin + s;
+    if (i >= end) continue;
+    Pack<T, W> v[SUM_ROWS];
 #pragma unroll
-      for (int u = 0; u < SUM_UNROLL; ++u) {
-        const uint2 e = i + u < end ? entry[i + u] : make_uint2(none, 0u);
-        k[u] = e.x;
-        if (k[u] != none) v[u] = load_pack<T, W>(dout + e.y * p.stride + c);
-      }
+    for (int u = 0; u < SUM_ROWS; ++u) v[u] = load_pack<T, W>((const T *)(from + (unsigned long long)entry[i + u].y * p.stride));
+    if (i + SUM_ROWS <= end && entry[i + SUM_ROWS - 1].x == now) { // one token all along
 #pragma unroll
-      for (int u = 0; u < SUM_UNROLL; ++u) {
-        if (k[u] == none) break;
-        if (k[u] != now) {
-          if (atHead) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) item[2 * group * width + lane * W + w] = sum[w];
-            if (lane == 0) itemKey[2 * group] = now;
-            atHead = false;
-          } else write_row<W>(p, now, c, sum);
-          now = k[u];
-#pragma unroll
-          for (int w = 0; w < W; ++w) sum[w] = 0.f;
-        }
-#pragma unroll
-        for (int w = 0; w < W; ++w) sum[w] += to_float(v[u].v[w]);
-      }
+      for (int u = 0; u < SUM_ROWS; ++u) sum.add(v[u]);
+      continue;
     }
-    if (now != none) {
-      const int at = 2 * group + (atHead ? 0 : 1);
 #pragma unroll
-      for (int w = 0; w < W; ++w) item[at * width + lane * W + w] = sum[w];
-      if (lane == 0) itemKey[at] = now;
+    for (int u = 0; u < SUM_ROWS; ++u) {
+      if (i + u < end) {
+        const unsigned k = entry[i + u].x;
+        if (k != now) {
+          if (atHead) to_item(2 * group);
+          else write_row<W>(p, now, c, sum);
+          atHead = false;
+          now = k;
+          sum.clear();
+        }
+        sum.add(v[u]);
+      }
     }
   }
-  __syncthreads();
-  for (int x = threadIdx.x; x < width && column0 + x < p.C; x += THREADS) {
-    unsigned now = none;
-    float sum[1] = {0.f};
-    for (int j = 0; j <= 2 * p.groups; ++j) {
-      const unsigned k = j < 2 * p.groups ? itemKey[j] : none;
-      if (k == none && j < 2 * p.groups) continue;
+  if (group < groups) {
+    to_item(2 * group + (atHead ? 0 : 1));
+    if (atHead) {
+      sum.clear();
+      to_item(2 * group + 1);
+    }
+  }
+  __syncwarp();
+  for (int x = lane; x < width && column0 + x < p.C; x += 32) {
+    Columns<1> total;
+    total.clear();
+    now = none;
+    for (int j = 0; j <= 2 * groups; ++j) {
+      const unsigned k = j < 2 * groups ? items.key[j] : none;
       if (k != now) {
-        if (now != none) {
-          if (now == before) p.head[(long long)blockIdx.x * p.C + column0 + x] = sum[0];
-          else if (now == after) p.tail[(long long)blockIdx.x * p.C + column0 + x] = sum[0];
-          else write_row<1>(p, now, column0 + x, sum);
-        }
+        if (now == none) ;
+        else if (now == before) head[column0 + x] = total.v;
+        else if (now == after) tail[column0 + x] = total.v;
+        else write_row<1>(p, now, column0 + x, total);
         now = k;
-        sum[0] = 0.f;
+        total.clear();
       }
-      if (j < 2 * p.groups) sum[0] += item[j * width + x];
+      if (k != none) total.v += items.sum[j * width + x];
     }
   }
 }
-template <class T, int W> __global__ void __launch_bounds__(THREADS) k_embedding_sums(const Sums p, const T *dout) {
-  extern __shared__ uint2 entry[];
-  unsigned *itemKey = (unsigned *)(entry + p.tile);
+template <class T, int W> __global__ void __launch_bounds__(THREADS, 4) k_embedding_sums(const Sums p, const T *dout) {
+  __shared__ uint2 entries[WARPS][MAX_TILE + SUM_ROWS];
+  __shared__ Items<W> items[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_prior_grids();
   dependents_may_launch();
-  const long long first = (long long)blockIdx.x * p.tile;
-  const int count = (int)min((long long)p.tile, p.n - first);
-  for (int i = threadIdx.x; i < count; i += THREADS) entry[i] = p.entries[first + i];
+  const long long tile = (long long)blockIdx.x * WARPS + warp, first = tile * p.tile;
+  if (first >= p.n) return;
+  uint2 *entry = entries[warp];
   const unsigned none = p.vocab;
-  const unsigned before = first > 0 ? p.entries[first - 1].x : none, after = first + count < p.n ? p.entries[first + count].x : none;
-  sum_entries<T, W>(p, dout, entry, count, before, after, itemKey, (float *)(itemKey + 2 * p.groups));
+  const int most = (int)min((long long)p.tile, p.n - first);
+  const unsigned before = first > 0 ? p.entries[first - 1].x : none, next = first + most < p.n ? p.entries[first + most].x : none;
+  uint2 e[MAX_TILE / 32];
+#pragma unroll
+  for (int r = 0; r < MAX_TILE / 32; ++r) e[r] = r * 32 + lane < most ? p.entries[first + r * 32 + lane] : make_uint2(none, 0u);
+  int count = 0; // entries with a token: they come first
+#pragma unroll
+  for (int r = 0; r < MAX_TILE / 32; ++r) {
+    if (r * 32 + lane < most) entry[r * 32 + lane] = e[r];
+    count += __popc(__ballot_sync(~0u, e[r].x != none));
+  }
+  if (count == 0) return;
+  __syncwarp();
+  const unsigned any = entry[count - 1].y;
+  __syncwarp();
+  if (lane < SUM_ROWS) entry[count + lane] = make_uint2(none, any);
+  __syncwarp();
+  warp_sums<T, W>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
 }
 // The whole gradient of at most SMALL rows in one launch: the first CTAs (one a slab) sort the entries in shared memory and
 // add them up; the others write the zeros of the rows that no token names, each for a range of `range` rows.
 constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
 template <class T, int W>
 __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums p, const T *dout, const int *tokens, int bits, int range, int *errors) {
-  extern __shared__ uint2 entry[]; // two copies of SMALL entries, then the items; the digit counts lie where the items go
-  __shared__ unsigned warpSum[WARPS], named[MOST_RANGE / 32];
+  __shared__ uint2 entries[2][SMALL + SUM_ROWS];
+  __shared__ union {
+    unsigned present[MOST_RANGE / 32];             // (the CTAs that write zeros)
+    unsigned short count[WARPS << SMALL_DIGIT];    // (while sorting)
+    Items<W> items[WARPS];
+  } sh;
+  __shared__ unsigned warpSum[WARPS], all;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_prior_grids();
   dependents_may_launch();
   if (blockIdx.x > 0) {
     if (blockIdx.y > 0) return;
     const int first = (int)(blockIdx.x - 1) * range, rows = min(range, p.vocab - first);
-    for (int i = threadIdx.x; i < (rows + 31) / 32; i += THREADS) named[i] = 0;
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += THREADS) sh.present[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.n; i += THREADS) {
       const int t = tokens[i] - first;
-      if (tokens[i] >= first && t < rows) atomicOr(&named[t >> 5], 1u << (t & 31));
+      if (tokens[i] >= first && t < rows) atomicOr(&sh.present[t >> 5], 1u << (t & 31));
     }
     __syncthreads();
     for (int r = warp; r < rows; r += WARPS)
-      if (!(named[r >> 5] >> (r & 31) & 1)) clear_floats(p.dtable + (long long)(first + r) * p.C, p.C, lane, 32);
+      if (!(sh.present[r >> 5] >> (r & 31) & 1)) clear_floats(p.dtable + (long long)(first + r) * p.C, p.C, lane, 32);
     return;
   }
-  uint2 *now = entry, *other = entry + SMALL;
-  unsigned *itemKey = (unsigned *)(entry + 2 * SMALL);
+  uint2 *now = entries[0], *other = entries[1];
+  const unsigned none = p.vocab;
+  if (threadIdx.x == 0) all = 0;
+  __syncthreads();
+  int named = 0; // entries with a token: they come first in the end
   for (int i = threadIdx.x; i < p.n; i += THREADS) {
     const int t = tokens[i];
     if (t >= p.vocab && errors && blockIdx.y == 0) atomicOr(errors, SCN_DEV_ERR_KEY);
     now[i] = make_uint2(key_of(t, p.vocab), i);
+    named += now[i].x != none;
   }
+  named = __reduce_add_sync(~0u, named);
+  if (lane == 0) atomicAdd(&all, (unsigned)named);
   __syncthreads();
-  const int passes = (bits + SMALL_DIGIT - 1) / SMALL_DIGIT, each = (bits + passes - 1) / passes;
+  const int count = (int)all;
+  if (count == 0) return;
+  const int passes = (bits + SMALL_DIGIT - 1) / SMALL_DIGIT;
   for (int k = 0; k < passes; ++k) {
     unsigned key[SMALL_ROUNDS], row[SMALL_ROUNDS], place[SMALL_ROUNDS];
 #pragma unroll
@@ -403,46 +508,131 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
       const uint2 e = j < p.n ? now[j] : make_uint2(0u, 0u);
       key[r] = e.x; row[r] = e.y;
     }
-    places_by_digit<SMALL_ROUNDS>(key, p.n, k * each, each, (unsigned short *)itemKey, warpSum, place, [](int, unsigned, unsigned) {});
+    places_by_digit<SMALL_ROUNDS, SMALL_DIGIT>(key, p.n, k * SMALL_DIGIT, sh.count, warpSum, place, [](int, unsigned) {});
 #pragma unroll
     for (int r = 0; r < SMALL_ROUNDS; ++r)
       if ((warp * SMALL_ROUNDS + r) * 32 + lane < p.n) other[place[r]] = make_uint2(key[r], row[r]);
     __syncthreads();
     uint2 *t = now; now = other; other = t;
   }
-  const unsigned none = p.vocab;
-  sum_entries<T, W>(p, dout, now, p.n, none, none, itemKey, (float *)(itemKey + 2 * p.groups));
+  const unsigned any = now[count - 1].y;
+  __syncthreads();
+  if (threadIdx.x < SUM_ROWS) now[count + threadIdx.x] = make_uint2(none, any);
+  __syncthreads();
+  const int tile = (count + WARPS - 1) / WARPS, first = min(warp * tile, count), end = min(first + tile, count), column0 = blockIdx.y * 32 * W;
+  const int width = (blockIdx.y + 1 < gridDim.y ? 32 : p.lanes) * W;
+  const auto key_at = [&](int i) { return i >= 0 && i < count ? now[i].x : none; };
+  if (first < end) // (a warp's head and tail take the places of its first two items, read by then)
+    warp_sums<T, W>(p, dout, now + first, end - first, key_at(first - 1), key_at(end), sh.items[warp], sh.items[warp].sum - column0,
+                    sh.items[warp].sum + width - column0);
+  __syncthreads();
+  if (first >= end) return;
+  const unsigned last = now[end - 1].x; // as in k_embedding_join
+  if (key_at(end) != last || key_at(first - 1) == last) return;
+  for (int x = lane; x < width && column0 + x < p.C; x += 32) {
+    Columns<1> sum;
+    sum.v = sh.items[warp].sum[width + x];
+    for (int w = warp + 1; w < WARPS && key_at(w * tile) == last; ++w) sum.v += sh.items[w].sum[x];
+    write_row<1>(p, last, column0 + x, sum);
+  }
 }
-// One CTA a tile (times 32-column slabs): if the tile's last token begins in it and goes on, its parts are added up, every
-// WARPS-th one by a warp, then over the warps.
-__global__ void __launch_bounds__(THREADS) k_embedding_join(const Sums p, int tiles) {
+// A token that begins in one tile and goes on in others: its parts are added up, in two steps so that one on most of the rows
+// does not keep a single CTA busy.  First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front
+// become one part, in the place of the first: a warp for each.
+__device__ __forceinline__ unsigned first_token(const Sums &p, int tiles, long long t) { return t < tiles ? p.entries[t * p.tile].x : (unsigned)p.vocab; }
+__global__ void __launch_bounds__(THREADS) k_embedding_join32(const Sums p, int tiles) {
   wait_for_prior_grids();
   dependents_may_launch();
-  const int b = blockIdx.x;
-  const long long first = (long long)b * p.tile, end = first + p.tile;
-  if (end >= p.n) return;
-  const unsigned k = p.entries[end - 1].x, after = p.entries[end].x, before = first > 0 ? p.entries[first - 1].x : (unsigned)p.vocab;
-  if (k == (unsigned)p.vocab || after != k || before == k) return;
-  __shared__ float part[WARPS][32];
-  int last = b + 1; // the first tile behind that does not begin with k
-  for (;;) {
-    const int t = last + threadIdx.x;
-    const int off = __syncthreads_count(t < tiles && p.entries[(long long)t * p.tile].x == k);
-    last += off;
-    if (off < THREADS) break;
+  const int lane = threadIdx.x & 31;
+  const long long t0 = 32ll * (blockIdx.x * WARPS + (threadIdx.x >> 5));
+  if (t0 == 0 || t0 + 32 > tiles) return;
+  const unsigned k = p.entries[t0 * p.tile - 1].x;
+  if (k == (unsigned)p.vocab || !__all_sync(~0u, first_token(p, tiles, t0 + lane) == k)) return;
+  for (int c = lane; c < p.C; c += 32) {
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 32; ++t) sum += p.head[(t0 + t) * p.C + c];
+    p.head[t0 * p.C + c] = sum;
   }
+}
+// Then a warp looks at one tile after the other and adds up a token that begins in it and goes on in fewer than 32 more; a longer
+// one is left for the whole CTA, whose warps take every JOIN_WARPS-th part and add up what they have.  joined: whether
+// k_embedding_join32 ran (not where there are few tiles).
+constexpr int JOIN_THREADS = 512, JOIN_WARPS = JOIN_THREADS / 32, JOIN_COLUMNS = 4; // columns of a thread at once
+__global__ void __launch_bounds__(JOIN_THREADS) k_embedding_join(const Sums p, int tiles, int joined) {
+  __shared__ float share[JOIN_WARPS][32 * JOIN_COLUMNS];
+  __shared__ int longOnes[JOIN_WARPS], found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int c0 = blockIdx.y * 32; c0 < p.C; c0 += gridDim.y * 32) {
-    float sum[1] = {0.f};
-    if (c0 + lane < p.C) {
-#pragma unroll 8
-      for (int t = b + warp; t < last; t += WARPS) sum[0] += (t == b ? p.tail : p.head)[(long long)t * p.C + c0 + lane];
+  const unsigned none = p.vocab;
+  wait_for_prior_grids();
+  dependents_may_launch();
+  // columns c, c + 32, ... of parts begin, begin + step, ...: added to sum
+  const auto add_parts = [&](float (&sum)[JOIN_COLUMNS], int c, int begin, int end, int step, auto row_of) {
+#pragma unroll 4
+    for (int i = begin; i < end; i += step) {
+      const float *part = row_of(i) + c;
+#pragma unroll
+      for (int j = 0; j < JOIN_COLUMNS; ++j) sum[j] += c + 32 * j < p.C ? part[32 * j] : 0.f;
     }
-    part[warp][lane] = sum[0];
+  };
+  for (int base = blockIdx.x * JOIN_WARPS; base < tiles; base += gridDim.x * JOIN_WARPS) {
+    const int b = base + warp;
+    const long long first = (long long)b * p.tile, end = first + p.tile;
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
-    if (warp == 0 && c0 + lane < p.C) {
-      for (int w = 1; w < WARPS; ++w) sum[0] += part[w][lane];
-      write_row<1>(p, k, c0 + lane, sum);
+    if (end < p.n) {
+      const unsigned k = p.entries[end - 1].x, before = first > 0 ? p.entries[first - 1].x : none;
+      const unsigned follows = first_token(p, tiles, (long long)b + 1 + lane); // the tokens that the next tiles begin with
+      const unsigned same = __ballot_sync(~0u, follows == k);
+      if (k != none && (same & 1) && before != k) {
+        if (same == ~0u) {
+          if (lane == 0) longOnes[atomicAdd(&found, 1)] = b;
+        } else {
+          for (int c = lane; c - lane < p.C; c += 32 * JOIN_COLUMNS) {
+            float sum[JOIN_COLUMNS] = {};
+            add_parts(sum, c, 0, __ffs(~same), 1, [&](int i) { return (i == 0 ? p.tail : p.head) + (long long)(b + i) * p.C; });
+#pragma unroll
+            for (int j = 0; j < JOIN_COLUMNS; ++j)
+              if (c + 32 * j < p.C) write_row<1>(p, k, c + 32 * j, Columns<1>{sum[j]});
+          }
+        }
+      }
+    }
+    __syncthreads();
+    for (int l = 0; l < found; ++l) {
+      const int t0 = longOnes[l];
+      const unsigned k = p.entries[(long long)(t0 + 1) * p.tile].x;
+      int last = t0 + 1, beyond = tiles; // the last tile that begins with k: `last` does, `beyond` does not
+      while (beyond - last > 1) {
+        const int step = (beyond - last + JOIN_THREADS - 1) / JOIN_THREADS;
+        const int with = __syncthreads_count(first_token(p, tiles, (long long)last + (long long)threadIdx.x * step) == k);
+        last += (with - 1) * step;
+        beyond = (int)min((long long)beyond, (long long)last + step);
+      }
+      ++last;
+      // the parts: t0's tail, single tiles, 32 tiles at a time where they have been joined, single tiles
+      const int from = min(last, joined ? (t0 + 32) / 32 * 32 : last), to = max(from, last / 32 * 32);
+      const int singles = from - t0, both = singles + (to - from) / 32, parts = both + max(0, last - to);
+      const auto row_of = [&](int i) {
+        const int t = i < singles ? t0 + i : i < both ? from + 32 * (i - singles) : to + i - both;
+        return (i == 0 ? p.tail : p.head) + (long long)t * p.C;
+      };
+      for (int c = lane; c - lane < p.C; c += 32 * JOIN_COLUMNS) {
+        float sum[JOIN_COLUMNS] = {};
+        add_parts(sum, c, warp, parts, JOIN_WARPS, row_of);
+#pragma unroll
+        for (int j = 0; j < JOIN_COLUMNS; ++j) share[warp][32 * j + lane] = sum[j];
+        __syncthreads();
+        const int column = c - lane + threadIdx.x;
+        if (threadIdx.x < 32 * JOIN_COLUMNS && column < p.C) {
+          Columns<1> total;
+          total.clear();
+#pragma unroll
+          for (int w = 0; w < JOIN_WARPS; ++w) total.v += share[w][threadIdx.x];
+          write_row<1>(p, k, column, total);
+        }
+        __syncthreads();
+      }
     }
     __syncthreads();
   }
@@ -455,14 +645,16 @@ int pack_width(int type, const void *dout, long long stride, const float *dtable
     if (C % W == 0 && stride % W == 0 && (uintptr_t)dout % (W * size) == 0 && (uintptr_t)dtable % (4 * std::min(W, 4)) == 0) return W;
   return 1;
 }
-// Entries a CTA sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than four CTAs each.
+// Entries a warp sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than 16 warps each.
 int sum_tile(long long n) {
   int tile = MAX_TILE;
-  while (tile > 64 && n / tile < 4 * 148) tile /= 2;
+  while (tile > MIN_TILE && n / tile < 16 * 148) tile /= 2;
   return tile;
 }
 
-int sort_rounds(long long n) { return n > (1 << 20) ? 16 : 4; } // large tiles: longer runs of a digit; small ones: work for every SM
+constexpr int LARGE_ROUNDS = 8, LEAST_DIGIT = 6;
+constexpr int FEW_TILES = 64;
+int sort_rounds(long long n) { return n > (1 << 20) ? LARGE_ROUNDS : 4; } // large tiles: longer runs of a digit; small ones: work for every SM
 struct SortPlan {
   int tiles, passes, bits, digit;            // digit: bits a pass
   size_t array, counts, totals, parts, total; // bytes
@@ -472,7 +664,7 @@ SortPlan plan_sort(long long n, int vocab, int C) {
   p.bits = 1;
   while (p.bits < 31 && ((long long)vocab >> p.bits) > 0) ++p.bits; // keys 0..vocab
   p.passes = (p.bits + MAX_DIGIT - 1) / MAX_DIGIT;
-  p.digit = (p.bits + p.passes - 1) / p.passes;
+  p.digit = std::max(LEAST_DIGIT, (p.bits + p.passes - 1) / p.passes);
   const long long tile = THREADS * sort_rounds(n);
   p.tiles = (int)((n + tile - 1) / tile);
   p.array = align_up(sizeof(uint2) * (size_t)n, 256);
@@ -486,10 +678,14 @@ template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
   const int digits = 1 << p.bits, clearing = p.clear ? 2 * sm_count() : 0;
   SCN_CUDA_TRY(launch_dependent(k_radix_count<ROUNDS>, dim3(p.tiles + clearing), dim3(THREADS), sizeof(unsigned) * digits, s, p));
   SCN_LAUNCH_CHECK("k_radix_count");
-  SCN_CUDA_TRY(launch_dependent(k_radix_scan, dim3(digits), dim3(THREADS), 0, s, p));
-  SCN_LAUNCH_CHECK("k_radix_scan");
-  const size_t smem = sizeof(uint2) * THREADS * ROUNDS + sizeof(unsigned) * digits + sizeof(unsigned short) * WARPS * digits;
-  SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS>, dim3(p.tiles), dim3(THREADS), smem, s, p));
+  if (p.totals) SCN_CUDA_TRY(launch_dependent(k_radix_scan, dim3(digits / SCAN_DIGITS), dim3(SCAN_THREADS), 0, s, p));
+  if (p.totals) SCN_LAUNCH_CHECK("k_radix_scan");
+  switch (p.bits) {
+  case 6: SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS, 6>, dim3(p.tiles), dim3(THREADS), 0, s, p)); break;
+  case 7: SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS, 7>, dim3(p.tiles), dim3(THREADS), 0, s, p)); break;
+  case 8: SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS, 8>, dim3(p.tiles), dim3(THREADS), 0, s, p)); break;
+  default: SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS, 9>, dim3(p.tiles), dim3(THREADS), 0, s, p)); break;
+  }
   SCN_LAUNCH_CHECK("k_radix_scatter");
   return SCN_OK;
 }
@@ -525,6 +721,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   if (vocab < 1 || C < 1 || n < 0 || n > 0x7fff0000ll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (dout_stride < C) return fail(SCN_ERR_INVALID, "embedding: the gradient's row stride is below the number of features");
   if (!type_known(dout_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
+  if (dout_stride > 0xffffffffll / type_bytes(dout_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the gradient's rows lie 4 GiB apart or more");
   if (!d_dtable || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
   if (n && (!d_tokens || !d_dout)) return fail(SCN_ERR_INVALID, "null pointer");
   const SortPlan sp = plan_sort(n, vocab, C);
@@ -536,16 +733,14 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     return SCN_OK;
   }
   char *w = (char *)d_workspace;
-  const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W, slabs = (vectors + MAX_LANES - 1) / MAX_LANES;
+  const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W, slabs = (vectors + 31) / 32;
   Sums q = {};
-  q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = dout_stride;
-  q.lanes = lanes_for(vectors);
-  q.groups = THREADS / q.lanes;
+  q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = (unsigned)(dout_stride * type_bytes(dout_type));
+  q.lanes = vectors - (slabs - 1) * 32;
   q.tile = sum_tile(n);
   q.scale = scale; q.accumulate = accumulate; q.dtable = d_dtable;
   q.head = (float *)(w + 2 * sp.array + sp.counts + sp.totals);
   q.tail = (float *)(w + 2 * sp.array + sp.counts + sp.totals + sp.parts);
-  const size_t items = 4ull * 2 * q.groups * (1 + q.lanes * W);
   // F<T, W> for dout's type and the width
 #define SCN_SUMS(F, ...)                                                                                              \
   SCN_DISPATCH_TYPE(dout_type, T, {                                                                                   \
@@ -556,10 +751,8 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     else SCN_CUDA_TRY(launch_dependent(F<T, 2>, __VA_ARGS__));                                                        \
   })
   if (n <= SMALL) {
-    const size_t counts = sizeof(unsigned short) * WARPS << SMALL_DIGIT;
     const int range = std::max(32, std::min(MOST_RANGE, (vocab + 4 * sm_count() - 1) / (4 * sm_count()))), clearing = accumulate ? 0 : (vocab + range - 1) / range;
-    SCN_SUMS(k_embedding_backward_small, dim3(1 + clearing, slabs), dim3(THREADS), sizeof(uint2) * 2 * SMALL + std::max(items, counts), s, q, (const T *)d_dout,
-             d_tokens, sp.bits, range, d_errors);
+    SCN_SUMS(k_embedding_backward_small, dim3(1 + clearing, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout, d_tokens, sp.bits, range, d_errors);
     SCN_LAUNCH_CHECK("k_embedding_backward_small");
     return SCN_OK;
   }
@@ -567,7 +760,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   Pass p = {};
   p.n = (int)n; p.vocab = vocab; p.tiles = sp.tiles; p.bits = sp.digit;
   p.counts = (unsigned *)(w + 2 * sp.array);
-  p.totals = (unsigned *)(w + 2 * sp.array + sp.counts);
+  p.totals = sp.tiles > FEW_TILES ? (unsigned *)(w + 2 * sp.array + sp.counts) : nullptr;
   p.errors = d_errors;
   for (int k = 0; k < sp.passes; ++k) {
     p.tokens = k == 0 ? d_tokens : nullptr;
@@ -576,16 +769,21 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     p.shift = k * sp.digit;
     p.clear = k == 0 && !accumulate ? d_dtable : nullptr;
     p.clearN = (long long)vocab * C;
-    const int rc = sort_rounds(n) == 16 ? sort_pass<16>(p, s) : sort_pass<4>(p, s);
+    const int rc = sort_rounds(n) == 4 ? sort_pass<4>(p, s) : sort_pass<LARGE_ROUNDS>(p, s);
     if (rc != SCN_OK) return rc;
   }
   q.entries = p.out;
   const int tiles = (int)((n + q.tile - 1) / q.tile);
-  SCN_SUMS(k_embedding_sums, dim3(tiles, slabs), dim3(THREADS), sizeof(uint2) * q.tile + items, s, q, (const T *)d_dout);
+  SCN_SUMS(k_embedding_sums, dim3((tiles + WARPS - 1) / WARPS, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout);
 #undef SCN_SUMS
   SCN_LAUNCH_CHECK("k_embedding_sums");
   if (tiles > 1) {
-    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(tiles, std::min((C + 31) / 32, 8)), dim3(THREADS), 0, s, q, tiles));
+    const int joined = tiles > 2048;
+    if (joined) {
+      SCN_CUDA_TRY(launch_dependent(k_embedding_join32, dim3((tiles / 32 + WARPS - 1) / WARPS), dim3(THREADS), 0, s, q, tiles));
+      SCN_LAUNCH_CHECK("k_embedding_join32");
+    }
+    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(std::min((tiles + JOIN_WARPS - 1) / JOIN_WARPS, 4 * sm_count())), dim3(JOIN_THREADS), 0, s, q, tiles, joined));
     SCN_LAUNCH_CHECK("k_embedding_join");
   }
   return SCN_OK;

@@ -34,6 +34,14 @@ template <class T, int W> __device__ __forceinline__ Pack<T, W> load_pack(const 
   return r;
 }
 
+// Values 2 i and 2 i + 1 of a pack as floats.
+template <int W> __device__ __forceinline__ float2 pair_of(const Pack<float, W> &p, int i) { return make_float2(p.v[2 * i], p.v[2 * i + 1]); }
+template <int W> __device__ __forceinline__ float2 pair_of(const Pack<__half, W> &p, int i) { return __half22float2(((const __half2 *)p.v)[i]); }
+template <int W> __device__ __forceinline__ float2 pair_of(const Pack<__nv_bfloat16, W> &p, int i) {
+  const unsigned x = ((const unsigned *)p.v)[i];
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
 // Eight consecutive values, 32-byte (float), 16-byte (16-bit) aligned, as one access.
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
   asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
