@@ -137,7 +137,7 @@ def lib():
 
 
 def check(status):
-    if status != SCN_OK:
+    if status:
         L = lib()
         raise ScnError("%s: %s" % (L.scn_status_string(status).decode(), L.scn_last_error().decode()))
 
@@ -153,7 +153,7 @@ def _stream():
 def _raw_stream():
     """The current stream of the current device as an integer (what torch.cuda.current_stream().cuda_stream gives, without making the
     Stream object, which takes longer than a kernel launch)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _i32(t):
@@ -577,54 +577,56 @@ def sgemm_rowmajor(A, B, C, l, m, r, alpha=1.0, beta=0.0, trans_a=False, trans_b
 
 
 # ---------------------------------------------------------------------------------------------- embedding table
-def _here(device):
-    """The current device's index, if `device` is it: kernels run on the current device's current stream."""
-    if device.type != "cuda":
-        raise ScnError("invalid argument: CUDA tensors are needed, not tensors on %s" % device)
-    if device.index != torch.cuda.current_device():
-        raise ScnError("invalid argument: tensors on %s, the current device is cuda:%d" % (device, torch.cuda.current_device()))
+def _on_current_device(*tensors):
+    """Raises unless every tensor given (None: an argument left out) lies on the current device, on whose current stream kernels run."""
+    at = -2
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != at:
+                if i < 0:
+                    raise ScnError("invalid argument: CUDA tensors are needed, not tensors on %s" % t.device)
+                if at == -2:
+                    at = torch._C._cuda_getDevice()
+                if i != at:
+                    raise ScnError("invalid argument: a tensor on cuda:%d, the current device is cuda:%d" % (i, at))
 
 
-def _rows_of(t, n, C, what):
-    """(pointer, type, row stride) of a 2-d tensor [n, C] whose rows may lie further apart than C."""
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != C or t.dtype not in _TYPES or not t.is_cuda:
-        raise ScnError("invalid argument: %s must be a CUDA tensor [%d, %d] of float32, bfloat16 or float16" % (what, n, C))
-    stride = t.stride(0) if n > 1 else C
-    if (C > 1 and t.stride(1) != 1) or stride < C:
-        raise ScnError("invalid argument: %s: the values of a row must lie together and rows must not overlap" % what)
-    return t.data_ptr(), _TYPES[t.dtype], stride
+def _row_stride(t, n, C, what):
+    """The row stride of a 2-d tensor [n, C] whose rows may lie further apart than C."""
+    if t.dim() == 2 and t.dtype in _TYPES:
+        rows, columns = t.shape
+        if rows == n and columns == C:
+            stride, inner = t.stride()
+            if n <= 1:
+                stride = max(stride, C)
+            if (inner == 1 or C == 1) and stride >= C:
+                return stride
+            raise ScnError("invalid argument: %s: the values of a row must lie together and rows must not overlap" % what)
+    raise ScnError("invalid argument: %s must be a CUDA tensor [%d, %d] of float32, bfloat16 or float16" % (what, n, C))
 
 
-def _tokens_of(tokens, device):
-    if tokens.dtype != torch.int32 or tokens.dim() != 1 or not tokens.is_contiguous() or tokens.device != device:
-        raise ScnError("invalid argument: tokens must be a contiguous 1-d int32 tensor on the other arguments' device")
-    return tokens.data_ptr(), tokens.numel()
-
-
-def _optional_i32(t, device, what):
-    if t is None:
-        return None
-    if t.dtype != torch.int32 or t.numel() < 1 or not t.is_contiguous() or t.device != device:
-        raise ScnError("invalid argument: %s must be an int32 tensor on the other arguments' device" % what)
-    return t.data_ptr()
+def _check_tokens(tokens, errors):
+    if tokens.dtype != torch.int32 or tokens.dim() != 1 or not tokens.is_contiguous():
+        raise ScnError("invalid argument: tokens must be a contiguous 1-d int32 tensor")
+    if errors is not None and (errors.dtype != torch.int32 or errors.numel() < 1 or not errors.is_contiguous()):
+        raise ScnError("invalid argument: errors must be an int32 tensor")
 
 
 def embedding_forward(table, tokens, scale=1.0, out=None, out_dtype=torch.float32, errors=None):
     """scn_embedding_forward: scale * table[tokens] as a new tensor [n, C] of out_dtype, or into `out` (a view with a row
     stride is fine).  errors: int32 tensor that gets DEV_ERR_KEY or-ed in where a token is not below the table's rows."""
-    dev = table.device
-    _here(dev)
+    _on_current_device(table, tokens, out, errors)
     if table.dim() != 2 or table.dtype not in _TYPES or not table.is_contiguous():
         raise ScnError("invalid argument: the table must be a contiguous 2-d tensor of float32, bfloat16 or float16")
+    _check_tokens(tokens, errors)
     V, C = table.shape
-    ptr, n = _tokens_of(tokens, dev)
+    n = tokens.numel()
     if out is None:
-        out = torch.empty((n, C), dtype=out_dtype, device=dev)
-    elif out.device != dev:
-        raise ScnError("invalid argument: out is on another device")
-    optr, otype, stride = _rows_of(out, n, C, "out")
-    check(lib().scn_embedding_forward(table.data_ptr(), _TYPES[table.dtype], V, C, ptr, n, scale, optr, otype, stride,
-                                      _optional_i32(errors, dev, "errors"), _raw_stream()))
+        out = torch.empty((n, C), dtype=out_dtype, device=table.device)
+    stride = _row_stride(out, n, C, "out")
+    check(lib().scn_embedding_forward(table.data_ptr(), _TYPES[table.dtype], V, C, tokens.data_ptr(), n, scale, out.data_ptr(), _TYPES[out.dtype], stride,
+                                      None if errors is None else errors.data_ptr(), _raw_stream()))
     return out
 
 
@@ -638,22 +640,19 @@ def embedding_backward_workspace(n, vocab, C, device):
 def embedding_backward(dout, tokens, dtable, scale=1.0, accumulate=False, workspace=None, errors=None):
     """scn_embedding_backward: the gradient of embedding_forward's table into the float32 tensor dtable [vocab, C] (added
     onto it with `accumulate`); returns dtable.  workspace: embedding_backward_workspace(n, vocab, C, device), to keep."""
-    dev = dtable.device
-    _here(dev)
+    _on_current_device(dout, tokens, dtable, workspace, errors)
     if dtable.dim() != 2 or dtable.dtype != torch.float32 or not dtable.is_contiguous():
         raise ScnError("invalid argument: dtable must be a contiguous 2-d float32 tensor")
+    _check_tokens(tokens, errors)
     V, C = dtable.shape
-    ptr, n = _tokens_of(tokens, dev)
-    if dout.device != dev:
-        raise ScnError("invalid argument: dout is on another device")
-    dptr, dtype, stride = _rows_of(dout, n, C, "dout")
+    n = tokens.numel()
+    stride = _row_stride(dout, n, C, "dout")
     if workspace is None:
-        workspace = embedding_backward_workspace(n, V, C, dev)
-    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise ScnError("invalid argument: the workspace must be a uint8 tensor on the other arguments' device")
-    check(lib().scn_embedding_backward(ptr, n, dptr, dtype, stride, V, C, scale, int(accumulate), dtable.data_ptr(),
-                                       _optional_i32(errors, dev, "errors"), workspace.data_ptr(), workspace.numel(),
-                                       _raw_stream()))
+        workspace = embedding_backward_workspace(n, V, C, dtable.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ScnError("invalid argument: the workspace must be a contiguous uint8 tensor")
+    check(lib().scn_embedding_backward(tokens.data_ptr(), n, dout.data_ptr(), _TYPES[dout.dtype], stride, V, C, scale, accumulate, dtable.data_ptr(),
+                                       None if errors is None else errors.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream()))
     return dtable
 
 
@@ -724,50 +723,58 @@ class AdamW:
                 written = max(written, last)
         self.h = AdamWParameters()
         self._h = ctypes.byref(self.h)
+        self._set = None  # the numbers that h holds
         self._norm = torch.empty((), device=self.device)
-        self._workspace = torch.empty(lib().scn_grad_norm_workspace_bytes(), dtype=torch.uint8, device=self.device)
+        self._workspace_bytes = lib().scn_grad_norm_workspace_bytes()
+        self._workspace = torch.empty(self._workspace_bytes, dtype=torch.uint8, device=self.device)
+        self._norm_ptr, self._workspace_ptr = self._norm.data_ptr(), self._workspace.data_ptr()
 
     def grad_norm(self):
         """The 2-norm of all gradients as a float32 tensor of no dimensions that this object owns."""
-        _here(self.device)
-        check(lib().scn_grad_norm(self.list, self.count, self._norm.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(),
-                                  _raw_stream()))
+        _on_current_device(self._norm)
+        check(lib().scn_grad_norm(self.list, self.count, self._norm_ptr, self._workspace_ptr, self._workspace_bytes, _raw_stream()))
         return self._norm
 
     def step(self, lr=None, step=None, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, seed=None, norm=None, max_norm=0.0, scalars=None):
         """Step number `step` (from 1).  seed: of the 8-bit states' rounding (the step number unless given).  norm: what
         grad_norm() returned, for max_norm > 0.  scalars: a CUDA copy of adamw_scalars(...) instead of the numbers, for a
         captured step."""
-        _here(self.device)
+        _on_current_device(self._norm, norm, scalars)
         if scalars is not None:
             if lr is not None or step is not None:
                 raise ScnError("invalid argument: pass the numbers or the scalars, not both")
-            if scalars.dtype != torch.int32 or scalars.numel() != 12 or scalars.device != self.device or not scalars.is_contiguous():
+            if scalars.dtype != torch.int32 or scalars.numel() != 12 or not scalars.is_contiguous():
                 raise ScnError("invalid argument: scalars must be a CUDA copy of adamw_scalars(...)")
             h, sp = None, scalars.data_ptr()
         else:
             if lr is None or step is None:
                 raise ScnError("invalid argument: a step needs lr and its number")
-            p = self.h
-            p.lr, p.beta1, p.beta2, p.eps, p.grad_scale, p.max_norm, p.step = lr, beta1, beta2, eps, grad_scale, max_norm, step
-            p.seed = (step if seed is None else seed) & 0xFFFFFFFF
+            numbers = (lr, beta1, beta2, eps, grad_scale, max_norm, step, step if seed is None else seed)
+            if numbers != self._set:
+                p = self.h
+                p.lr, p.beta1, p.beta2, p.eps, p.grad_scale, p.max_norm, p.step, p.seed = numbers[:7] + (numbers[7] & 0xFFFFFFFF,)
+                self._set = numbers
             h, sp = self._h, None
-        if norm is not None and (norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != self.device):
-            raise ScnError("invalid argument: norm must be a float32 tensor of one value on the tensors' device")
-        check(lib().scn_adamw_step(self.list, self.count, h, sp, None if norm is None else norm.data_ptr(),
-                                   _raw_stream()))
+        if norm is None:
+            np = None
+        elif norm is self._norm:
+            np = self._norm_ptr
+        elif norm.dtype != torch.float32 or norm.numel() != 1:
+            raise ScnError("invalid argument: norm must be a float32 tensor of one value")
+        else:
+            np = norm.data_ptr()
+        check(lib().scn_adamw_step(self.list, self.count, h, sp, np, _raw_stream()))
 
 
 def adamw_decode(codes, scale):
     """What 8-bit moments stand for, as a new float32 tensor: codes int8 (first moment) or uint8 (second)."""
-    n = codes.numel()
-    if codes.dtype not in (torch.int8, torch.uint8) or not codes.is_contiguous() or scale.dtype != torch.float32 or not scale.is_contiguous() \
-            or scale.numel() != -(-n // ADAMW_BLOCK) or scale.device != codes.device:
+    _on_current_device(codes, scale)
+    n, dtype = codes.numel(), codes.dtype
+    if (dtype != torch.int8 and dtype != torch.uint8) or not codes.is_contiguous() or scale.dtype != torch.float32 or not scale.is_contiguous() \
+            or scale.numel() != -(-n // ADAMW_BLOCK):
         raise ScnError("invalid argument: codes must be int8 or uint8 with a float32 scale for each %d of them" % ADAMW_BLOCK)
-    _here(codes.device)
-    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
-    check(lib().scn_adamw_decode(codes.data_ptr(), scale.data_ptr(), n, int(codes.dtype == torch.uint8), out.data_ptr(),
-                                 _raw_stream()))
+    out = torch.empty_like(codes, dtype=torch.float32)
+    check(lib().scn_adamw_decode(codes.data_ptr(), scale.data_ptr(), n, dtype == torch.uint8, out.data_ptr(), _raw_stream()))
     return out
 
 

@@ -206,45 +206,44 @@ __device__ __forceinline__ int scale_exponent(float most, float top, int bits) {
   e = max(e, -126);
   return most > top * power_of_two(e) ? e + 1 : e;
 }
-// floor(r) for 0 <= r < 2^22, of an r made a little smaller first, so that an approximate root never comes out too large:
-// adding 2^23 with rounding down leaves the whole part.
-__device__ __forceinline__ float2 floor_below(float2 r) { return add(__fadd2_rd(mul(r, both(1.f - 0x1p-20f)), both(8388608.f)), both(-8388608.f)); }
-// Largest whole q with q^2 <= x (the comparison decides; floor_below is right or one too small), then one more where
-// the dither says so.  (x - q^2 and 2 q + 1 are exact.)
+// 1 where x is above 0, else 0, for an x that is 0 or at least 2^-50 away from it.
+__device__ __forceinline__ float2 positive(float2 x) { return make_float2(__saturatef(x.x * 0x1p60f), __saturatef(x.y * 0x1p60f)); }
+__device__ __forceinline__ float2 nearest(float2 r) { return add(add(r, both(8388608.f)), both(-8388608.f)); } // 0 <= r < 2^22
+// The largest whole q with q^2 <= x, then one more where x lies further above q^2 than u times the step to (q + 1)^2.  The
+// whole number nearest to an approximate root is q or q + 1; which one, and what the dither decides, comes from differences
+// that are 0 or at least 2^-41 (u is no smaller than 2^-17), so a multiplication that saturates tells their signs.
+// (x - q^2 and 2 q + 1 are exact.)
 __device__ __forceinline__ float2 code_m(float2 x, float2 u) {
-  float2 q = floor_below(make_float2(root(x.x), root(x.y)));
-  const float2 next = add(q, both(1.f)), square = mul(next, next);
-  q.x = square.x <= x.x ? next.x : q.x;
-  q.y = square.y <= x.y ? next.y : q.y;
+  float2 q = nearest(make_float2(root(x.x), root(x.y)));
+  q = sub(q, positive(__ffma2_rn(q, q, make_float2(-x.x, -x.y))));
   const float2 over = sub(x, mul(q, q)), limit = mul(u, __ffma2_rn(q, both(2.f), both(1.f)));
-  if (over.x > limit.x) q.x += 1.f;
-  if (over.y > limit.y) q.y += 1.f;
-  return q;
+  return add(q, positive(sub(over, limit)));
 }
 __device__ __forceinline__ float2 fourth(float2 q) { q = mul(q, q); return mul(q, q); }
 __device__ __forceinline__ float2 code_v(float2 y, float2 u) {
-  float2 q = floor_below(make_float2(root(root(y.x)), root(root(y.y))));
-  const float2 next = add(q, both(1.f)), power = fourth(next);
-  q.x = power.x <= y.x ? next.x : q.x;
-  q.y = power.y <= y.y ? next.y : q.y;
-  const float2 low = fourth(q), over = sub(y, low), limit = mul(u, sub(fourth(add(q, both(1.f))), low));
-  if (over.x > limit.x) q.x += 1.f;
-  if (over.y > limit.y) q.y += 1.f;
-  return q;
+  float2 q = nearest(make_float2(root(root(y.x)), root(root(y.y))));
+  q = sub(q, positive(sub(fourth(q), y)));
+  const float2 low = fourth(q), limit = mul(u, sub(fourth(add(q, both(1.f))), low));
+  return add(q, positive(sub(sub(y, low), limit)));
 }
 // A 32-bit mix of a position and the seed: multiplications by odd numbers (the fractional bits of the square roots of 2, 3,
-// 5 and 7) between shifts that bring the high bits down.
-__device__ __forceinline__ unsigned mix(unsigned at, unsigned key) {
+// 5 and 7) between shifts that bring the high bits down.  Its two halves, the lower one with the upper one mixed in once more,
+// become (b + 1/2) / 2^16 each: the bits lie in the upper places of a fraction of 1.
+__device__ __forceinline__ void dither(unsigned at, unsigned key, float &um, float &uv) {
   unsigned h = at * 0x6A09E667u + key;
   h ^= h >> 16;
   h *= 0xBB67AE85u;
   h ^= h >> 15;
   h *= 0x3C6EF373u;
-  return h ^ h >> 16;
+  const unsigned upper = ((h >> 9) & 0x7FFF80u) | 0x3F800000u;
+  uv = __uint_as_float(upper);
+  um = __uint_as_float(((h << 7) & 0x7FFF80u) ^ upper);
 }
-// (b + 1/2) / 2^16 of the 16 bits at bit 7 of x and of y: they become the upper bits of fractions of 1.
-__device__ __forceinline__ float2 dither(unsigned x, unsigned y) {
-  return add(make_float2(__uint_as_float((x & 0x7FFF80u) | 0x3F800000u), __uint_as_float((y & 0x7FFF80u) | 0x3F800000u)), both(0x1p-17f - 1.f));
+constexpr float DITHER = 0x1p-17f - 1.f; // to be added to both
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 // Bytes K and K + 1 of a word as floats: the byte in the low bits of 2^23, less 2^23 (less 2^23 + 128 where every sign bit
 // has been turned over).
@@ -259,11 +258,11 @@ template <int K> __device__ __forceinline__ float2 decode_m(unsigned word, float
 template <int K> __device__ __forceinline__ float2 decode_v(unsigned word, float s) { return mul(fourth(bytes_of<K>(word, UNSIGNED)), both(s)); }
 
 // A warp takes one block, a lane eight consecutive values of it.  Values behind the end of the tensor count as zeros.
-// The largest |m| and v are found as whole numbers: the bits of floats that are not negative are in the floats' order, and what
-// is not finite lies above all of them.
+// The largest |m| and v of the lanes are compared as whole numbers: the bits of floats that are not negative are in the floats' order,
+// and what is not finite lies above all of them.
 constexpr unsigned NOT_FINITE = 0x7F800000u;
 template <int CAP>
-__global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
+__global__ void __launch_bounds__(THREADS, 5) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   const Tensor &t = l.t[owner(l, blockIdx.x)];
   const int lane = threadIdx.x & 31;
   long long block = (long long)((int)blockIdx.x - t.chunk) * l.turns * WARPS + (threadIdx.x >> 5);
@@ -302,7 +301,7 @@ __global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ Lis
       m[2 * k] = decode_m<0>(turned, sm); m[2 * k + 1] = decode_m<2>(turned, sm);
       v[2 * k] = decode_v<0>(vw[k], sv); v[2 * k + 1] = decode_v<2>(vw[k], sv);
     }
-    unsigned mostM = 0, mostV = 0;
+    float topM = 0.f, topV = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       moments(h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
@@ -312,15 +311,14 @@ __global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ Lis
         if (i + 2 * k >= t.n) m[k].x = v[k].x = 0.f;
         if (i + 2 * k + 1 >= t.n) m[k].y = v[k].y = 0.f;
       }
-      mostM = max(mostM, max(__float_as_uint(fabsf(m[k].x)), __float_as_uint(fabsf(m[k].y))));
-      mostV = max(mostV, max(__float_as_uint(v[k].x), __float_as_uint(v[k].y)));
+      topM = max_abs_nan(topM, m[k].x, m[k].y);
+      topV = max_abs_nan(topV, v[k].x, v[k].y);
     }
     if (wide) {
       store8(t.w + i, w);
       if (t.w16) store8_typed(t.w16, t.w16type, i, w);
     }
-    mostM = __reduce_max_sync(~0u, mostM);
-    mostV = __reduce_max_sync(~0u, mostV);
+    const unsigned mostM = __reduce_max_sync(~0u, __float_as_uint(topM)), mostV = __reduce_max_sync(~0u, __float_as_uint(topV));
     const bool lost = max(mostM, mostV) >= NOT_FINITE;
     const int em = lost ? 0 : scale_exponent(__uint_as_float(mostM), TOP_M, 13), ev = lost ? 0 : scale_exponent(__uint_as_float(mostV), TOP_V, 31);
     if (lane == 0) {
@@ -330,18 +328,30 @@ __global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ Lis
     const float im = power_of_two(-em), iv = power_of_two(-ev);
     const unsigned long long at0 = (t.block + block) * BLOCK;
     const unsigned at = (unsigned)at0 + lane * 8, key = h.seed * 0xBB67AE85u + (unsigned)(at0 >> 32) * 0xA54FF53Bu;
+    float2 qv[4], product = both(1.f);
     unsigned mb[8], vb[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const unsigned r = mix(at + 2 * k, key), s = mix(at + 2 * k + 1, key);
-      float2 qm = code_m(make_float2(__fmul_rn(fabsf(m[k].x), im), __fmul_rn(fabsf(m[k].y), im)), dither(r << 7, s << 7));
-      float2 qv = code_v(mul(v[k], both(iv)), dither(r >> 9, s >> 9));
-      if (v[k].x > 0.f) qv.x = fmaxf(qv.x, 1.f);
-      if (v[k].y > 0.f) qv.y = fmaxf(qv.y, 1.f);
-      qm = add(make_float2(copysignf(qm.x, m[k].x), copysignf(qm.y, m[k].y)), both(SIGNED)); // the bytes in the low bits again
-      qv = add(qv, both(UNSIGNED));
-      mb[2 * k] = __float_as_uint(qm.x); mb[2 * k + 1] = __float_as_uint(qm.y);
-      vb[2 * k] = __float_as_uint(qv.x); vb[2 * k + 1] = __float_as_uint(qv.y);
+      float2 um, uv;
+      dither(at + 2 * k, key, um.x, uv.x);
+      dither(at + 2 * k + 1, key, um.y, uv.y);
+      const float2 qm = code_m(make_float2(__fmul_rn(fabsf(m[k].x), im), __fmul_rn(fabsf(m[k].y), im)), add(um, both(DITHER)));
+      qv[k] = code_v(mul(v[k], both(iv)), add(uv, both(DITHER)));
+      product = mul(product, qv[k]);
+      const float2 bytes = add(make_float2(copysignf(qm.x, m[k].x), copysignf(qm.y, m[k].y)), both(SIGNED)); // the bytes in the low bits again
+      mb[2 * k] = __float_as_uint(bytes.x); mb[2 * k + 1] = __float_as_uint(bytes.y);
+    }
+    if (product.x * product.y == 0.f) { // a second moment's code is 0: only if it is 0 itself
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (v[k].x > 0.f) qv[k].x = fmaxf(qv[k].x, 1.f);
+        if (v[k].y > 0.f) qv[k].y = fmaxf(qv[k].y, 1.f);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 bytes = add(qv[k], both(UNSIGNED));
+      vb[2 * k] = __float_as_uint(bytes.x); vb[2 * k + 1] = __float_as_uint(bytes.y);
     }
     const auto pack = [](const unsigned *b) { return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410); };
 #pragma unroll
@@ -364,16 +374,20 @@ __global__ void __launch_bounds__(THREADS) k_adamw_8(const __grid_constant__ Lis
     }
   }
 }
-// Four codes a thread where the arrays are aligned for it (`wide`: so many values are), then one by one.
+// Eight codes a thread where the arrays are aligned for it (`wide`: so many values are), then one by one.
 __global__ void __launch_bounds__(THREADS) k_adamw_decode(const unsigned char *codes, const float *scale, long long n, long long wide, int second, float *out) {
   const long long step = (long long)gridDim.x * THREADS, self = blockIdx.x * (long long)THREADS + threadIdx.x;
-  for (long long j = self; j < wide / 4; j += step) {
-    const unsigned q = ((const unsigned *)codes)[j];
-    const float s = scale[j / (BLOCK / 4)];
-    float2 a, b;
-    if (second) { a = decode_v<0>(q, s); b = decode_v<2>(q, s); }
-    else { a = decode_m<0>(q ^ 0x80808080u, s); b = decode_m<2>(q ^ 0x80808080u, s); }
-    ((float4 *)out)[j] = make_float4(a.x, a.y, b.x, b.y);
+  for (long long j = self; j < wide / 8; j += step) {
+    const uint2 q = ((const uint2 *)codes)[j];
+    const float s = scale[j / (BLOCK / 8)];
+    float2 x[4];
+    if (second) { x[0] = decode_v<0>(q.x, s); x[1] = decode_v<2>(q.x, s); x[2] = decode_v<0>(q.y, s); x[3] = decode_v<2>(q.y, s); }
+    else {
+      const unsigned a = q.x ^ 0x80808080u, b = q.y ^ 0x80808080u;
+      x[0] = decode_m<0>(a, s); x[1] = decode_m<2>(a, s); x[2] = decode_m<0>(b, s); x[3] = decode_m<2>(b, s);
+    }
+    const float o[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+    store8(out + 8 * j, o);
   }
   for (long long i = wide + self; i < n; i += step)
     out[i] = second ? decode_v<0>(codes[i], scale[i / BLOCK]).x : decode_m<0>(codes[i] ^ 0x80u, scale[i / BLOCK]).x;
@@ -523,8 +537,8 @@ extern "C" int scn_adamw_decode(const void *d_codes, const float *d_scale, long 
   if (n < 0) return fail(SCN_ERR_INVALID, "bad size");
   if (n == 0) return SCN_OK;
   if (!d_codes || !d_scale || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
-  const long long wide = (((uintptr_t)d_codes & 3) | ((uintptr_t)d_out & 15)) == 0 ? n / 4 * 4 : 0;
-  k_adamw_decode<<<grid_for((n + 3) / 4, THREADS, 32), THREADS, 0, (cudaStream_t)stream>>>((const unsigned char *)d_codes, d_scale, n, wide, second, d_out);
+  const long long wide = (((uintptr_t)d_codes & 7) | ((uintptr_t)d_out & 31)) == 0 ? n / 8 * 8 : 0;
+  k_adamw_decode<<<grid_for((n + 7) / 8, THREADS, 32), THREADS, 0, (cudaStream_t)stream>>>((const unsigned char *)d_codes, d_scale, n, wide, second, d_out);
   SCN_LAUNCH_CHECK("k_adamw_decode");
   return SCN_OK;
 }

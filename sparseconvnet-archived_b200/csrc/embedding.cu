@@ -52,6 +52,43 @@ __global__ void __launch_bounds__(THREADS) k_embedding_forward(const T *__restri
     }
   }
 }
+// The same value by value, for widths, strides and addresses that allow no more: a warp takes ROWS rows and 32 * COLS columns at
+// once, so that about as many bytes are on their way.
+template <class T, class O, int ROWS, int COLS>
+__global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const T *__restrict__ table, int vocab, int C, const int *__restrict__ tokens, long long n,
+                                                                      float scale, O *__restrict__ out, long long stride, int *errors) {
+  const int lane = threadIdx.x & 31;
+  const long long step = (long long)gridDim.x * WARPS * ROWS;
+  for (long long i = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS; i < n; i += step) {
+    int mine = lane < ROWS && i + lane < n ? __ldg(tokens + i + lane) : -1;
+    if (mine >= vocab) {
+      if (errors) atomicOr(errors, SCN_DEV_ERR_KEY);
+      mine = -1;
+    }
+    const T *from[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int t = __shfl_sync(~0u, mine, u);
+      from[u] = t >= 0 ? table + (long long)t * C : nullptr;
+    }
+    for (int c = lane; c - lane < C; c += 32 * COLS) {
+      T v[ROWS][COLS];
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+          if (from[u] && c + 32 * j < C) v[u][j] = __ldg(from[u] + c + 32 * j);
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        if (i + u >= n) break;
+        O *to = out + (i + u) * stride + c;
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+          if (c + 32 * j < C) __stcs(to + 32 * j, from_float<O>(from[u] ? to_float(v[u][j]) * scale : 0.f));
+      }
+    }
+  }
+}
 // Threads of a group for rows of so many W-value pieces: all of them at once up to MAX_LANES, else in equal turns.
 int lanes_for(int vectors) {
   const int turns = (vectors + MAX_LANES - 1) / MAX_LANES;
@@ -63,6 +100,16 @@ template <class T, class O> void launch_forward(const T *table, int vocab, int C
   constexpr int MOST = 16 / (int)sizeof(T);
   int W = MOST;
   while (W > 1 && !(C % W == 0 && stride % W == 0 && (uintptr_t)table % (W * sizeof(T)) == 0 && (uintptr_t)out % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
+  if (W == 1 && C > 16) {
+    const auto single = [&](auto kernel, int rows) {
+      kernel<<<(int)std::min((n + WARPS * rows - 1) / (WARPS * rows), 16ll * sm_count()), THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, errors);
+    };
+    if (C <= 32) single(k_embedding_forward_single<T, O, 16, 1>, 16);
+    else if (C <= 64) single(k_embedding_forward_single<T, O, 8, 2>, 8);
+    else if (C <= 96) single(k_embedding_forward_single<T, O, 5, 3>, 5);
+    else single(k_embedding_forward_single<T, O, 4, 4>, 4);
+    return;
+  }
   const int lanes = lanes_for(C / W), groups = THREADS / lanes;
   const auto launch = [&](auto kernel, int rows) {
     const int grid = (int)std::min((n + groups * rows - 1) / (groups * rows), 16ll * sm_count());
@@ -308,7 +355,7 @@ struct Sums {
   const uint2 *entries;        // (token, row), sorted
   int n, vocab, C, tile;       // tile: entries a warp
   unsigned stride;             // of dout's rows, in bytes
-  int lanes;                   // threads of a group in the last slab (32 in the others); a slab is lanes * W columns
+  int lanes;                   // threads of a group in the last slab (32 in the others); a slab is lanes * W columns (times J)
   float scale;
   int accumulate;
   float *dtable;
@@ -348,27 +395,31 @@ template <int W> __device__ __forceinline__ void write_row(const Sums &p, unsign
   }
 }
 // The sums of a warp's `count` sorted entries in shared memory, all of them of tokens, with SUM_ROWS more entries behind them that
-// name any row of dout; before, after: the tokens around them.  item[2 g], item[2 g + 1]: what group g's run holds of its first
-// and last token (0 for the last one where the run holds one token only), so that the items' tokens ascend.  head, tail: where
-// the parts go that other warps have to do with.
-template <int W> struct Items {
-  unsigned key[64];
-  float sum[64 * W];
+// name any row of dout; before, after: the tokens around them.  A slab is J pieces of lanes * W columns side by side (J > 1: for
+// single values, with 32 lanes), a thread takes W columns of each.  item[2 g], item[2 g + 1]: what group g's run holds of its
+// first and last token (0 for the last one where the run holds one token only), so that the items' tokens ascend.  head, tail:
+// where the parts go that other warps have to do with.
+template <int W, int J> struct Items {
+  unsigned key[J > 1 ? 2 : 64];
+  float sum[64 * W * J];
 };
-template <class T, int W>
-__device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const uint2 *entry, int count, unsigned before, unsigned after, Items<W> &items, float *head,
+template <class T, int W, int J>
+__device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const uint2 *entry, int count, unsigned before, unsigned after, Items<W, J> &items, float *head,
                                           float *tail) {
   const unsigned none = p.vocab;
-  const int lanes = blockIdx.y + 1 < gridDim.y ? 32 : p.lanes, groups = 32 / lanes, width = lanes * W, column0 = blockIdx.y * 32 * W;
+  const int lanes = J > 1 || blockIdx.y + 1 < gridDim.y ? 32 : p.lanes, groups = J > 1 ? 1 : 32 / lanes, width = lanes * W * J, column0 = blockIdx.y * 32 * W * J;
   const int lane = threadIdx.x & 31, group = lane / lanes, column = (lane - group * lanes) * W, c = column0 + column;
   const int each = (count + groups - 1) / groups, begin = min(group * each, count), end = group < groups && c < p.C ? min(begin + each, count) : begin;
-  Columns<W> sum;
-  sum.clear();
+  Columns<W> sum[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) sum[j].clear();
   unsigned now = begin < end ? entry[begin].x : none;
   bool atHead = true;
   const auto to_item = [&](int at) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) items.sum[at * width + column + w] = sum.at(w);
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int w = 0; w < W; ++w) items.sum[at * width + column + 32 * W * j + w] = sum[j].at(w);
     if (column == 0) items.key[at] = now;
   };
   const char *from = (const char *)(dout + c);
@@ -376,12 +427,19 @@ __device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const ui
     __syncwarp(); // the groups part where their tokens change, and ask for their next rows together
     const int i = begin + s;
     if (i >= end) continue;
-    Pack<T, W> v[SUM_ROWS];
+    Pack<T, W> v[SUM_ROWS][J];
 #pragma unroll
-    for (int u = 0; u < SUM_ROWS; ++u) v[u] = load_pack<T, W>((const T *)(from + (unsigned long long)entry[i + u].y * p.stride));
+    for (int u = 0; u < SUM_ROWS; ++u) {
+      const T *row = (const T *)(from + (unsigned long long)entry[i + u].y * p.stride);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (j == 0 || c + 32 * W * j < p.C) v[u][j] = load_pack<T, W>(row + 32 * W * j);
+    }
     if (i + SUM_ROWS <= end && entry[i + SUM_ROWS - 1].x == now) { // one token all along
 #pragma unroll
-      for (int u = 0; u < SUM_ROWS; ++u) sum.add(v[u]);
+      for (int u = 0; u < SUM_ROWS; ++u)
+#pragma unroll
+        for (int j = 0; j < J; ++j) sum[j].add(v[u][j]);
       continue;
     }
 #pragma unroll
@@ -390,19 +448,26 @@ __device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const ui
         const unsigned k = entry[i + u].x;
         if (k != now) {
           if (atHead) to_item(2 * group);
-          else write_row<W>(p, now, c, sum);
+          else {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+              if (j == 0 || c + 32 * W * j < p.C) write_row<W>(p, now, c + 32 * W * j, sum[j]);
+          }
           atHead = false;
           now = k;
-          sum.clear();
+#pragma unroll
+          for (int j = 0; j < J; ++j) sum[j].clear();
         }
-        sum.add(v[u]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) sum[j].add(v[u][j]);
       }
     }
   }
   if (group < groups) {
     to_item(2 * group + (atHead ? 0 : 1));
     if (atHead) {
-      sum.clear();
+#pragma unroll
+      for (int j = 0; j < J; ++j) sum[j].clear();
       to_item(2 * group + 1);
     }
   }
@@ -425,9 +490,9 @@ __device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const ui
     }
   }
 }
-template <class T, int W> __global__ void __launch_bounds__(THREADS, 4) k_embedding_sums(const Sums p, const T *dout) {
+template <class T, int W, int J> __global__ void __launch_bounds__(THREADS, 4) k_embedding_sums(const Sums p, const T *dout) {
   __shared__ uint2 entries[WARPS][MAX_TILE + SUM_ROWS];
-  __shared__ Items<W> items[WARPS];
+  __shared__ Items<W, J> items[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_prior_grids();
   dependents_may_launch();
@@ -452,18 +517,18 @@ template <class T, int W> __global__ void __launch_bounds__(THREADS, 4) k_embedd
   __syncwarp();
   if (lane < SUM_ROWS) entry[count + lane] = make_uint2(none, any);
   __syncwarp();
-  warp_sums<T, W>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
+  warp_sums<T, W, J>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
 }
 // The whole gradient of at most SMALL rows in one launch: the first CTAs (one a slab) sort the entries in shared memory and
 // add them up; the others write the zeros of the rows that no token names, each for a range of `range` rows.
 constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
-template <class T, int W>
+template <class T, int W, int J>
 __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums p, const T *dout, const int *tokens, int bits, int range, int *errors) {
   __shared__ uint2 entries[2][SMALL + SUM_ROWS];
   __shared__ union {
     unsigned present[MOST_RANGE / 32];             // (the CTAs that write zeros)
     unsigned short count[WARPS << SMALL_DIGIT];    // (while sorting)
-    Items<W> items[WARPS];
+    Items<W, J> items[WARPS];
   } sh;
   __shared__ unsigned warpSum[WARPS], all;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -519,11 +584,11 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
   __syncthreads();
   if (threadIdx.x < SUM_ROWS) now[count + threadIdx.x] = make_uint2(none, any);
   __syncthreads();
-  const int tile = (count + WARPS - 1) / WARPS, first = min(warp * tile, count), end = min(first + tile, count), column0 = blockIdx.y * 32 * W;
-  const int width = (blockIdx.y + 1 < gridDim.y ? 32 : p.lanes) * W;
+  const int tile = (count + WARPS - 1) / WARPS, first = min(warp * tile, count), end = min(first + tile, count), column0 = blockIdx.y * 32 * W * J;
+  const int width = (J > 1 || blockIdx.y + 1 < gridDim.y ? 32 : p.lanes) * W * J;
   const auto key_at = [&](int i) { return i >= 0 && i < count ? now[i].x : none; };
   if (first < end) // (a warp's head and tail take the places of its first two items, read by then)
-    warp_sums<T, W>(p, dout, now + first, end - first, key_at(first - 1), key_at(end), sh.items[warp], sh.items[warp].sum - column0,
+    warp_sums<T, W, J>(p, dout, now + first, end - first, key_at(first - 1), key_at(end), sh.items[warp], sh.items[warp].sum - column0,
                     sh.items[warp].sum + width - column0);
   __syncthreads();
   if (first >= end) return;
@@ -733,22 +798,25 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     return SCN_OK;
   }
   char *w = (char *)d_workspace;
-  const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W, slabs = (vectors + 31) / 32;
+  const int W = pack_width(dout_type, d_dout, dout_stride, d_dtable, C), vectors = C / W;
+  const int J = W > 1 || C <= 32 ? 1 : C <= 64 ? 2 : 4, slabs = (vectors + 32 * J - 1) / (32 * J); // (see warp_sums)
   Sums q = {};
   q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = (unsigned)(dout_stride * type_bytes(dout_type));
-  q.lanes = vectors - (slabs - 1) * 32;
+  q.lanes = J > 1 ? 32 : vectors - (slabs - 1) * 32;
   q.tile = sum_tile(n);
   q.scale = scale; q.accumulate = accumulate; q.dtable = d_dtable;
   q.head = (float *)(w + 2 * sp.array + sp.counts + sp.totals);
   q.tail = (float *)(w + 2 * sp.array + sp.counts + sp.totals + sp.parts);
-  // F<T, W> for dout's type and the width
+  // F<T, W, J> for dout's type, the width and the pieces
 #define SCN_SUMS(F, ...)                                                                                              \
   SCN_DISPATCH_TYPE(dout_type, T, {                                                                                   \
     constexpr int MOST = 16 / (int)sizeof(T);                                                                         \
-    if (W == MOST) SCN_CUDA_TRY(launch_dependent(F<T, MOST>, __VA_ARGS__));                                           \
-    else if (W == MOST / 2) SCN_CUDA_TRY(launch_dependent(F<T, MOST / 2>, __VA_ARGS__));                              \
-    else if (W == 1) SCN_CUDA_TRY(launch_dependent(F<T, 1>, __VA_ARGS__));                                            \
-    else SCN_CUDA_TRY(launch_dependent(F<T, 2>, __VA_ARGS__));                                                        \
+    if (W == MOST) SCN_CUDA_TRY(launch_dependent(F<T, MOST, 1>, __VA_ARGS__));                                        \
+    else if (W == MOST / 2) SCN_CUDA_TRY(launch_dependent(F<T, MOST / 2, 1>, __VA_ARGS__));                           \
+    else if (W == 2) SCN_CUDA_TRY(launch_dependent(F<T, 2, 1>, __VA_ARGS__));                                         \
+    else if (J == 1) SCN_CUDA_TRY(launch_dependent(F<T, 1, 1>, __VA_ARGS__));                                         \
+    else if (J == 2) SCN_CUDA_TRY(launch_dependent(F<T, 1, 2>, __VA_ARGS__));                                         \
+    else SCN_CUDA_TRY(launch_dependent(F<T, 1, 4>, __VA_ARGS__));                                                     \
   })
   if (n <= SMALL) {
     const int range = std::max(32, std::min(MOST_RANGE, (vocab + 4 * sm_count() - 1) / (4 * sm_count()))), clearing = accumulate ? 0 : (vocab + range - 1) / range;
