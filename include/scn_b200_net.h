@@ -88,6 +88,27 @@ int scn_net_forward_host(scn_net_t *net, int batch, const int *h_keys, const int
  * batch (NetworkInNetworkLayer.cu:152-154): the others are zero in the forward pass and untouched by the update. */
 int scn_net_train_batch(scn_net_t *net, int batch, const int *h_keys, const int *h_off, const float *h_features, const int *h_labels,
                         float learningRate, float momentum, float *h_probs, double *stats);
+/* Training by AdamW instead of the reference's momentum SGD (scn_adamw_step in scn_b200.h gives the formula): one step over all
+ * learnt layers' weights, biases and slopes (and the symbol table) behind a training batch's backward pass, on gradients
+ * averaged over the batch; `momentum` of the training calls is then not used.  weight_decay applies to matrices and the
+ * table; max_norm > 0 clips the gradients' common norm (a norm that is not finite leaves the weights alone); state_bits: 32,
+ * or 8 for moments in 8 bits, or 0 to return to SGD.  The moments start at zero with this call; weight files do not hold them.
+ * Weights of features that a batch drops see gradients of zero (SGD skips them).  An index learner layer goes on updating itself. */
+int scn_net_use_adamw(scn_net_t *net, float beta1, float beta2, float eps, float weight_decay, float max_norm, int state_bits);
+
+/* Inputs whose rows carry a code instead of features: a table h_table [n_symbols x nInputFeatures] turns symbol s into the
+ * features scale * table[s] (scn_embedding_forward; a negative symbol, a background row's say, into zeros), and training
+ * batches of symbols learn it as well (scn_embedding_backward).  Call it before scn_net_use_adamw if it replaces a table.
+ * Weight files then hold the table behind everything else. */
+int scn_net_set_symbols(scn_net_t *net, int n_symbols, float scale, const float *h_table);
+/* The table as it is now and its gradient of the last training batch (either may be NULL). */
+int scn_net_get_symbols(scn_net_t *net, float *h_table, float *h_gradient);
+/* scn_net_forward_host and scn_net_train_batch with h_symbols[rows], each below n_symbols, in place of the features. */
+int scn_net_forward_host_symbols(scn_net_t *net, int batch, const int *h_keys, const int *h_off, const int *h_symbols, float *h_probs,
+                                 int *h_predictions);
+int scn_net_train_batch_symbols(scn_net_t *net, int batch, const int *h_keys, const int *h_off, const int *h_symbols, const int *h_labels,
+                                float learningRate, float momentum, float *h_probs, double *stats);
+
 /* The output features learnt layer `layer` keeps in the training batches that follow, instead of a random draw: n
  * ascending indices below its nFeaturesOut (n = 0: back to random draws).  For repeating a run with known subsets. */
 int scn_net_set_dropout_features(scn_net_t *net, int layer, const int *present, int n);

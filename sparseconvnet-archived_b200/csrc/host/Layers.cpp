@@ -419,7 +419,7 @@ int TerminalPoolingLayer::calculateInputSpatialSize(int outputSpatialSize) {
 NetworkInNetworkLayer::NetworkInNetworkLayer(cudaMemStream &memStream, cublasHandle_t &, int nFeaturesIn, int nFeaturesOut, float dropout,
                                              ActivationFunction fn, float alpha)
     : SpatiallySparseLayer(memStream), W(false, nFeaturesIn * nFeaturesOut), MW(false, 0), B(false, nFeaturesOut), MB(false, 0), fn(fn),
-      nFeaturesIn(nFeaturesIn), nFeaturesOut(nFeaturesOut), dropout(dropout), precision(SCN_PREC_AUTO), fusePoolNext(false), precisionFallback(false), packedT(nullptr), packedTBytes(0), packed(nullptr),
+      nFeaturesIn(nFeaturesIn), nFeaturesOut(nFeaturesOut), dropout(dropout), precision(SCN_PREC_AUTO), fusePoolNext(false), precisionFallback(false), deferUpdate(false), packedT(nullptr), packedTBytes(0), packed(nullptr),
       packedBytes(0), packedPrecision(-100), packedFs(0) {
   // uniform(+-sqrt(6/(nIn + nOut*alpha))) as NetworkInNetworkLayer.cu:135-137, from a fixed
   // seed (the reference seeds from the clock); real runs load weights.
@@ -962,6 +962,7 @@ void NetworkInNetworkLayer::backwards(SpatiallySparseBatch &batch, SpatiallySpar
     }
   }
   multiplyAddCount += (__int128_t)rows * K * N;
+  if (deferUpdate) return;
   if ((int)MW.size() != K * N) { zeroed(MW, K * N, memStream); zeroed(MB, N, memStream); }
   if (inMask || outMask) {
     scnSafeCall(scn_sgd_update_masked(W.dPtr(), MW.dPtr(), dw.dPtr(), K, N, inMask, inPeriod, outMask, learningRate, momentum, 0, s));
@@ -972,6 +973,14 @@ void NetworkInNetworkLayer::backwards(SpatiallySparseBatch &batch, SpatiallySpar
   }
   updateSlopes(learningRate, momentum, outMask);
   weightsChanged();
+}
+void NetworkInNetworkLayer::learntParameters(std::vector<LearntParameter> &list) {
+  list.push_back({&W, &dw, true, -INFINITY});
+  list.push_back({&B, &db, false, -INFINITY});
+}
+void NetworkInNetworkPReLULayer::learntParameters(std::vector<LearntParameter> &list) {
+  NetworkInNetworkLayer::learntParameters(list);
+  list.push_back({&PReLU, &dprelu, false, 0.001f}); // (held there by the SGD update too)
 }
 float *NetworkInNetworkPReLULayer::slopeGradient() {
   dprelu.copyToGPU();

@@ -44,6 +44,8 @@ public:
                          long long rowsInBound, int *d_result);
   void finishRules(SpatiallySparseBatch &batch, SpatiallySparseBatchInterface &input, SpatiallySparseBatchInterface &output,
                    const int *h_result);
+  bool deferUpdate; // backwards() leaves dw, db (and the slopes' gradient) to an optimiser over all layers
+  void learntParameters(std::vector<LearntParameter> &list) override;
   // Call after writing W directly (e.g. W.hVector()[i] = ...): drops the packed copy the
   // tensor-core kernel reads.
   void weightsChanged();

@@ -359,6 +359,40 @@ std::vector<float> SparseConvNetCUDA::layerTimes() {
   return ms;
 }
 
+void SparseConvNetCUDA::useAdamW(float beta1, float beta2, float eps, float weightDecay, float maxNorm, int stateBits) {
+  std::unique_ptr<AdamW> next(new AdamW(beta1, beta2, eps, weightDecay, maxNorm, stateBits));
+  useSGD(); // (the old one's moments may still be in use)
+  adamW = std::move(next);
+}
+void SparseConvNetCUDA::useSGD() {
+  cudaSafeCall(cudaStreamSynchronize(memStream.stream));
+  adamW.reset();
+}
+void SparseConvNetCUDA::useSymbols(int nSymbols, float scale, const float *values) {
+  std::unique_ptr<SymbolTable> next(new SymbolTable(memStream, nSymbols, nInputFeatures, scale, values));
+  cudaSafeCall(cudaStreamSynchronize(memStream.stream));
+  if (adamW && symbolTable) throw ScnException("useSymbols: set the table before useAdamW"); // (its moments belong to the old table)
+  symbolTable = std::move(next);
+}
+// Every layer's backwards in reverse order, then, where they leave it, the update.
+void SparseConvNetCUDA::learn(SpatiallySparseBatch &batch, float learningRate, float momentum) {
+  for (auto l : layers)
+    if (auto n = dynamic_cast<NetworkInNetworkLayer *>(l)) n->deferUpdate = adamW != nullptr;
+  for (int i = (int)layers.size() - 1; i >= 0; --i) layers[i]->backwards(batch, batch.interfaces[i], batch.interfaces[i + 1], learningRate, momentum);
+  SpatiallySparseBatchInterface &in = batch.interfaces[0];
+  const bool symbols = symbolTable && in.symbols.size() > 0;
+  if (symbols) symbolTable->backwards(in);
+  if (adamW) {
+    std::vector<LearntParameter> list;
+    for (auto l : layers) l->learntParameters(list);
+    if (symbols) list.push_back({&symbolTable->table, &symbolTable->dtable, true, -INFINITY});
+    adamW->update(list, learningRate, batch.batchSize, memStream);
+    for (auto l : layers)
+      if (auto n = dynamic_cast<NetworkInNetworkLayer *>(l)) n->weightsChanged();
+  } else if (symbols)
+    symbolTable->update(learningRate, momentum);
+}
+
 // SparseConvNetCUDA.cu:227-271: every layer's forwards (on a RESCALEBATCH each followed by its scaleWeights),
 // SoftmaxClassifier and, for a TRAINBATCH, every layer's backwards in reverse order (each learnt layer updates its
 // weights on the way).
@@ -376,7 +410,7 @@ void SparseConvNetCUDA::processBatch(SpatiallySparseBatch &batch, float learning
     forwardLayers(batch);
   SoftmaxClassifier(batch.interfaces.back(), batch, nTop, memStream);
   if (batch.type == TRAINBATCH)
-    for (int i = (int)layers.size() - 1; i >= 0; --i) layers[i]->backwards(batch, batch.interfaces[i], batch.interfaces[i + 1], learningRate, momentum);
+    learn(batch, learningRate, momentum);
   if (f)
     for (auto &p : batch.predictions) {
       for (size_t k = 0; k < p.size(); ++k) f << (k ? " " : "") << p[k];
@@ -415,7 +449,7 @@ void SparseConvNetCUDA::processIndexLearnerBatch(SpatiallySparseBatch &batch, fl
     batch.interfaces[n].sub->reset();
     top->forwards(batch, under, batch.interfaces[n]);
     IndexLearner(batch.interfaces[n], batch, nTop, memStream);
-    for (int i = n - 1; i >= 0; --i) layers[i]->backwards(batch, batch.interfaces[i], batch.interfaces[i + 1], learningRate, momentum);
+    learn(batch, learningRate, momentum);
   }
 }
 
@@ -575,6 +609,11 @@ void SparseConvNetCUDA::loadWeights(std::string baseName, int epoch, bool moment
   std::cout << "Loading network parameters from " << filename << std::endl;
   for (int i = 0; i < std::min((int)layers.size(), firstNlayers); ++i) layers[i]->loadWeightsFromStream(f, momentum);
   if (!inputNormalizingConstants.empty()) f.read((char *)inputNormalizingConstants.data(), sizeof(float) * inputNormalizingConstants.size());
+  if (symbolTable && firstNlayers >= (int)layers.size()) {
+    std::vector<float> &h = symbolTable->table.hVector();
+    f.read((char *)h.data(), sizeof(float) * h.size());
+    if (!f) throw ScnException("weight file ends early");
+  }
 }
 void SparseConvNetCUDA::saveWeights(std::string baseName, int epoch, bool momentum) {
   std::string filename = baseName + "_epoch-" + std::to_string(epoch) + ".cnn";
@@ -582,4 +621,11 @@ void SparseConvNetCUDA::saveWeights(std::string baseName, int epoch, bool moment
   if (!f) throw ScnException("Cannot write " + filename);
   for (auto l : layers) l->putWeightsToStream(f, momentum);
   if (!inputNormalizingConstants.empty()) f.write((char *)inputNormalizingConstants.data(), sizeof(float) * inputNormalizingConstants.size());
+  if (symbolTable) {
+    cudaSafeCall(cudaStreamSynchronize(memStream.stream));
+    vectorCUDA<float> &t = symbolTable->table;
+    const bool on = t.onGPU;
+    f.write((char *)t.hVector().data(), sizeof(float) * t.hVector().size());
+    if (on) t.copyToGPU();
+  }
 }

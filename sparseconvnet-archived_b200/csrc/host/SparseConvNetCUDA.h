@@ -3,12 +3,14 @@
 #pragma once
 #include <fstream>
 #include <iostream>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
 #include "SpatiallySparseBatch.h"
 #include "SpatiallySparseDataset.h"
 #include "SpatiallySparseLayer.h"
+#include "SymbolTable.h"
 #define N_MAX_BATCH_PRODUCER_THREADS 20
 
 class SparseConvNetCUDA {
@@ -70,6 +72,16 @@ public:
   void saveWeights(std::string baseName, int epoch, bool momentum);
 
   // ---- additions (no reference counterpart)
+  // Training batches update all learnt tensors by one AdamW step instead of each by momentum SGD (the batch's `momentum` is
+  // then not used).  A batch with dropout gives its dropped features' weights gradients of zero; the index learner goes on
+  // updating itself.  The moments start at zero here and are not part of the weight files.
+  void useAdamW(float beta1 = 0.9f, float beta2 = 0.999f, float eps = 1e-8f, float weightDecay = 0.01f, float maxNorm = 0.0f, int stateBits = 32);
+  void useSGD();
+  std::unique_ptr<AdamW> adamW;
+  // Inputs may carry a symbol per row (interfaces[0].symbols) instead of features: symbolTable->forwards(interfaces[0]) puts the
+  // features there, and a training batch updates the table too.  Weight files carry the table behind everything else.
+  void useSymbols(int nSymbols, float scale, const float *values);
+  std::unique_ptr<SymbolTable> symbolTable;
   // Run every layer's rule construction on the device for a batch whose interface 0 holds
   // the input grids in device form, with a single read-back of all per-layer counts.
   void preprocessBatchOnDevice(SpatiallySparseBatch &batch);
@@ -87,6 +99,7 @@ public:
 
 private:
   void init(int nInputFeatures, int nClasses);
+  void learn(SpatiallySparseBatch &batch, float learningRate, float momentum);
   vectorCUDA<int> chainResults; // two sets of 4 ints per layer, used by alternate batches
   bool timing;
   int chainRowsHint; // rows per sample seen so far (+25 %): sizes the fused rule chain's shared memory

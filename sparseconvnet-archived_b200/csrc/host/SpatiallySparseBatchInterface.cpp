@@ -18,7 +18,8 @@ SpatiallySparseBatchInterface::SpatiallySparseBatchInterface(SpatiallySparseBatc
       spatialSize(o.spatialSize), backpropErrors(o.backpropErrors), grids(std::move(o.grids)), rules(std::move(o.rules)),
       siteKeys(std::move(o.siteKeys)), sampleOffsets(std::move(o.sampleOffsets)), backgroundRows(std::move(o.backgroundRows)),
       maxSitesPerSample(o.maxSitesPerSample), gridOwner(this), deferredFrom(nullptr), deferredCells(0), deferredLearnt(nullptr), deferredLearntInput(nullptr),
-      presentSubset(std::move(o.presentSubset)), presentMask(std::move(o.presentMask)), learntOutput(o.learntOutput) {}
+      presentSubset(std::move(o.presentSubset)), presentMask(std::move(o.presentMask)), learntOutput(o.learntOutput),
+      symbols(std::move(o.symbols)) {}
 void SpatiallySparseBatchInterface::summary() {
   std::cout << "nFeatures " << nFeatures << " featuresPresent " << featuresPresent.size() << " spatialSize " << spatialSize
             << " nSpatialSites " << nSpatialSites << " features " << sub->features.size() << " grids " << grids.size() << std::endl;
@@ -34,6 +35,7 @@ void SpatiallySparseBatchInterface::reset() {
   presentSubset.clear();
   presentMask.resize(0);
   learntOutput = false;
+  symbols.resize(0);
   maxSitesPerSample = 0;
   gridOwner = this;
   deferredFrom = nullptr;

@@ -52,6 +52,8 @@ public:
   std::vector<int> presentSubset;
   vectorCUDA<float> presentMask;
   bool learntOutput;
+  // The input's codes, one per row, where they stand for its features (SymbolTable; empty otherwise).
+  vectorCUDA<int> symbols;
 
   explicit SpatiallySparseBatchInterface(SpatiallySparseBatchSubInterface *s);
   SpatiallySparseBatchInterface(SpatiallySparseBatchInterface &&o) noexcept; // pointers into a moved-from interface are dropped

@@ -11,3 +11,4 @@ void SpatiallySparseLayer::putWeightsToStream(std::ofstream &, bool) {}
 long long SpatiallySparseLayer::enqueueRules(SpatiallySparseBatch &, SpatiallySparseBatchInterface &, SpatiallySparseBatchInterface &,
                                              long long rowsInBound, int *) { return rowsInBound; }
 void SpatiallySparseLayer::finishRules(SpatiallySparseBatch &, SpatiallySparseBatchInterface &, SpatiallySparseBatchInterface &, const int *) {}
+void SpatiallySparseLayer::learntParameters(std::vector<LearntParameter> &) {}

@@ -6,6 +6,7 @@
 #include <fstream>
 #include <iostream>
 #include "SpatiallySparseBatch.h"
+#include "AdamW.h"
 #include "SpatiallySparseBatchInterface.h"
 
 class SpatiallySparseLayer {
@@ -36,4 +37,7 @@ public:
   virtual void finishRules(SpatiallySparseBatch &batch, SpatiallySparseBatchInterface &input,
                            SpatiallySparseBatchInterface &output, const int *h_result);
   bool changesGeometry;
+  // The tensors that backwards() finds gradients for, for an optimiser over all layers (none: nothing to learn, or the layer
+  // updates itself, as the index learner does).
+  virtual void learntParameters(std::vector<LearntParameter> &list);
 };

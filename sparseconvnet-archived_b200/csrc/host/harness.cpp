@@ -117,10 +117,17 @@ void adoptDeviceInput(SparseConvNetCUDA &cnn, SpatiallySparseBatch &b, int batch
   in.sub->features.borrowDevice(const_cast<float *>(d_features), rows * cnn.nInputFeatures);
 }
 // Interface 0 of the network's first pool slot filled from host arrays (pinned ones are copied from where they lie,
-// pageable ones through the stream's staging block); the features travel on a stream of their own.
-SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, const int *off, const float *features, batchType type) {
+// pageable ones through the stream's staging block); the features travel on a stream of their own.  symbols: one code a row
+// instead of features; the network's table turns them into features behind their copy.
+SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, const int *off, const float *features, batchType type,
+                                      const int *symbols = nullptr) {
   SparseConvNetCUDA &cnn = *net->cnn;
   if (batch < 1) throw ScnException("batch must be positive");
+  if (symbols) {
+    if (!cnn.symbolTable) throw ScnException("no symbol table (scn_net_set_symbols)");
+    for (int r = 0; r < off[batch]; ++r)
+      if (symbols[r] >= cnn.symbolTable->nSymbols) throw ScnException("row " + std::to_string(r) + " has a symbol that the table does not hold");
+  }
   SpatiallySparseBatch &b = cnn.batchPool[0];
   cnn.prepareBatch(b);
   b.reset();
@@ -135,7 +142,8 @@ SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, 
   in.nSpatialSites = rows;
   in.gridOwner = &in;
   in.backpropErrors = false;
-  const size_t kb = sizeof(int) * rows, ob = sizeof(int) * (batch + 1), fb = sizeof(float) * (size_t)rows * nF;
+  const size_t kb = sizeof(int) * rows, ob = sizeof(int) * (batch + 1), fb = symbols ? sizeof(int) * (size_t)rows : sizeof(float) * (size_t)rows * nF;
+  const void *values = symbols ? (const void *)symbols : (const void *)features;
   auto pinned = [&](const void *p) {
     for (const void *k : net->knownPinned) if (k == p) return true;
     cudaPointerAttributes a;
@@ -145,12 +153,12 @@ SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, 
     net->knownPinned.push_back(p);
     return true;
   };
-  const void *sk = keys, *so = off, *sf = features;
-  if (!(pinned(keys) && pinned(off) && pinned(features))) {
+  const void *sk = keys, *so = off, *sf = values;
+  if (!(pinned(keys) && pinned(off) && pinned(values))) {
     char *stage = (char *)cnn.memStream.staging(kb + ob + fb);
     std::memcpy(stage, keys, kb);
     std::memcpy(stage + kb, off, ob);
-    std::memcpy(stage + kb + ob, features, fb);
+    std::memcpy(stage + kb + ob, values, fb);
     sk = stage; so = stage + kb; sf = stage + kb + ob;
   }
   int maxRows = 0;
@@ -166,6 +174,15 @@ SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, 
   cudaStream_t s = cnn.memStream.stream;
   if (rows) cudaSafeCall(cudaMemcpyAsync(in.siteKeys.dPtr(), sk, kb, cudaMemcpyHostToDevice, s));
   cudaSafeCall(cudaMemcpyAsync(in.sampleOffsets.dPtr(), so, ob, cudaMemcpyHostToDevice, s));
+  cnn.inputBackgroundPending = true; // found by the rule chain's kernel (or by a kernel of its own where that one does not apply)
+  if (symbols) {
+    in.symbols.copyToGPU();
+    in.symbols.resize(rows);
+    if (rows) cudaSafeCall(cudaMemcpyAsync(in.symbols.dPtr(), sf, fb, cudaMemcpyHostToDevice, s));
+    in.backpropErrors = type == TRAINBATCH; // the table learns
+    cnn.symbolTable->forwards(in);
+    return b;
+  }
   if (!net->copyStream) {
     cudaSafeCall(cudaStreamCreateWithFlags(&net->copyStream, cudaStreamNonBlocking));
     cudaSafeCall(cudaEventCreateWithFlags(&net->copyDone, cudaEventDisableTiming));
@@ -177,7 +194,6 @@ SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, 
     cudaSafeCall(cudaMemcpyAsync(dst, sf, fb, cudaMemcpyHostToDevice, net->copyStream));
     cudaSafeCall(cudaEventRecord(net->copyDone, net->copyStream));
   }
-  cnn.inputBackgroundPending = true; // found by the rule chain's kernel (or by a kernel of its own where that one does not apply)
   if (rows) cnn.inputReady = net->copyDone; // the layers (not the rule chain) wait for the features
   return b;
 }
@@ -496,21 +512,66 @@ int scn_net_exchange_step_device(scn_net_t *net, const float *d_probs, int rows,
   });
 }
 
+namespace {
+void trainHostBatch(scn_net *net, int batch, const int *keys, const int *off, const float *features, const int *symbols, const int *labels,
+                    float learningRate, float momentum, float *probs, double *stats) {
+  SparseConvNetCUDA &cnn = *net->cnn;
+  if (!labels) throw ScnException("a training step needs labels");
+  SpatiallySparseBatch &b = uploadHostInput(net, batch, keys, off, features, TRAINBATCH, symbols);
+  b.labels.copyToCPU();
+  b.labels.hVector().assign(labels, labels + batch);
+  cnn.preprocessBatchOnDevice(b);
+  std::ofstream nof, nog;
+  cnn.processBatch(b, learningRate, momentum, nof, nog);
+  net->last = &b;
+  cudaSafeCall(cudaStreamSynchronize(cnn.memStream.stream));
+  for (int i = 0; i < batch && probs; ++i) std::memcpy(probs + (size_t)i * cnn.nClasses, b.probabilities[i].data(), sizeof(float) * cnn.nClasses);
+  if (stats) { stats[0] = b.negativeLogLikelihood; stats[1] = b.mistakes; }
+}
+} // namespace
 int scn_net_train_batch(scn_net_t *net, int batch, const int *keys, const int *off, const float *features, const int *labels, float learningRate,
                         float momentum, float *probs, double *stats) {
+  return guarded([&] { trainHostBatch(net, batch, keys, off, features, nullptr, labels, learningRate, momentum, probs, stats); });
+}
+
+int scn_net_set_symbols(scn_net_t *net, int nSymbols, float scale, const float *table) {
+  return guarded([&] { net->cnn->useSymbols(nSymbols, scale, table); });
+}
+int scn_net_get_symbols(scn_net_t *net, float *table, float *gradient) {
   return guarded([&] {
     SparseConvNetCUDA &cnn = *net->cnn;
-    if (!labels) throw ScnException("a training step needs labels");
-    SpatiallySparseBatch &b = uploadHostInput(net, batch, keys, off, features, TRAINBATCH);
-    b.labels.copyToCPU();
-    b.labels.hVector().assign(labels, labels + batch);
-    cnn.preprocessBatchOnDevice(b);
-    std::ofstream nof, nog;
-    cnn.processBatch(b, learningRate, momentum, nof, nog);
-    net->last = &b;
+    if (!cnn.symbolTable) throw ScnException("no symbol table (scn_net_set_symbols)");
     cudaSafeCall(cudaStreamSynchronize(cnn.memStream.stream));
-    for (int i = 0; i < batch && probs; ++i) std::memcpy(probs + (size_t)i * cnn.nClasses, b.probabilities[i].data(), sizeof(float) * cnn.nClasses);
-    if (stats) { stats[0] = b.negativeLogLikelihood; stats[1] = b.mistakes; }
+    vectorCUDA<float> &t = cnn.symbolTable->table, &g = cnn.symbolTable->dtable;
+    const size_t bytes = sizeof(float) * (size_t)cnn.symbolTable->nSymbols * cnn.nInputFeatures;
+    if (table) {
+      if (t.onGPU) cudaSafeCall(cudaMemcpy(table, t.dPtr(), bytes, cudaMemcpyDeviceToHost));
+      else std::memcpy(table, t.hVector().data(), bytes);
+    }
+    if (gradient) {
+      if (g.size() == 0) throw ScnException("no training batch of symbols has run");
+      cudaSafeCall(cudaMemcpy(gradient, g.dPtr(), bytes, cudaMemcpyDeviceToHost));
+    }
+  });
+}
+int scn_net_forward_host_symbols(scn_net_t *net, int batch, const int *keys, const int *off, const int *symbols, float *probs, int *predictions) {
+  return guarded([&] {
+    if (!symbols) throw ScnException("symbols are needed");
+    SpatiallySparseBatch &b = uploadHostInput(net, batch, keys, off, nullptr, UNLABELEDBATCH, symbols);
+    runHostBatch(net, b, batch, probs, predictions, false, nullptr, nullptr);
+  });
+}
+int scn_net_train_batch_symbols(scn_net_t *net, int batch, const int *keys, const int *off, const int *symbols, const int *labels, float learningRate,
+                                float momentum, float *probs, double *stats) {
+  return guarded([&] {
+    if (!symbols) throw ScnException("symbols are needed");
+    trainHostBatch(net, batch, keys, off, nullptr, symbols, labels, learningRate, momentum, probs, stats);
+  });
+}
+int scn_net_use_adamw(scn_net_t *net, float beta1, float beta2, float eps, float weightDecay, float maxNorm, int stateBits) {
+  return guarded([&] {
+    if (stateBits == 0) net->cnn->useSGD();
+    else net->cnn->useAdamW(beta1, beta2, eps, weightDecay, maxNorm, stateBits);
   });
 }
 

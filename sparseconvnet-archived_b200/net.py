@@ -21,7 +21,8 @@ EXPORTS = [
     "scn_net_layer_times", "scn_net_process_dataset", "scn_host_vectorTopIndices",
     "scn_net_exchange_create", "scn_net_exchange_buffer", "scn_net_exchange_connect", "scn_net_exchange_connect_local", "scn_net_exchange_destroy",
     "scn_net_forward_host_exchange", "scn_net_exchange_flush", "scn_net_exchange_step_device",
-    "scn_net_forward_host_begin", "scn_net_forward_host_end", "scn_net_rescale_batch", "scn_net_addIndexLearnerLayer", "scn_net_index_learner_batch", "scn_net_set_dropout_features", "scn_net_iface_present",
+    "scn_net_forward_host_begin", "scn_net_forward_host_end", "scn_net_rescale_batch", "scn_net_addIndexLearnerLayer", "scn_net_index_learner_batch", "scn_net_use_adamw", "scn_net_set_symbols", "scn_net_get_symbols", "scn_net_forward_host_symbols",
+    "scn_net_train_batch_symbols", "scn_net_set_dropout_features", "scn_net_iface_present",
 ]
 
 LAYER_KEYS = ("type", "size", "stride", "minActive", "nIn", "nOut", "fs", "act", "inSpatial", "outSpatial")
@@ -93,6 +94,11 @@ def lib():
         L.scn_net_index_learner_batch.argtypes = [c_p, c_int, c_p, c_p, c_p, c_p, c_f, c_f, c_p, c_p]
         L.scn_net_iface_present.argtypes = [c_p, c_int, c_p]
         L.scn_net_forward_host_end.argtypes = [c_p, c_p, c_p, c_p, c_p]
+        L.scn_net_use_adamw.argtypes = [c_p] + [c_f] * 5 + [c_int]
+        L.scn_net_set_symbols.argtypes = [c_p, c_int, c_f, c_p]
+        L.scn_net_get_symbols.argtypes = [c_p, c_p, c_p]
+        L.scn_net_forward_host_symbols.argtypes = [c_p, c_int] + [c_p] * 5
+        L.scn_net_train_batch_symbols.argtypes = [c_p, c_int] + [c_p] * 4 + [c_f, c_f, c_p, c_p]
         _lib = L
     return _lib
 
@@ -320,6 +326,50 @@ class Net:
         probs = np.empty((B, self.nClasses), np.float32)
         stats = np.zeros(2, np.float64)
         _check(self.L.scn_net_train_batch(self.h, B, _np(keys), _np(off), _np(features), _np(labels), learning_rate, momentum, _np(probs), _np(stats)))
+        return probs, dict(nll=float(stats[0]), mistakes=int(stats[1]))
+
+    def use_adamw(self, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, max_norm=0.0, state_bits=32):
+        """Train by one AdamW step over all learnt tensors a batch (gradients averaged over the batch; the training calls' momentum
+        is not used).  state_bits: 32, or 8, or 0 to return to momentum SGD."""
+        _check(self.L.scn_net_use_adamw(self.h, beta1, beta2, eps, weight_decay, max_norm, state_bits))
+
+    def set_symbols(self, table, scale=1.0):
+        """Take inputs as one code a row: table [n_symbols, nInputFeatures]."""
+        table = np.ascontiguousarray(table, np.float32)
+        if table.ndim != 2 or table.shape[1] != self.nIn:
+            raise abi.ScnError("the table must be [symbols, %d]" % self.nIn)
+        _check(self.L.scn_net_set_symbols(self.h, table.shape[0], scale, _np(table)))
+        self._symbols = table.shape
+
+    def get_symbols(self, gradient=False):
+        """The symbol table as it is now; with `gradient` also its gradient of the last training batch."""
+        if not hasattr(self, "_symbols"):
+            raise abi.ScnError("no symbol table (set_symbols)")
+        t, g = np.empty(self._symbols, np.float32), np.empty(self._symbols, np.float32)
+        _check(self.L.scn_net_get_symbols(self.h, _np(t), _np(g) if gradient else None))
+        return (t, g) if gradient else t
+
+    def forward_host_symbols(self, keys, off, symbols):
+        """forward_host with one symbol a row (negative: no features) instead of features."""
+        keys = np.ascontiguousarray(keys, np.int32)
+        off = np.ascontiguousarray(off, np.int32)
+        symbols = np.ascontiguousarray(symbols, np.int32)
+        B = len(off) - 1
+        probs = np.empty((B, self.nClasses), np.float32)
+        pred = np.empty((B, self.nTop), np.int32)
+        _check(self.L.scn_net_forward_host_symbols(self.h, B, _np(keys), _np(off), _np(symbols), _np(probs), _np(pred)))
+        return probs, pred
+
+    def train_batch_symbols(self, keys, off, symbols, labels, learning_rate, momentum=0.0):
+        """train_batch with one symbol a row instead of features; the table learns too."""
+        keys = np.ascontiguousarray(keys, np.int32)
+        off = np.ascontiguousarray(off, np.int32)
+        symbols = np.ascontiguousarray(symbols, np.int32)
+        labels = np.ascontiguousarray(labels, np.int32)
+        B = len(off) - 1
+        probs = np.empty((B, self.nClasses), np.float32)
+        stats = np.zeros(2, np.float64)
+        _check(self.L.scn_net_train_batch_symbols(self.h, B, _np(keys), _np(off), _np(symbols), _np(labels), learning_rate, momentum, _np(probs), _np(stats)))
         return probs, dict(nll=float(stats[0]), mistakes=int(stats[1]))
 
     def addIndexLearnerLayer(self):
