@@ -94,17 +94,19 @@ template <int CAP> __global__ void __launch_bounds__(THREADS) k_grad_norm_partia
     partial[blockIdx.x] = sum;
   }
 }
-__global__ void __launch_bounds__(THREADS) k_grad_norm_finish(const double *partial, int n, float *norm) {
+constexpr int FINISH = 1024;
+__global__ void __launch_bounds__(FINISH) k_grad_norm_finish(const double *partial, int n, float *norm) {
   wait_for_prior_grids();
   double sum = 0;
-  for (int i = threadIdx.x; i < n; i += THREADS) sum += partial[i];
-  __shared__ double warpSum[WARPS];
+  for (int i = threadIdx.x; i < n; i += FINISH) sum += partial[i];
+  __shared__ double warpSum[FINISH / 32];
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
   if ((threadIdx.x & 31) == 0) warpSum[threadIdx.x >> 5] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < WARPS; ++w) sum += warpSum[w];
-    *norm = (float)sqrt(sum);
+  if (threadIdx.x < 32) {
+    sum = warpSum[threadIdx.x];
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (threadIdx.x == 0) *norm = (float)sqrt(sum);
   }
 }
 
@@ -261,28 +263,63 @@ template <int K> __device__ __forceinline__ float2 decode_v(unsigned word, float
 // The largest |m| and v of the lanes are compared as whole numbers: the bits of floats that are not negative are in the floats' order,
 // and what is not finite lies above all of them.
 constexpr unsigned NOT_FINITE = 0x7F800000u;
+// A block's share of everything, on its way to a warp while it works on the block before: the step issues instructions for
+// most of the time that its memory needs, so a warp cannot do without either.
+struct Incoming {
+  float w[BLOCK];
+  float g[BLOCK]; // (of the gradient's type)
+  unsigned char m[BLOCK], v[BLOCK];
+};
+template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void ask(const Tensor &t, long long block, int lane, Incoming &in) {
+  const long long i = block * BLOCK;
+  const int bytes = t.gtype == SCN_F32 ? 4 : 2;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) copy_async<16>(in.w + (k * 32 + lane) * 4, t.w + i + (k * 32 + lane) * 4);
+  copy_async<16>((char *)in.g + lane * 16, (const char *)t.g + i * bytes + lane * 16);
+  if (bytes == 4) copy_async<16>((char *)in.g + 512 + lane * 16, (const char *)t.g + i * 4 + 512 + lane * 16);
+  if (lane < 16) copy_async<16>(in.m + lane * 16, (const unsigned char *)t.m + i + lane * 16);
+  else copy_async<16>(in.v + (lane - 16) * 16, (const unsigned char *)t.v + i + (lane - 16) * 16);
+}
 template <int CAP>
-__global__ void __launch_bounds__(THREADS, 5) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
+__global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
+  __shared__ __align__(16) Incoming incoming[2][WARPS];
   const Tensor &t = l.t[owner(l, blockIdx.x)];
-  const int lane = threadIdx.x & 31;
-  long long block = (long long)((int)blockIdx.x - t.chunk) * l.turns * WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long block = (long long)((int)blockIdx.x - t.chunk) * l.turns * WARPS + warp;
   signed char *mq = (signed char *)t.m;
   unsigned char *vq = (unsigned char *)t.v;
   wait_for_prior_grids();
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
+  const auto whole = [&](long long b) { return t.wide && (b + 1) * BLOCK <= t.n; };
+  if (whole(block)) ask(t, block, lane, incoming[0][warp]);
+  asm volatile("cp.async.commit_group;" ::: "memory");
   for (int turn = 0; turn < l.turns && block * BLOCK < t.n; ++turn, block += WARPS) {
     const long long i = block * BLOCK + lane * 8;
-    const bool wide = t.wide && (block + 1) * BLOCK <= t.n;
+    const bool wide = whole(block);
     float w[8], g[8];
     unsigned mw[2], vw[2];
     const float sm = t.ms[block], sv = t.vs[block];
+    __syncwarp(); // (every lane has read what this turn's copies overwrite)
+    if (turn + 1 < l.turns && whole(block + WARPS)) ask(t, block + WARPS, lane, incoming[(turn + 1) & 1][warp]);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (wide) {
-      load8_typed(t.g, t.gtype, i, g);
-      const uint2 a = *(const uint2 *)(mq + i), b = *(const uint2 *)(vq + i);
-      load8(t.w + i, w);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+      const Incoming &in = incoming[turn & 1][warp];
+      const uint2 a = ((const uint2 *)in.m)[lane], b = ((const uint2 *)in.v)[lane];
       mw[0] = a.x; mw[1] = a.y; vw[0] = b.x; vw[1] = b.y;
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) *(float4 *)(w + k) = *(const float4 *)(in.w + lane * 8 + k);
+      if (t.gtype == SCN_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) *(float4 *)(g + k) = *(const float4 *)(in.g + lane * 8 + k);
+      } else if (t.gtype == SCN_BF16) load8_16((const __nv_bfloat16 *)in.g + lane * 8, g);
+      else load8_16((const __half *)in.g + lane * 8, g);
     } else {
       mw[0] = mw[1] = vw[0] = vw[1] = 0;
 #pragma unroll
@@ -416,7 +453,7 @@ const char *wrong_list(const scn_adamw_tensor_t *t, int count, bool step) {
 }
 bool wide(const scn_adamw_tensor_t &t) {
   const uintptr_t states = (uintptr_t)t.d_m | (uintptr_t)t.d_v;
-  return !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 7 : 31));
+  return !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 15 : 31));
 }
 // launch(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.  Where one turn a
 // chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes `most`: it finds its tensor once for all of them.
@@ -450,7 +487,6 @@ template <class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, i
   if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, most, take, launch);
   return for_lists<CAP_LARGE>(t, count, most, take, launch);
 }
-int norm_ctas() { return 4 * sm_count(); }
 
 } // namespace
 } // namespace scn
@@ -493,7 +529,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
   const int most = (int)(scn_grad_norm_workspace_bytes() / sizeof(double));
   int used = 0, launches = (count + CAP_LARGE - 1) / CAP_LARGE;
   if (launches > most) return fail(SCN_ERR_UNSUPPORTED, "AdamW: list too long");
-  const int each = std::min(norm_ctas(), most / std::max(launches, 1));
+  const int each = most / std::max(launches, 1); // a CTA a chunk as far as there are places for their sums
   const int rc = for_lists(tensors, count, 4, [](const scn_adamw_tensor_t &) { return true; }, [&](const auto &l) -> int {
     const int grid = std::min(l.chunks, each);
     SCN_CUDA_TRY(launch_dependent(k_grad_norm_partial<std::decay_t<decltype(l)>::capacity>, dim3(grid), dim3(THREADS), 0, s, l, partial + used));
@@ -502,7 +538,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
     return SCN_OK;
   });
   if (rc != SCN_OK) return rc;
-  SCN_CUDA_TRY(launch_dependent(k_grad_norm_finish, dim3(1), dim3(THREADS), 0, s, partial, used, d_norm));
+  SCN_CUDA_TRY(launch_dependent(k_grad_norm_finish, dim3(1), dim3(FINISH), 0, s, partial, used, d_norm));
   SCN_LAUNCH_CHECK("k_grad_norm_finish");
   return SCN_OK;
 }
@@ -525,7 +561,7 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
     return SCN_OK;
   });
   if (rc != SCN_OK) return rc;
-  return for_lists(tensors, count, 4, eight, [&](const auto &l) -> int {
+  return for_lists(tensors, count, 8, eight, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_8<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
     SCN_LAUNCH_CHECK("k_adamw_8");
     return SCN_OK;

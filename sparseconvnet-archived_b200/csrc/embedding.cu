@@ -10,43 +10,57 @@ constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_LANES = 64;
 // out[i][c] = scale * table[tokens[i]][c]; a zero row for a token outside [0, vocab).  Groups of `lanes` threads take a row, W
 // columns a thread at a time, LOOKUP_ROWS rows at once so that as many table rows are on their way; the output, which is
 // not read again here, is stored past the caches' reach of the table.
-template <class T, class O, int W, int ROWS>
-__global__ void __launch_bounds__(THREADS) k_embedding_forward(const T *__restrict__ table, int vocab, int C, const int *__restrict__ tokens, long long n, float scale,
-                                                               O *__restrict__ out, long long stride, int lanes, int groups, int *errors) {
+struct Lookup {
+  const char *table;
+  const int *tokens;
+  char *out;
+  long long n, stride;    // stride: bytes from row to row of the output
+  unsigned rowBytes;      // of the table
+  int vocab, C;
+  float scale;
+  int *errors;
+};
+// The token, or -1 where it names no row.
+__device__ __forceinline__ int row_of(const Lookup &p, long long i, bool tell) {
+  int t = i < p.n ? __ldg(p.tokens + i) : -1;
+  if (t >= p.vocab) {
+    if (tell && p.errors) atomicOr(p.errors, SCN_DEV_ERR_KEY);
+    t = -1;
+  }
+  return t;
+}
+template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(THREADS) k_embedding_forward(const Lookup p, int lanes, int groups) {
   constexpr int V = W * sizeof(O) > 16 ? 16 / (int)sizeof(O) : W; // values a store
-  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = C / W;
+  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = p.C / W;
   if (group >= groups) return;
-  const long long step = (long long)gridDim.x * groups * ROWS;
+  wait_for_prior_grids();
+  dependents_may_launch();
+  const long long step = (long long)gridDim.x * groups * ROWS, between = groups * p.stride;
   long long i = (long long)blockIdx.x * groups * ROWS + group;
   int next[ROWS];
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) next[u] = i + u * groups < n ? __ldg(tokens + i + u * groups) : -1;
-  for (; i < n; i += step) {
+  for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + u * groups, lane == 0);
+  for (; i < p.n; i += step) {
     int t[ROWS];
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      t[u] = next[u];
-      if (t[u] >= vocab) {
-        if (lane == 0 && errors) atomicOr(errors, SCN_DEV_ERR_KEY);
-        t[u] = -1;
-      }
-      next[u] = i + step + u * groups < n ? __ldg(tokens + i + step + u * groups) : -1; // the next turn's, while this one's rows travel
-    }
+    for (int u = 0; u < ROWS; ++u) t[u] = next[u];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + step + u * groups, lane == 0); // the next turn's, while this one's rows travel
     for (int v = lane; v < vectors; v += lanes) {
+      const char *column = p.table + v * (W * (int)sizeof(T));
       Pack<T, W> from[ROWS];
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-        if (t[u] >= 0) from[u] = load_pack<T, W>(table + (long long)t[u] * C + v * W);
+      for (int u = 0; u < ROWS; ++u) from[u] = load_pack<T, W>((const T *)(column + (unsigned long long)(unsigned)max(t[u], 0) * p.rowBytes));
+      char *to = p.out + i * p.stride + v * (W * (int)sizeof(O));
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        if (i + u * groups >= n) break;
-        O *to = out + (i + u * groups) * stride + v * W;
+      for (int u = 0; u < ROWS; ++u, to += between) {
+        if (i + u * groups >= p.n) break;
 #pragma unroll
         for (int w = 0; w < W; w += V) {
           Pack<O, V> o;
 #pragma unroll
-          for (int k = 0; k < V; ++k) o.v[k] = from_float<O>(t[u] >= 0 ? to_float(from[u].v[w + k]) * scale : 0.f);
-          __stcs((typename Raw<V * (int)sizeof(O)>::type *)(to + w), o.raw);
+          for (int k = 0; k < V; ++k) o.v[k] = from_float<O>(t[u] >= 0 ? to_float(from[u].v[w + k]) * p.scale : 0.f);
+          __stcs((typename Raw<V * (int)sizeof(O)>::type *)((O *)to + w), o.raw);
         }
       }
     }
@@ -54,37 +68,32 @@ __global__ void __launch_bounds__(THREADS) k_embedding_forward(const T *__restri
 }
 // The same value by value, for widths, strides and addresses that allow no more: a warp takes ROWS rows and 32 * COLS columns at
 // once, so that about as many bytes are on their way.
-template <class T, class O, int ROWS, int COLS>
-__global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const T *__restrict__ table, int vocab, int C, const int *__restrict__ tokens, long long n,
-                                                                      float scale, O *__restrict__ out, long long stride, int *errors) {
+template <class T, class O, int ROWS, int COLS> __global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const Lookup p) {
   const int lane = threadIdx.x & 31;
-  const long long step = (long long)gridDim.x * WARPS * ROWS;
-  for (long long i = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS; i < n; i += step) {
-    int mine = lane < ROWS && i + lane < n ? __ldg(tokens + i + lane) : -1;
-    if (mine >= vocab) {
-      if (errors) atomicOr(errors, SCN_DEV_ERR_KEY);
-      mine = -1;
-    }
-    const T *from[ROWS];
+  const long long i = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS;
+  const int rows = (int)min((long long)ROWS, p.n - i);
+  if (rows <= 0) return;
+  wait_for_prior_grids();
+  dependents_may_launch();
+  const int mine = row_of(p, lane < rows ? i + lane : p.n, true);
+  for (int c = lane; c - lane < p.C; c += 32 * COLS) {
+    const char *column = p.table + c * sizeof(T);
+    T v[ROWS][COLS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
-      const int t = __shfl_sync(~0u, mine, u);
-      from[u] = t >= 0 ? table + (long long)t * C : nullptr;
+      const T *row = (const T *)(column + (unsigned long long)(unsigned)max(__shfl_sync(~0u, mine, u), 0) * p.rowBytes);
+#pragma unroll
+      for (int j = 0; j < COLS; ++j)
+        if (c + 32 * j < p.C) v[u][j] = __ldg(row + 32 * j);
     }
-    for (int c = lane; c - lane < C; c += 32 * COLS) {
-      T v[ROWS][COLS];
+    O *to = (O *)(p.out + i * p.stride) + c;
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int j = 0; j < COLS; ++j)
-          if (from[u] && c + 32 * j < C) v[u][j] = __ldg(from[u] + c + 32 * j);
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        if (i + u >= n) break;
-        O *to = out + (i + u) * stride + c;
+    for (int u = 0; u < ROWS; ++u, to = (O *)((char *)to + p.stride)) {
+      const bool row = __shfl_sync(~0u, mine, u) >= 0;
+      if (u < rows) {
 #pragma unroll
         for (int j = 0; j < COLS; ++j)
-          if (c + 32 * j < C) __stcs(to + 32 * j, from_float<O>(from[u] ? to_float(v[u][j]) * scale : 0.f));
+          if (c + 32 * j < p.C) __stcs(to + 32 * j, from_float<O>(row ? to_float(v[u][j]) * p.scale : 0.f));
       }
     }
   }
@@ -94,32 +103,29 @@ int lanes_for(int vectors) {
   const int turns = (vectors + MAX_LANES - 1) / MAX_LANES;
   return (vectors + turns - 1) / turns;
 }
-template <class T, class O> void launch_forward(const T *table, int vocab, int C, const int *tokens, long long n, float scale, O *out, long long stride,
-                                                int *errors, cudaStream_t s) {
+template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStream_t s) {
   // the widest access that addresses, width and stride allow: at most 16 bytes of the table
   constexpr int MOST = 16 / (int)sizeof(T);
   int W = MOST;
-  while (W > 1 && !(C % W == 0 && stride % W == 0 && (uintptr_t)table % (W * sizeof(T)) == 0 && (uintptr_t)out % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
-  if (W == 1 && C > 16) {
-    const auto single = [&](auto kernel, int rows) {
-      kernel<<<(int)std::min((n + WARPS * rows - 1) / (WARPS * rows), 16ll * sm_count()), THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, errors);
-    };
-    if (C <= 32) single(k_embedding_forward_single<T, O, 16, 1>, 16);
-    else if (C <= 64) single(k_embedding_forward_single<T, O, 8, 2>, 8);
-    else if (C <= 96) single(k_embedding_forward_single<T, O, 5, 3>, 5);
-    else single(k_embedding_forward_single<T, O, 4, 4>, 4);
-    return;
+  while (W > 1 && !(p.C % W == 0 && (uintptr_t)p.table % (W * sizeof(T)) == 0 && ((uintptr_t)p.out | (uintptr_t)p.stride) % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
+  if (W == 1 && p.C > 16) {
+    const auto single = [&](auto kernel, int rows) { return launch_dependent(kernel, dim3((unsigned)((p.n + WARPS * rows - 1) / (WARPS * rows))), dim3(THREADS), 0, s, p); };
+    if (p.C <= 32) return single(k_embedding_forward_single<T, O, 16, 1>, 16);
+    if (p.C <= 64) return single(k_embedding_forward_single<T, O, 8, 2>, 8);
+    if (p.C <= 96) return single(k_embedding_forward_single<T, O, 5, 3>, 5);
+    return single(k_embedding_forward_single<T, O, 4, 4>, 4);
   }
-  const int lanes = lanes_for(C / W), groups = THREADS / lanes;
+  const int lanes = lanes_for(p.C / W), groups = THREADS / lanes;
   const auto launch = [&](auto kernel, int rows) {
-    const int grid = (int)std::min((n + groups * rows - 1) / (groups * rows), 16ll * sm_count());
-    kernel<<<grid, THREADS, 0, s>>>(table, vocab, C, tokens, n, scale, out, stride, lanes, groups, errors);
+    const int grid = (int)std::min((p.n + groups * rows - 1) / (groups * rows), 64ll * sm_count());
+    return launch_dependent(kernel, dim3(grid), dim3(THREADS), 0, s, p, lanes, groups);
   };
-  // narrow accesses: more rows at once, for as many bytes on their way
-  if (W == MOST) launch(k_embedding_forward<T, O, MOST, 4>, 4);
-  else if (W == 1) launch(k_embedding_forward<T, O, 1, 8>, 8);
-  else if (W == MOST / 2) launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
-  else launch(k_embedding_forward<T, O, 2, 8>, 8);
+  // narrow accesses: more rows at once, for as many bytes on their way (four rows of 16 bytes at once took longer: 197 us for
+  // 3.4 M rows of 64 floats, against 164 us with two)
+  if (W == MOST) return launch(k_embedding_forward<T, O, MOST, 2>, 2);
+  if (W == 1) return launch(k_embedding_forward<T, O, 1, 8>, 8);
+  if (W == MOST / 2) return launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
+  return launch(k_embedding_forward<T, O, 2, 8>, 8);
 }
 
 // ------------------------------------------------------------------ stable radix sort of (token, row)
@@ -257,16 +263,13 @@ __device__ __forceinline__ void places_by_digit(const unsigned (&key)[ROUNDS], i
     unsigned peers = __ballot_sync(~0u, in);
 #pragma unroll
     for (int b = 0; b < BITS; ++b) {
-      const bool set = d >> b & 1;
-      const unsigned votes = __ballot_sync(~0u, set);
-      peers &= set ? votes : ~votes;
+      const unsigned votes = __ballot_sync(~0u, d >> b & 1), other = (d >> b & 1) - 1u;
+      peers &= votes ^ other;
     }
-    if (in) {
-      const unsigned n = own[d];
-      place[r] = n + __popc(peers & ((1u << lane) - 1));
-      __syncwarp(peers);
-      if (peers >> lane == 1u) own[d] = (unsigned short)(n + __popc(peers)); // the last of the lanes with this digit
-    }
+    const unsigned n = in ? own[d] : 0u;
+    place[r] = n + __popc(peers & ((1u << lane) - 1));
+    __syncwarp(); // (of the whole warp: lanes that waited for those with their digit alone would go on one digit after the other)
+    if (in && peers >> lane == 1u) own[d] = (unsigned short)(n + __popc(peers)); // the last of the lanes with this digit
     __syncwarp();
   }
   __syncthreads();
@@ -759,23 +762,24 @@ template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
 } // namespace scn
 
 using namespace scn;
+static constexpr int MOST_COLUMNS = 1 << 28; // (a row's bytes fit 32 bits)
 
 extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vocab, int C, const int *d_tokens, long long n, float scale, void *d_out,
                                      int out_type, long long out_stride, int *d_errors, scn_stream_t stream) {
   clear_error();
-  if (vocab < 1 || C < 1 || n < 0 || n > 0x7fffffffll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
+  if (vocab < 1 || C < 1 || C > MOST_COLUMNS || n < 0 || n > 0x7fffffffll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (out_stride < C) return fail(SCN_ERR_INVALID, "embedding: the output's row stride is below the number of features");
   if (!type_known(table_type) || !type_known(out_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (n == 0) return SCN_OK;
   if (!d_table || !d_tokens || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
-  SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, launch_forward((const T *)d_table, vocab, C, d_tokens, n, scale, (O *)d_out, out_stride,
-                                                                                 d_errors, (cudaStream_t)stream)));
+  const Lookup p = {(const char *)d_table, d_tokens, (char *)d_out, n, out_stride * type_bytes(out_type), (unsigned)C * type_bytes(table_type), vocab, C, scale, d_errors};
+  SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, SCN_CUDA_TRY((launch_forward<T, O>(p, (cudaStream_t)stream)))));
   SCN_LAUNCH_CHECK("k_embedding_forward");
   return SCN_OK;
 }
 
 extern "C" size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C) {
-  if (n < 0 || n > 0x7fff0000ll || vocab < 1 || C < 1) return 0;
+  if (n < 0 || n > 0x7fff0000ll || vocab < 1 || C < 1 || C > MOST_COLUMNS) return 0;
   return plan_sort(n, vocab, C).total;
 }
 
@@ -783,7 +787,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
                                       float scale, int accumulate, float *d_dtable, int *d_errors, void *d_workspace, size_t workspace_bytes,
                                       scn_stream_t stream) {
   clear_error();
-  if (vocab < 1 || C < 1 || n < 0 || n > 0x7fff0000ll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
+  if (vocab < 1 || C < 1 || C > MOST_COLUMNS || n < 0 || n > 0x7fff0000ll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (dout_stride < C) return fail(SCN_ERR_INVALID, "embedding: the gradient's row stride is below the number of features");
   if (!type_known(dout_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (dout_stride > 0xffffffffll / type_bytes(dout_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the gradient's rows lie 4 GiB apart or more");
@@ -851,7 +855,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
       SCN_CUDA_TRY(launch_dependent(k_embedding_join32, dim3((tiles / 32 + WARPS - 1) / WARPS), dim3(THREADS), 0, s, q, tiles));
       SCN_LAUNCH_CHECK("k_embedding_join32");
     }
-    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(std::min((tiles + JOIN_WARPS - 1) / JOIN_WARPS, 4 * sm_count())), dim3(JOIN_THREADS), 0, s, q, tiles, joined));
+    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(std::min((tiles + JOIN_WARPS - 1) / JOIN_WARPS, 8 * sm_count())), dim3(JOIN_THREADS), 0, s, q, tiles, joined));
     SCN_LAUNCH_CHECK("k_embedding_join");
   }
   return SCN_OK;
