@@ -527,7 +527,8 @@ int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float *d_norm, v
 
 /* The step.  `tensors` and `h` are host arrays, read before the call returns.  d_scalars: NULL, or a device copy of the
  * scalars to use instead of h's (h may then be NULL).  d_norm: NULL, or the norm of all gradients on the device
- * (scn_grad_norm's): needed for max_norm, and a norm that is not finite makes the step change nothing at all. */
+ * (scn_grad_norm's): needed for max_norm (scalars on the device that ask for it without one are not clipped), and a norm that
+ * is not finite makes the step change nothing at all. */
 int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, const scn_adamw_t *h, const scn_adamw_scalars_t *d_scalars,
                    const float *d_norm, scn_stream_t stream);
 

@@ -112,8 +112,8 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
     const auto single = [&](auto kernel, int rows) { return launch_dependent(kernel, dim3((unsigned)((p.n + WARPS * rows - 1) / (WARPS * rows))), dim3(THREADS), 0, s, p); };
     if (p.C <= 32) return single(k_embedding_forward_single<T, O, 16, 1>, 16);
     if (p.C <= 64) return single(k_embedding_forward_single<T, O, 8, 2>, 8);
-    if (p.C <= 96) return single(k_embedding_forward_single<T, O, 5, 3>, 5);
-    return single(k_embedding_forward_single<T, O, 4, 4>, 4);
+    if (p.C <= 96) return single(k_embedding_forward_single<T, O, 3, 3>, 3);
+    return single(k_embedding_forward_single<T, O, 2, 4>, 2);
   }
   const int lanes = lanes_for(p.C / W), groups = THREADS / lanes;
   const auto launch = [&](auto kernel, int rows) {
@@ -768,6 +768,7 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
                                      int out_type, long long out_stride, int *d_errors, scn_stream_t stream) {
   clear_error();
   if (vocab < 1 || C < 1 || C > MOST_COLUMNS || n < 0 || n > 0x7fffffffll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
+  if (out_stride > (1ll << 48)) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (out_stride < C) return fail(SCN_ERR_INVALID, "embedding: the output's row stride is below the number of features");
   if (!type_known(table_type) || !type_known(out_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
   if (n == 0) return SCN_OK;

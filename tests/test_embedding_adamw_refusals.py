@@ -24,7 +24,7 @@ INVALID, WORKSPACE = 1, 3
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(vocab=0), "sizes"), (dict(C=0), "sizes"), (dict(n=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(stride=3), "row stride"),
+    (dict(vocab=0), "sizes"), (dict(C=0), "sizes"), (dict(n=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(stride=3), "row stride"), (dict(stride=1 << 50), "sizes"), (dict(C=1 << 29, stride=1 << 29), "sizes"),
     (dict(table_type=3), "type"), (dict(out_type=-1), "type"), (dict(table=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
 ])
 def test_lookup_refusals(a, change, text):

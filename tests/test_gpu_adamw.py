@@ -450,3 +450,25 @@ def test_refusals_of_the_binding(abi):
         abi.adamw_decode(torch.zeros(300, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda"))
     with pytest.raises(abi.ScnError):
         abi.adamw_decode(torch.zeros(300, dtype=torch.int16, device="cuda"), torch.zeros(2, device="cuda"))
+
+
+def test_more_than_32_bits_of_values(abi):
+    """A tensor of more than 2^32 values with 8-bit states: offsets and the dither's places past 32 bits, at both ends."""
+    n = (1 << 32) + 1000
+    t = dict(w=torch.zeros(n, device="cuda"), g=torch.zeros(n, device="cuda", dtype=torch.bfloat16), weight_decay=0.0, w_min=-math.inf, **abi.adamw_states(n, "cuda", 8))
+    ends = [slice(0, 3 * BLOCK), slice((1 << 32) - 2 * BLOCK, (1 << 32) + 2 * BLOCK), slice(n - 1000 + 2 * BLOCK, n)]
+    for e in ends:
+        t["g"][e] = torch.randn(e.stop - e.start, device="cuda").to(torch.bfloat16)
+    opt = abi.AdamW([t])
+    norm = opt.grad_norm().item()
+    want = math.sqrt(sum((t["g"][e].double() ** 2).sum().item() for e in ends))
+    assert abs(norm - want) <= 1.001 * U * want
+    opt.step(1e-3, 1, seed=7)
+    for e in ends:
+        at = np.arange(e.start, e.stop, dtype=np.uint64)
+        m, v = np_moments(np.zeros(len(at), f32), np.zeros(len(at), f32), t["g"][e].float().cpu().numpy())
+        um, uv = np_mix(at, 7)
+        for k, x, u in (("m", m, um), ("v", v, uv)):
+            codes, scale = np_encode(x, u, k == "v")
+            assert np.array_equal(t[k][e].cpu().numpy(), codes) and np.array_equal(t[k + "_scale"][e.start // BLOCK:-(-e.stop // BLOCK)].cpu().numpy(), scale)
+    assert t["w"][4096].item() == 0 and t["m"][1 << 31].item() == 0
