@@ -22,25 +22,31 @@ struct Tensor {
   long long n;
   unsigned long long block; // blocks of BLOCK values in front of this tensor in the call's whole list
   float decay, least;
-  int chunk;           // this tensor's first chunk in the launch
   short gtype, w16type;
   int wide;            // every array is aligned for eight values at once
 };
 template <int CAP> struct List {
   static constexpr int capacity = CAP;
   int count, chunks;
-  int turns; // of a chunk: its CTA takes turns * TURN values
+  int turns;      // of a chunk: its CTA takes turns * TURN values
+  int first[CAP]; // each tensor's first chunk in the launch (apart from the tensors: the search touches few lines)
   Tensor t[CAP];
 };
 constexpr int CAP_SMALL = 16, CAP_MEDIUM = 64, CAP_LARGE = SCN_ADAMW_MAX_TENSORS;
 static_assert(sizeof(List<CAP_LARGE>) <= 32000, "a launch takes at most 32764 bytes of parameters");
 
-// The tensor that owns a chunk (tensors without values own none).
+// The tensor that owns a chunk (tensors without values own none): for a short list without a chain of dependent reads.
 template <int CAP> __device__ __forceinline__ int owner(const List<CAP> &l, int chunk) {
+  if (CAP <= CAP_SMALL) {
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < CAP; ++i) at += i < l.count && l.first[i] <= chunk;
+    return at;
+  }
   int lo = 0, hi = l.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (l.t[mid].chunk <= chunk) lo = mid; else hi = mid - 1;
+    if (l.first[mid] <= chunk) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -68,8 +74,9 @@ template <int CAP> __global__ void __launch_bounds__(THREADS) k_grad_norm_partia
   wait_for_prior_grids();
   double sum = 0;
   for (int chunk = blockIdx.x; chunk < l.chunks; chunk += gridDim.x) {
-    const Tensor &t = l.t[owner(l, chunk)];
-    long long first = (long long)(chunk - t.chunk) * l.turns * TURN;
+    const int at = owner(l, chunk);
+    const Tensor &t = l.t[at];
+    long long first = (long long)(chunk - l.first[at]) * l.turns * TURN;
     for (int turn = 0; turn < l.turns && first < t.n; ++turn, first += TURN) {
       if (t.wide && first + TURN <= t.n) {
         float g[8];
@@ -157,8 +164,9 @@ __device__ __forceinline__ float2 updated(const scn_adamw_scalars_t &h, float2 w
 // A CTA takes one chunk, a thread eight values a turn: everything it reads is on its way before the first is used.
 template <int CAP>
 __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
-  const Tensor &t = l.t[owner(l, blockIdx.x)];
-  long long first = (long long)((int)blockIdx.x - t.chunk) * l.turns * TURN;
+  const int at = owner(l, blockIdx.x);
+  const Tensor &t = l.t[at];
+  long long first = (long long)((int)blockIdx.x - l.first[at]) * l.turns * TURN;
   float *ms = (float *)t.m, *vs = (float *)t.v;
   wait_for_prior_grids();
   if (dh) h = *dh;
@@ -286,9 +294,10 @@ __device__ __forceinline__ void ask(const Tensor &t, long long block, int lane, 
 template <int CAP>
 __global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   __shared__ __align__(16) Incoming incoming[2][WARPS];
-  const Tensor &t = l.t[owner(l, blockIdx.x)];
+  const int own = owner(l, blockIdx.x);
+  const Tensor &t = l.t[own];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long block = (long long)((int)blockIdx.x - t.chunk) * l.turns * WARPS + warp;
+  long long block = (long long)((int)blockIdx.x - l.first[own]) * l.turns * WARPS + warp;
   signed char *mq = (signed char *)t.m;
   unsigned char *vq = (unsigned char *)t.v;
   wait_for_prior_grids();
@@ -473,8 +482,9 @@ template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tenso
         if (rc != SCN_OK) return rc;
         l.count = l.chunks = 0;
       }
+      l.first[l.count] = l.chunks;
       l.t[l.count++] = Tensor{t[i].d_w, t[i].d_g, t[i].d_m, t[i].d_v, t[i].d_m_scale, t[i].d_v_scale, t[i].d_w16, t[i].n, block,
-                              t[i].weight_decay, t[i].w_min, l.chunks, (short)t[i].g_type, (short)t[i].w16_type, wide(t[i])};
+                              t[i].weight_decay, t[i].w_min, (short)t[i].g_type, (short)t[i].w16_type, wide(t[i])};
       l.chunks += (int)chunks;
     }
     block += blocks;
