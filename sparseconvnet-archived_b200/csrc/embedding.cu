@@ -14,53 +14,55 @@ struct Lookup {
   const char *table;
   const int *tokens;
   char *out;
-  long long n, stride;    // stride: bytes from row to row of the output
+  unsigned n, stride;     // stride: bytes from row to row of the output
   unsigned rowBytes;      // of the table
   int vocab, C;
   float scale;
   int *errors;
 };
 // The token, or -1 where it names no row.
-__device__ __forceinline__ int row_of(const Lookup &p, long long i, bool tell) {
+__device__ __forceinline__ int row_of(const Lookup &p, unsigned i) {
   int t = i < p.n ? __ldg(p.tokens + i) : -1;
   if (t >= p.vocab) {
-    if (tell && p.errors) atomicOr(p.errors, SCN_DEV_ERR_KEY);
+    if (p.errors) atomicOr(p.errors, SCN_DEV_ERR_KEY);
     t = -1;
   }
   return t;
 }
-template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(THREADS) k_embedding_forward(const Lookup p, int lanes, int groups) {
+template <class P> __device__ __forceinline__ P *at_row(P *base, unsigned row, unsigned bytes) { return base + (unsigned long long)row * bytes; }
+template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(THREADS) k_embedding_forward(const Lookup p, unsigned lanes, unsigned groups) {
   constexpr int V = W * sizeof(O) > 16 ? 16 / (int)sizeof(O) : W; // values a store
-  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = p.C / W;
+  const unsigned group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes, vectors = p.C / W;
   if (group >= groups) return;
   wait_for_prior_grids();
   dependents_may_launch();
-  const long long step = (long long)gridDim.x * groups * ROWS, between = groups * p.stride;
-  long long i = (long long)blockIdx.x * groups * ROWS + group;
+  const unsigned step = gridDim.x * groups * ROWS;
+  unsigned i = blockIdx.x * groups * ROWS + group;
   int next[ROWS];
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + u * groups, lane == 0);
+  for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + u * groups);
   for (; i < p.n; i += step) {
     int t[ROWS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) t[u] = next[u];
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + step + u * groups, lane == 0); // the next turn's, while this one's rows travel
-    for (int v = lane; v < vectors; v += lanes) {
-      const char *column = p.table + v * (W * (int)sizeof(T));
+    for (int u = 0; u < ROWS; ++u) next[u] = row_of(p, i + step + u * groups); // the next turn's, while this one's rows travel
+    for (unsigned v = lane; v < vectors; v += lanes) {
+      const char *column = p.table + v * (W * (unsigned)sizeof(T));
       Pack<T, W> from[ROWS];
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u) from[u] = load_pack<T, W>((const T *)(column + (unsigned long long)(unsigned)max(t[u], 0) * p.rowBytes));
-      char *to = p.out + i * p.stride + v * (W * (int)sizeof(O));
+      for (int u = 0; u < ROWS; ++u) from[u] = load_pack<T, W>((const T *)at_row(column, max(t[u], 0), p.rowBytes));
+      char *to = p.out + v * (W * (unsigned)sizeof(O));
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u, to += between) {
-        if (i + u * groups >= p.n) break;
+      for (int u = 0; u < ROWS; ++u) {
+        if (u > 0 && i + u * groups >= p.n) break;
+        O *row = (O *)at_row(to, i + u * groups, p.stride);
 #pragma unroll
         for (int w = 0; w < W; w += V) {
           Pack<O, V> o;
 #pragma unroll
           for (int k = 0; k < V; ++k) o.v[k] = from_float<O>(t[u] >= 0 ? to_float(from[u].v[w + k]) * p.scale : 0.f);
-          __stcs((typename Raw<V * (int)sizeof(O)>::type *)((O *)to + w), o.raw);
+          __stcs((typename Raw<V * (int)sizeof(O)>::type *)(row + w), o.raw);
         }
       }
     }
@@ -70,31 +72,30 @@ template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(T
 // once, so that about as many bytes are on their way.
 template <class T, class O, int ROWS, int COLS> __global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const Lookup p) {
   const int lane = threadIdx.x & 31;
-  const long long i = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS;
-  const int rows = (int)min((long long)ROWS, p.n - i);
-  if (rows <= 0) return;
+  const unsigned i = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS;
+  if (i >= p.n) return;
   wait_for_prior_grids();
   dependents_may_launch();
-  const int mine = row_of(p, lane < rows ? i + lane : p.n, true);
+  const int mine = row_of(p, lane < ROWS ? i + lane : p.n);
   for (int c = lane; c - lane < p.C; c += 32 * COLS) {
-    const char *column = p.table + c * sizeof(T);
+    const char *column = p.table + c * (int)sizeof(T);
     T v[ROWS][COLS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
-      const T *row = (const T *)(column + (unsigned long long)(unsigned)max(__shfl_sync(~0u, mine, u), 0) * p.rowBytes);
+      const T *row = (const T *)at_row(column, max(__shfl_sync(~0u, mine, u), 0), p.rowBytes);
 #pragma unroll
       for (int j = 0; j < COLS; ++j)
         if (c + 32 * j < p.C) v[u][j] = __ldg(row + 32 * j);
     }
-    O *to = (O *)(p.out + i * p.stride) + c;
+    char *to = p.out + c * (int)sizeof(O);
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u, to = (O *)((char *)to + p.stride)) {
-      const bool row = __shfl_sync(~0u, mine, u) >= 0;
-      if (u < rows) {
+    for (int u = 0; u < ROWS; ++u) {
+      const bool named = __shfl_sync(~0u, mine, u) >= 0;
+      if (u > 0 && i + u >= p.n) break;
+      O *row = (O *)at_row(to, i + u, p.stride);
 #pragma unroll
-        for (int j = 0; j < COLS; ++j)
-          if (c + 32 * j < p.C) __stcs(to + 32 * j, from_float<O>(row ? to_float(v[u][j]) * p.scale : 0.f));
-      }
+      for (int j = 0; j < COLS; ++j)
+        if (c + 32 * j < p.C) __stcs(row + 32 * j, from_float<O>(named ? to_float(v[u][j]) * p.scale : 0.f));
     }
   }
 }
@@ -109,15 +110,15 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
   int W = MOST;
   while (W > 1 && !(p.C % W == 0 && (uintptr_t)p.table % (W * sizeof(T)) == 0 && ((uintptr_t)p.out | (uintptr_t)p.stride) % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
   if (W == 1 && p.C > 16) {
-    const auto single = [&](auto kernel, int rows) { return launch_dependent(kernel, dim3((unsigned)((p.n + WARPS * rows - 1) / (WARPS * rows))), dim3(THREADS), 0, s, p); };
+    const auto single = [&](auto kernel, unsigned rows) { return launch_dependent(kernel, dim3((p.n + WARPS * rows - 1) / (WARPS * rows)), dim3(THREADS), 0, s, p); };
     if (p.C <= 32) return single(k_embedding_forward_single<T, O, 16, 1>, 16);
     if (p.C <= 64) return single(k_embedding_forward_single<T, O, 8, 2>, 8);
     if (p.C <= 96) return single(k_embedding_forward_single<T, O, 3, 3>, 3);
     return single(k_embedding_forward_single<T, O, 2, 4>, 2);
   }
-  const int lanes = lanes_for(p.C / W), groups = THREADS / lanes;
-  const auto launch = [&](auto kernel, int rows) {
-    const int grid = (int)std::min((p.n + groups * rows - 1) / (groups * rows), 64ll * sm_count());
+  const unsigned lanes = lanes_for(p.C / W), groups = THREADS / lanes;
+  const auto launch = [&](auto kernel, unsigned rows) {
+    const unsigned grid = std::min((p.n + groups * rows - 1) / (groups * rows), 64u * sm_count());
     return launch_dependent(kernel, dim3(grid), dim3(THREADS), 0, s, p, lanes, groups);
   };
   // narrow accesses: more rows at once, for as many bytes on their way (four rows of 16 bytes at once took longer: 197 us for
@@ -768,12 +769,12 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
                                      int out_type, long long out_stride, int *d_errors, scn_stream_t stream) {
   clear_error();
   if (vocab < 1 || C < 1 || C > MOST_COLUMNS || n < 0 || n > 0x7fffffffll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
-  if (out_stride > (1ll << 48)) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (out_stride < C) return fail(SCN_ERR_INVALID, "embedding: the output's row stride is below the number of features");
   if (!type_known(table_type) || !type_known(out_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
+  if (out_stride > 0xffffffffll / type_bytes(out_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the output's rows lie 4 GiB apart or more");
   if (n == 0) return SCN_OK;
   if (!d_table || !d_tokens || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
-  const Lookup p = {(const char *)d_table, d_tokens, (char *)d_out, n, out_stride * type_bytes(out_type), (unsigned)C * type_bytes(table_type), vocab, C, scale, d_errors};
+  const Lookup p = {(const char *)d_table, d_tokens, (char *)d_out, (unsigned)n, (unsigned)(out_stride * type_bytes(out_type)), (unsigned)C * type_bytes(table_type), vocab, C, scale, d_errors};
   SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, SCN_CUDA_TRY((launch_forward<T, O>(p, (cudaStream_t)stream)))));
   SCN_LAUNCH_CHECK("k_embedding_forward");
   return SCN_OK;

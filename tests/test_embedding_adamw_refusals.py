@@ -20,11 +20,16 @@ def refused(a, status, code, text):
     assert text in a.lib().scn_last_error().decode()
 
 
-INVALID, WORKSPACE = 1, 3
+INVALID, WORKSPACE, UNSUPPORTED = 1, 3, 4
+
+
+def test_rows_too_far_apart(a):
+    refused(a, a.lib().scn_embedding_forward(P, 0, 5, 4, P, 7, 1.0, P, 0, 1 << 30, None, None), UNSUPPORTED, "4 GiB")
+    refused(a, a.lib().scn_embedding_backward(P, 7, P, 1, 1 << 31, 5, 4, 1.0, 0, P, None, P, 1 << 40, None), UNSUPPORTED, "4 GiB")
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(vocab=0), "sizes"), (dict(C=0), "sizes"), (dict(n=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(stride=3), "row stride"), (dict(stride=1 << 50), "sizes"), (dict(C=1 << 29, stride=1 << 29), "sizes"),
+    (dict(vocab=0), "sizes"), (dict(C=0), "sizes"), (dict(n=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(stride=3), "row stride"), (dict(C=1 << 29, stride=1 << 29), "sizes"),
     (dict(table_type=3), "type"), (dict(out_type=-1), "type"), (dict(table=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
 ])
 def test_lookup_refusals(a, change, text):
