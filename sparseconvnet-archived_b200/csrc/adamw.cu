@@ -129,8 +129,11 @@ __device__ __forceinline__ float gradient_scale(const scn_adamw_scalars_t &h, co
 // Two values in one instruction each, as far as there is one: the 8-bit step is bound by the instructions it issues.
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ float2 sub(float2 a, float2 b) { return __ffma2_rn(b, both(-1.f), a); }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); } // of nothing that mul() gave
+// A sum that a product goes into, where both roundings count: one value at a time.  (A paired product and the paired sum behind it come
+// out as one fused operation, also where PTX names the rounding of each; the tests that count codes show it.)
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 minus(float2 a, float2 b) { return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y)); }
 __device__ __forceinline__ float root(float x) { // an ulp or so off; 0 below 2^-126
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -150,8 +153,8 @@ __device__ __forceinline__ float max_nan(float a, float b) { // a NaN stays one
 // against these values, come out the same in any program that computes the formula in 32 bits.
 __device__ __forceinline__ void moments(const scn_adamw_scalars_t &h, float gs, float2 g, float2 &m, float2 &v) {
   g = mul(g, both(gs));
-  m = add(mul(m, both(h.beta1)), mul(g, both(h.one_minus_beta1)));
-  v = add(mul(v, both(h.beta2)), mul(mul(g, g), both(h.one_minus_beta2)));
+  m = plus(mul(m, both(h.beta1)), mul(g, both(h.one_minus_beta1)));
+  v = plus(mul(v, both(h.beta2)), mul(mul(g, g), both(h.one_minus_beta2)));
 }
 // The parameter's step may use the hardware's approximate root and reciprocal (an ulp or two of 32 bits): unlike the states it
 // is compared with nothing.
@@ -225,16 +228,16 @@ __device__ __forceinline__ float2 nearest(float2 r) { return add(add(r, both(838
 // (x - q^2 and 2 q + 1 are exact.)
 __device__ __forceinline__ float2 code_m(float2 x, float2 u) {
   float2 q = nearest(make_float2(root(x.x), root(x.y)));
-  q = sub(q, positive(__ffma2_rn(q, q, make_float2(-x.x, -x.y))));
-  const float2 over = sub(x, mul(q, q)), limit = mul(u, __ffma2_rn(q, both(2.f), both(1.f)));
-  return add(q, positive(sub(over, limit)));
+  q = minus(q, positive(__ffma2_rn(q, q, make_float2(-x.x, -x.y))));
+  const float2 over = __ffma2_rn(q, make_float2(-q.x, -q.y), x), limit = mul(u, __ffma2_rn(q, both(2.f), both(1.f)));
+  return plus(q, positive(minus(over, limit)));
 }
 __device__ __forceinline__ float2 fourth(float2 q) { q = mul(q, q); return mul(q, q); }
 __device__ __forceinline__ float2 code_v(float2 y, float2 u) {
   float2 q = nearest(make_float2(root(root(y.x)), root(root(y.y))));
-  q = sub(q, positive(sub(fourth(q), y)));
-  const float2 low = fourth(q), limit = mul(u, sub(fourth(add(q, both(1.f))), low));
-  return add(q, positive(sub(sub(y, low), limit)));
+  q = minus(q, positive(minus(fourth(q), y)));
+  const float2 low = fourth(q), limit = mul(u, minus(fourth(add(q, both(1.f))), low));
+  return plus(q, positive(minus(minus(y, low), limit)));
 }
 // A 32-bit mix of a position and the seed: multiplications by odd numbers (the fractional bits of the square roots of 2, 3,
 // 5 and 7) between shifts that bring the high bits down.  Its two halves, the lower one with the upper one mixed in once more,
