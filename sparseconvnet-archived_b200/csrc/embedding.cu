@@ -1,4 +1,7 @@
-// Embedding table in front of the first layer: rows by token, and the table's gradient by sorted tokens.
+// Embedding table in front of the first layer: rows by token, out[i] = scale * table[tokens[i]], and the table's gradient,
+// dtable[t] = scale * sum of dout[i] over tokens[i] == t, by sorted tokens.  Both are bound by memory: the lookup by its
+// output (and the table rows, which mostly come out of the caches), the gradient by one read of dout and one write of the
+// table, next to which the sort moves 8 bytes a row four times.
 #include <algorithm>
 #include "scn_types.cuh"
 
@@ -8,8 +11,11 @@ namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_LANES = 64;
 
 // out[i][c] = scale * table[tokens[i]][c]; a zero row for a token outside [0, vocab).  Groups of `lanes` threads take a row, W
-// columns a thread at a time, LOOKUP_ROWS rows at once so that as many table rows are on their way; the output, which is
-// not read again here, is stored past the caches' reach of the table.
+// columns a thread at a time, ROWS rows at once so that as many table rows are on their way, with the tokens of the next turn
+// already asked for; the output, which is not read again here, is stored so that it leaves the caches to the table.
+// 3.4 M rows of 64 floats from a table of 65536: 160 us, 5.6 TB/s of the 889 MB it cannot do without (85 % of a plain copy's rate).
+// Rows that end or begin inside a 32-byte sector next to bytes that nobody writes cost the memory a read of the sector each:
+// the same rows 16 bytes apart take 350 us, 32 bytes apart 162 us.
 struct Lookup {
   const char *table;
   const int *tokens;
@@ -69,7 +75,8 @@ template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(T
   }
 }
 // The same value by value, for widths, strides and addresses that allow no more: a warp takes ROWS rows and 32 * COLS columns at
-// once, so that about as many bytes are on their way.
+// once, so that about as many bytes are on their way.  224 k rows of 96 from a 16-bit table into rows of 99 floats: 26 us (a
+// plain fill of as many bytes takes 14.5 us); groups of 48 threads with two turns a row took 39 us.
 template <class T, class O, int ROWS, int COLS> __global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const Lookup p) {
   const int lane = threadIdx.x & 31;
   const unsigned i = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS;
@@ -132,6 +139,10 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
 // ------------------------------------------------------------------ stable radix sort of (token, row)
 // Digits of at most MAX_DIGIT bits, least significant first; per pass: digit counts of each tile, their running sums
 // over the tiles, and the scatter.  A tile is THREADS * ROUNDS consecutive entries, a warp of it 32 * ROUNDS consecutive ones.
+// 3.4 M rows, 18-bit keys: 83 us for both passes (counts 11 + 5, running sums 9 + 8, scatters 24 + 21, overlapped launches
+// included; the table's 33 MB of zeros are written beside the first counts).  It is bound by the latency of its short kernels
+// and the scatter by the instructions that rank entries within a warp; wider digits (10 bits) and larger tiles (15 rounds: 219 us for the
+// whole gradient, 8 rounds: 199, 4 rounds: 212) did not help.
 constexpr int MAX_DIGIT = 9;
 struct Pass {
   const int *tokens;  // first pass: the caller's tokens (row = index), else null
@@ -353,7 +364,10 @@ template <int ROUNDS, int BITS> __global__ void __launch_bounds__(THREADS) k_rad
 // shared memory, and what is left of the tile's first and last token over the tiles by k_embedding_join.  So a token's
 // rows are added in an order that depends on the sorted tokens alone, a token on most of the rows costs no more than
 // others, and each table row is written once.  Warps wait for no other warp: a CTA whose warps met at its end would stand
-// idle while its last rows arrive.
+// idle while its last rows arrive (that cost 22 of 129 us).  3.4 M rows of 64 16-bit values, 131072 tokens, the k-th in
+// frequency about 1 / k: 97 us, 4.8 TB/s of the 463 MB read and written; reading rows of 128 bytes in that order and adding them up
+// takes 76 us at best.  Tiles of 2048 entries a CTA took 120 us, a ring of asynchronous copies in front of the registers 130 us,
+// rows interleaved over a warp's groups with a sum over the warp at each change of token 156 us.
 constexpr int SUM_ROWS = 8, MAX_TILE = 256, MIN_TILE = 64; // rows a thread asks for at once
 struct Sums {
   const uint2 *entries;        // (token, row), sorted
@@ -523,7 +537,8 @@ template <class T, int W, int J> __global__ void __launch_bounds__(THREADS, 4) k
   __syncwarp();
   warp_sums<T, W, J>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
 }
-// The whole gradient of at most SMALL rows in one launch: the first CTAs (one a slab) sort the entries in shared memory and
+// The whole gradient of at most SMALL rows in one launch (203 rows of 32: 5.5 us on the GPU, where the eight launches of the
+// general form take 22 us): the first CTAs (one a slab) sort the entries in shared memory and
 // add them up; the others write the zeros of the rows that no token names, each for a range of `range` rows.
 constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
 template <class T, int W, int J>
@@ -606,7 +621,7 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
   }
 }
 // A token that begins in one tile and goes on in others: its parts are added up, in two steps so that one on most of the rows
-// does not keep a single CTA busy.  First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front
+// does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token; in two steps 9 us).  First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front
 // become one part, in the place of the first: a warp for each.
 __device__ __forceinline__ unsigned first_token(const Sums &p, int tiles, long long t) { return t < tiles ? p.entries[t * p.tile].x : (unsigned)p.vocab; }
 __global__ void __launch_bounds__(THREADS) k_embedding_join32(const Sums p, int tiles) {
