@@ -460,8 +460,9 @@ int scn_embedding_forward(const void *d_table, int table_type, int vocab, int C,
 /* The table's gradient: dtable[t][c] = scale * sum of dout[i][c] over the rows i with tokens[i] == t, in 32 bits.  The
  * rows are sorted by token (stably), each token's rows are added in an order that depends on the tokens alone: the
  * same call gives the same bits.  Without `accumulate` all vocab rows are written (zeros where no token points); with
- * it the sums are added onto what is there and rows without a token are left as they are.  Negative tokens and tokens at
- * or above vocab (these set SCN_DEV_ERR_KEY in *d_errors if not NULL) contribute nothing.
+ * it the sums are added onto what is there (magnitudes below 2^-126, there or in the result, may count as zero) and
+ * rows without a token are left as they are.  Negative tokens and tokens at or above vocab (these set
+ * SCN_DEV_ERR_KEY in *d_errors if not NULL) contribute nothing.
  *   d_dout      n rows of C values of dout_type, dout_stride (>= C) values apart
  *   d_workspace scn_embedding_backward_workspace_bytes(n, vocab, C) bytes (0: bad sizes), 16-byte aligned, nothing kept
  *               in it between calls; calls that can overlap on the GPU need a workspace each. */

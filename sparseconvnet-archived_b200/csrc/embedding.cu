@@ -538,8 +538,8 @@ template <class T, int W, int J> __global__ void __launch_bounds__(THREADS, 4) k
   warp_sums<T, W, J>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
 }
 // The whole gradient of at most SMALL rows in one launch (203 rows of 32: 5.5 us on the GPU, where the eight launches of the
-// general form take 22 us): the first CTAs (one a slab) sort the entries in shared memory and
-// add them up; the others write the zeros of the rows that no token names, each for a range of `range` rows.
+// general form take 22 us): the first CTAs (one a slab) sort the entries in shared memory and add them up; the others write the
+// zeros of the rows that no token names, each for a range of `range` rows.
 constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
 template <class T, int W, int J>
 __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums p, const T *dout, const int *tokens, int bits, int range, int *errors) {
@@ -621,8 +621,9 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
   }
 }
 // A token that begins in one tile and goes on in others: its parts are added up, in two steps so that one on most of the rows
-// does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token; in two steps 9 us).  First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front
-// become one part, in the place of the first: a warp for each.
+// does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token; in two steps 9 us).
+// First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front become one part, in the place
+// of the first: a warp for each.
 __device__ __forceinline__ unsigned first_token(const Sums &p, int tiles, long long t) { return t < tiles ? p.entries[t * p.tile].x : (unsigned)p.vocab; }
 __global__ void __launch_bounds__(THREADS) k_embedding_join32(const Sums p, int tiles) {
   wait_for_prior_grids();
