@@ -780,6 +780,7 @@ template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
 
 using namespace scn;
 static constexpr int MOST_COLUMNS = 1 << 28; // (a row's bytes fit 32 bits)
+static constexpr int MOST_GRADIENT_COLUMNS = 65535 * 64; // (slabs of at least 64 columns are a grid's second dimension)
 
 extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vocab, int C, const int *d_tokens, long long n, float scale, void *d_out,
                                      int out_type, long long out_stride, int *d_errors, scn_stream_t stream) {
@@ -797,7 +798,7 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
 }
 
 extern "C" size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C) {
-  if (n < 0 || n > 0x7fff0000ll || vocab < 1 || C < 1 || C > MOST_COLUMNS) return 0;
+  if (n < 0 || n > 0x7fff0000ll || vocab < 1 || C < 1 || C > MOST_GRADIENT_COLUMNS) return 0;
   return plan_sort(n, vocab, C).total;
 }
 
@@ -808,6 +809,7 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   if (vocab < 1 || C < 1 || C > MOST_COLUMNS || n < 0 || n > 0x7fff0000ll) return fail(SCN_ERR_INVALID, "bad embedding sizes");
   if (dout_stride < C) return fail(SCN_ERR_INVALID, "embedding: the gradient's row stride is below the number of features");
   if (!type_known(dout_type)) return fail(SCN_ERR_INVALID, "embedding: unknown type");
+  if (C > MOST_GRADIENT_COLUMNS) return fail(SCN_ERR_UNSUPPORTED, "embedding: a gradient has at most 4194240 features");
   if (dout_stride > 0xffffffffll / type_bytes(dout_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the gradient's rows lie 4 GiB apart or more");
   if (!d_dtable || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
   if (n && (!d_tokens || !d_dout)) return fail(SCN_ERR_INVALID, "null pointer");

@@ -28,6 +28,15 @@ def test_rows_too_far_apart(a):
     refused(a, a.lib().scn_embedding_backward(P, 7, P, 1, 1 << 31, 5, 4, 1.0, 0, P, None, P, 1 << 40, None), UNSUPPORTED, "4 GiB")
 
 
+@pytest.mark.parametrize("n", [7, 5000])
+@pytest.mark.parametrize("C", [4194241, 1 << 23, 1 << 28])
+def test_gradient_rows_too_wide(a, n, C):
+    """The gradient's kernels take 64 columns and more a slab, at most 65535 slabs."""
+    assert a.lib().scn_embedding_backward_workspace_bytes(n, 5, C) == 0
+    refused(a, a.lib().scn_embedding_backward(P, n, P, 0, C, 5, C, 1.0, 0, P, None, P, 1 << 40, None), UNSUPPORTED, "4194240")
+    assert a.lib().scn_embedding_backward_workspace_bytes(n, 5, 4194240) > 0
+
+
 @pytest.mark.parametrize("change,text", [
     (dict(vocab=0), "sizes"), (dict(C=0), "sizes"), (dict(n=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(stride=3), "row stride"), (dict(C=1 << 29, stride=1 << 29), "sizes"),
     (dict(table_type=3), "type"), (dict(out_type=-1), "type"), (dict(table=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
