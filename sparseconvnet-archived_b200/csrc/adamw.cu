@@ -549,6 +549,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
   if (!d_norm || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
   if (workspace_bytes < scn_grad_norm_workspace_bytes()) return fail(SCN_ERR_WORKSPACE, "workspace smaller than scn_grad_norm_workspace_bytes()");
   if ((uintptr_t)d_workspace & 7) return fail(SCN_ERR_INVALID, "AdamW: the workspace must be 8-byte aligned");
+  if ((uintptr_t)d_norm & 3) return fail(SCN_ERR_INVALID, "AdamW: misaligned pointer");
   cudaStream_t s = (cudaStream_t)stream;
   double *partial = (double *)d_workspace;
   const int most = (int)(scn_grad_norm_workspace_bytes() / sizeof(double));
@@ -572,6 +573,7 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
                               scn_stream_t stream) {
   clear_error();
   if (const char *why = wrong_list(tensors, count, true)) return fail(SCN_ERR_INVALID, why);
+  if (((uintptr_t)d_scalars | (uintptr_t)d_norm) & 3) return fail(SCN_ERR_INVALID, "AdamW: misaligned pointer");
   scn_adamw_scalars_t scalars = {};
   if (!d_scalars) {
     const int rc = scn_adamw_scalars(h, &scalars);
@@ -598,6 +600,7 @@ extern "C" int scn_adamw_decode(const void *d_codes, const float *d_scale, long 
   if (n < 0) return fail(SCN_ERR_INVALID, "bad size");
   if (n == 0) return SCN_OK;
   if (!d_codes || !d_scale || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
+  if (((uintptr_t)d_scale | (uintptr_t)d_out) & 3) return fail(SCN_ERR_INVALID, "AdamW: misaligned pointer");
   const long long wide = (((uintptr_t)d_codes & 7) | ((uintptr_t)d_out & 31)) == 0 ? n / 8 * 8 : 0;
   k_adamw_decode<<<grid_for((n + 7) / 8, THREADS, 32), THREADS, 0, (cudaStream_t)stream>>>((const unsigned char *)d_codes, d_scale, n, wide, second, d_out);
   SCN_LAUNCH_CHECK("k_adamw_decode");

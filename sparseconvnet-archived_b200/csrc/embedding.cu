@@ -791,6 +791,8 @@ extern "C" int scn_embedding_forward(const void *d_table, int table_type, int vo
   if (out_stride > 0xffffffffll / type_bytes(out_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the output's rows lie 4 GiB apart or more");
   if (n == 0) return SCN_OK;
   if (!d_table || !d_tokens || !d_out) return fail(SCN_ERR_INVALID, "null pointer");
+  if (((uintptr_t)d_table & (type_bytes(table_type) - 1)) | ((uintptr_t)d_out & (type_bytes(out_type) - 1)) | (((uintptr_t)d_tokens | (uintptr_t)d_errors) & 3))
+    return fail(SCN_ERR_INVALID, "embedding: misaligned pointer");
   const Lookup p = {(const char *)d_table, d_tokens, (char *)d_out, (unsigned)n, (unsigned)(out_stride * type_bytes(out_type)), (unsigned)C * type_bytes(table_type), vocab, C, scale, d_errors};
   SCN_DISPATCH_TYPE(table_type, T, SCN_DISPATCH_TYPE(out_type, O, SCN_CUDA_TRY((launch_forward<T, O>(p, (cudaStream_t)stream)))));
   SCN_LAUNCH_CHECK("k_embedding_forward");
@@ -813,6 +815,8 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   if (dout_stride > 0xffffffffll / type_bytes(dout_type)) return fail(SCN_ERR_UNSUPPORTED, "embedding: the gradient's rows lie 4 GiB apart or more");
   if (!d_dtable || !d_workspace) return fail(SCN_ERR_INVALID, "null pointer");
   if (n && (!d_tokens || !d_dout)) return fail(SCN_ERR_INVALID, "null pointer");
+  if (((uintptr_t)d_dout & (type_bytes(dout_type) - 1)) | (((uintptr_t)d_tokens | (uintptr_t)d_dtable | (uintptr_t)d_errors) & 3))
+    return fail(SCN_ERR_INVALID, "embedding: misaligned pointer");
   const SortPlan sp = plan_sort(n, vocab, C);
   if (workspace_bytes < sp.total) return fail(SCN_ERR_WORKSPACE, "workspace smaller than scn_embedding_backward_workspace_bytes()");
   if ((uintptr_t)d_workspace & 15) return fail(SCN_ERR_INVALID, "embedding: the workspace must be 16-byte aligned");

@@ -61,6 +61,24 @@ def test_gradient_refusals(a, change, code, text):
                                               need - k["short"], None), code, text)
 
 
+@pytest.mark.parametrize("at", range(9))
+def test_misaligned_pointers(a, at):
+    """Each pointer has to be aligned to its own type."""
+    L, h, t = a.lib(), parameters(a), (a.AdamWTensor * 1)(entry(a))
+    q = [P] * 9
+    q[at] += 1 if at < 3 else 2
+    if at < 4:  # 16-bit table and values at odd addresses, tokens and errors at half a word
+        refused(a, L.scn_embedding_forward(q[0], 1, 5, 4, q[3], 7, 1.0, q[1], 2, 4, q[2], None), INVALID, "misaligned")
+    if at in (1, 2, 3, 4):
+        refused(a, L.scn_embedding_backward(q[3], 7, q[1], 1, 4, 5, 4, 1.0, 0, q[4], q[2], P, 1 << 20, None), INVALID, "misaligned")
+    if at == 5:
+        refused(a, L.scn_grad_norm(t, 1, q[5], P, 1 << 20, None), INVALID, "misaligned")
+    if at >= 5 and at < 7:
+        refused(a, L.scn_adamw_step(t, 1, ctypes.byref(h), q[6] if at == 6 else None, q[5], None), INVALID, "misaligned")
+    if at >= 7:
+        refused(a, L.scn_adamw_decode(P + 1, q[7], 9, 0, q[8], None), INVALID, "misaligned")
+
+
 def test_workspace_sizes(a):
     f = a.lib().scn_embedding_backward_workspace_bytes
     assert f(-1, 5, 4) == f(1 << 31, 5, 4) == f(7, 0, 4) == f(7, 5, 0) == 0
