@@ -496,7 +496,7 @@ typedef struct {
   void *d_m, *d_v;     /* [n] the moments                                                              */
   float *d_m_scale, *d_v_scale;
   void *d_w16;         /* NULL, or [n]: the updated parameters rounded to w16_type (SCN_BF16, SCN_F16) */
-  long long n;
+  long long n;         /* at most 2^40; 2^43 in a list                                                 */
   float weight_decay, w_min;
   int g_type, w16_type;
 } scn_adamw_tensor_t;

@@ -111,6 +111,14 @@ def test_step_refuses_bad_tensors(a, change, text):
     refused(a, a.lib().scn_adamw_step(t, 2, ctypes.byref(h), None, None, None), INVALID, text)
 
 
+def test_lists_of_too_many_values(a):
+    """Several gradients may lie on one another for the norm: the list's values, not the memory, are what bounds it."""
+    t = (a.AdamWSeveralsor * 9)(*[entry(a, n=1 << 40) for _ in range(9)])
+    h = parameters(a)
+    refused(a, a.lib().scn_grad_norm(t, 9, P, P, 1 << 20, None), INVALID, "number of values")
+    refused(a, a.lib().scn_adamw_step(t, 9, ctypes.byref(h), None, None, None), INVALID, "number of values")
+
+
 @pytest.mark.parametrize("change,text", [
     (dict(lr=math.nan), "finite"), (dict(lr=math.inf), "finite"), (dict(grad_scale=math.nan), "finite"), (dict(beta1=1.0), "beta"), (dict(beta1=-0.1), "beta"),
     (dict(beta2=1.0), "beta"), (dict(beta2=math.nan), "beta"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=1e-39), "eps"), (dict(eps=-1.0), "eps"), (dict(step=0), "steps"),
