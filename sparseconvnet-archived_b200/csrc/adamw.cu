@@ -461,7 +461,8 @@ const char *wrong_list(const scn_adamw_tensor_t *t, int count, bool step) {
   for (int i = 0; i < count; ++i) {
     if (t[i].n < 0 || t[i].n > (1ll << 40)) return "AdamW: bad number of values";
     all += t[i].n;
-    if (all > (1ll << 43)) return "AdamW: bad number of values"; // (a list's chunks count in 32 bits: one launch for each SCN_ADAMW_MAX_TENSORS, as the norm's workspace expects)
+    // (chunks count in 32 bits: so many fit one launch for each SCN_ADAMW_MAX_TENSORS, which the norm's workspace expects)
+    if (all > (1ll << 43)) return "AdamW: bad number of values";
     if (!type_known(t[i].g_type)) return "AdamW: unknown gradient type";
     if (t[i].n && !t[i].d_g) return "null pointer";
     if (!step) continue;

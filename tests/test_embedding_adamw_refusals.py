@@ -113,7 +113,7 @@ def test_step_refuses_bad_tensors(a, change, text):
 
 def test_lists_of_too_many_values(a):
     """Several gradients may lie on one another for the norm: the list's values, not the memory, are what bounds it."""
-    t = (a.AdamWSeveralsor * 9)(*[entry(a, n=1 << 40) for _ in range(9)])
+    t = (a.AdamWTensor * 9)(*[entry(a, n=1 << 40) for _ in range(9)])
     h = parameters(a)
     refused(a, a.lib().scn_grad_norm(t, 9, P, P, 1 << 20, None), INVALID, "number of values")
     refused(a, a.lib().scn_adamw_step(t, 9, ctypes.byref(h), None, None, None), INVALID, "number of values")
