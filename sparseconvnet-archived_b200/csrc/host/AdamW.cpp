@@ -43,8 +43,7 @@ void AdamW::update(const std::vector<LearntParameter> &parameters, float learnin
     t.g_type = SCN_F32;
     list.push_back(t);
   }
-  ++step;
-  const scn_adamw_t h = {learningRate, beta1, beta2, eps, 1.0 / batchSize, maxNorm, step, (unsigned)step};
+  const scn_adamw_t h = {learningRate, beta1, beta2, eps, 1.0 / batchSize, maxNorm, step + 1, (unsigned)(step + 1)};
   float *norm = nullptr;
   if (maxNorm > 0) {
     const size_t bytes = scn_grad_norm_workspace_bytes();
@@ -53,4 +52,5 @@ void AdamW::update(const std::vector<LearntParameter> &parameters, float learnin
     scnSafeCall(scn_grad_norm(list.data(), (int)list.size(), norm, scratch, bytes, memStream.stream));
   }
   scnSafeCall(scn_adamw_step(list.data(), (int)list.size(), &h, nullptr, norm, memStream.stream));
+  ++step; // (not where a call above was refused)
 }

@@ -25,7 +25,7 @@ public:
   AdamW(const AdamW &) = delete;
   AdamW &operator=(const AdamW &) = delete;
   // One step.  The gradients are sums over `batchSize` samples; the step takes their mean (and clips its norm).  A norm that is
-  // not finite, where maxNorm is set, leaves everything as it is.
+  // not finite, where maxNorm is set, leaves the parameters and moments as they are (the step counts all the same).
   void update(const std::vector<LearntParameter> &parameters, float learningRate, int batchSize, cudaMemStream &memStream);
 
 private:

@@ -376,8 +376,15 @@ void SparseConvNetCUDA::useSymbols(int nSymbols, float scale, const float *value
 }
 // Every layer's backwards in reverse order, then, where they leave it, the update.
 void SparseConvNetCUDA::learn(SpatiallySparseBatch &batch, float learningRate, float momentum) {
-  for (auto l : layers)
-    if (auto n = dynamic_cast<NetworkInNetworkLayer *>(l)) n->deferUpdate = adamW != nullptr;
+  struct Deferring { // (a layer's backwards() called by itself still updates that layer)
+    std::vector<SpatiallySparseLayer *> &layers;
+    Deferring(std::vector<SpatiallySparseLayer *> &layers, bool on) : layers(layers) { set(on); }
+    ~Deferring() { set(false); }
+    void set(bool on) {
+      for (auto l : layers)
+        if (auto n = dynamic_cast<NetworkInNetworkLayer *>(l)) n->deferUpdate = on;
+    }
+  } deferring(layers, adamW != nullptr);
   for (int i = (int)layers.size() - 1; i >= 0; --i) layers[i]->backwards(batch, batch.interfaces[i], batch.interfaces[i + 1], learningRate, momentum);
   SpatiallySparseBatchInterface &in = batch.interfaces[0];
   const bool symbols = symbolTable && in.symbols.size() > 0;
