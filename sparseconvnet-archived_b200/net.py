@@ -354,6 +354,8 @@ class Net:
         keys = np.ascontiguousarray(keys, np.int32)
         off = np.ascontiguousarray(off, np.int32)
         symbols = np.ascontiguousarray(symbols, np.int32)
+        if len(off) and not off[-1] <= min(len(keys), len(symbols)):
+            raise abi.ScnError("%d rows need a key and a symbol each" % off[-1])
         B = len(off) - 1
         probs = np.empty((B, self.nClasses), np.float32)
         pred = np.empty((B, self.nTop), np.int32)
@@ -365,6 +367,8 @@ class Net:
         keys = np.ascontiguousarray(keys, np.int32)
         off = np.ascontiguousarray(off, np.int32)
         symbols = np.ascontiguousarray(symbols, np.int32)
+        if len(off) and not off[-1] <= min(len(keys), len(symbols)):
+            raise abi.ScnError("%d rows need a key and a symbol each" % off[-1])
         labels = np.ascontiguousarray(labels, np.int32)
         B = len(off) - 1
         probs = np.empty((B, self.nClasses), np.float32)

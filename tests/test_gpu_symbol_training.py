@@ -297,3 +297,33 @@ def test_refusals(scn, abi, table):
         net.set_symbols(table)  # its moments belong to the table that is there
     probs, _ = net.forward_host_symbols(keys, off, syms)
     assert np.isfinite(probs).all()
+
+
+def test_fewer_symbols_than_rows(scn, abi, table):
+    net = build(scn, abi, abi.VLEAKYRELU)
+    net.set_symbols(table)
+    keys, off, syms, labels = batch(net.inputSpatialSize, 8)
+    for k, y in [(keys, syms[:-1]), (keys[:-1], syms)]:
+        with pytest.raises(abi.ScnError, match="rows need"):
+            net.forward_host_symbols(k, off, y)
+        with pytest.raises(abi.ScnError, match="rows need"):
+            net.train_batch_symbols(k, off, y, labels, 0.1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_dropped_features_stay(scn, abi, table, bits):
+    """A first step without weight decay: the weights of the features that the batch drops have gradients of zero and moments of
+    zero, so they keep their bits; each of the others with a gradient far above eps moves by the learning rate."""
+    net = build(scn, abi, abi.VLEAKYRELU, dropout=0.5)
+    at = [i for i, L in enumerate(net.layers()) if L["type"] == 2][1]
+    net.set_symbols(table)
+    keys, off, syms, labels = batch(net.inputSpatialSize, 5)
+    kept = np.arange(0, 64, 2)
+    net.set_dropout_features(at, kept)
+    net.use_adamw(weight_decay=0.0, state_bits=bits)
+    W0, B0 = net.get_weights(at)[:2]
+    net.train_batch_symbols(keys, off, syms, labels, 1e-3)
+    W1, B1 = net.get_weights(at)[:2]
+    dropped = np.setdiff1d(np.arange(64), kept)
+    assert np.array_equal(W0[:, dropped], W1[:, dropped]) and np.array_equal(B0[dropped], B1[dropped])
+    assert (W0[:, kept] != W1[:, kept]).mean() > 0.5
