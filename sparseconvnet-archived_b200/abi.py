@@ -599,7 +599,7 @@ def _row_stride(t, n, C, what):
         if rows == n and columns == C:
             stride, inner = t.stride()
             if n <= 1:
-                stride = max(stride, C)
+                stride = C  # (no second row)
             if (inner == 1 or C == 1) and stride >= C:
                 return stride
             raise ScnError("invalid argument: %s: the values of a row must lie together and rows must not overlap" % what)
@@ -680,7 +680,8 @@ class AdamW:
     """scn_adamw_step / scn_grad_norm over a fixed list of tensors.  Each entry is a dict of contiguous CUDA tensors: w (float32),
     g (float32, bfloat16 or float16), m and v (float32; or int8 and uint8 with float32 m_scale and v_scale, see
     adamw_states), optionally w16 (bfloat16 or float16, receives the updated w), and numbers weight_decay and w_min.
-    The object keeps references to the tensors; their memory must stay where it is."""
+    The object keeps references to the tensors; their memory must stay where it is.  It owns one norm and one workspace: its
+    calls on different streams, or captured into graphs, must not overlap on the GPU."""
 
     def __init__(self, tensors):
         self.tensors = [dict(t) for t in tensors]
@@ -751,7 +752,7 @@ class AdamW:
                 raise ScnError("invalid argument: a step needs lr and its number")
             numbers = (lr, beta1, beta2, eps, grad_scale, max_norm, step, step if seed is None else seed)
             if numbers != self._set:
-                p = self.h
+                p, self._set = self.h, None
                 p.lr, p.beta1, p.beta2, p.eps, p.grad_scale, p.max_norm, p.step, p.seed = numbers[:7] + (numbers[7] & 0xFFFFFFFF,)
                 self._set = numbers
             h, sp = self._h, None

@@ -172,3 +172,14 @@ def test_python_binding_refuses_cpu_tensors(a):
         a.adamw_states(5, "cpu", bits=16)
     with pytest.raises(a.ScnError, match="w must be"):
         a.AdamW([dict(w=torch.zeros(4), g=torch.zeros(4), **a.adamw_states(4, "cpu", bits=32))])
+
+
+def test_row_strides(a):
+    """A single row has no stride to speak of, however its view was made; several rows must not overlap."""
+    assert a._row_stride(torch.empty_strided((1, 4), (1 << 40, 1)), 1, 4, "out") == 4
+    assert a._row_stride(torch.empty(0, 4), 0, 4, "out") == 4
+    assert a._row_stride(torch.empty(3, 9)[:, 2:6], 3, 4, "out") == 9
+    assert a._row_stride(torch.empty(3, 9)[:, 2:3], 3, 1, "out") == 9
+    for bad in [torch.empty(1, 4).expand(3, 4), torch.empty(4, 3).t(), torch.empty(3, 8)[:, ::2], torch.empty(3, 4, dtype=torch.float64), torch.empty(12)]:
+        with pytest.raises(a.ScnError):
+            a._row_stride(bad, 3, 4, "out")

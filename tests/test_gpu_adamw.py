@@ -521,3 +521,17 @@ def test_codes_of_a_large_tensor(abi):
             codes, scale = torch_encode(x, (bits.float() + 0.5) * 2.0 ** -16, k == "v")
             assert torch.equal(t[k + "_scale"], scale) and int((t[k] != codes).sum()) == 0, k
         m, v = abi.adamw_decode(t["m"], t["m_scale"]), abi.adamw_decode(t["v"], t["v_scale"])
+
+
+def test_numbers_after_a_refused_step(abi):
+    """A step with numbers that are none raises and leaves nothing behind: the next one takes its own."""
+    def run(spoil):
+        w, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+        opt = abi.AdamW([dict(w=w, g=g, **abi.adamw_states(300, "cuda", 32))])
+        opt.step(0.1, 1)
+        if spoil:
+            with pytest.raises(TypeError):
+                opt.step(0.7, "two", seed=0)
+        opt.step(0.1, 1)
+        return w
+    assert torch.equal(run(False), run(True))
