@@ -154,6 +154,8 @@ struct Pass {
   int *errors;
   float *clear;       // first pass: clearN values to set to zero on the side, or null
   long long clearN;
+  unsigned *arrived;  // first pass: the sums' counters to set to zero (see join_group), or null
+  long long arrivedN;
 };
 // The token, or vocab (sorted behind all tokens) where it names no row.
 __device__ __forceinline__ unsigned key_of(int token, int vocab) { return token >= 0 && token < vocab ? (unsigned)token : (unsigned)vocab; }
@@ -172,6 +174,7 @@ template <int ROUNDS> __global__ void __launch_bounds__(THREADS) k_radix_count(c
     clear_floats(p.clear, p.clearN, (long long)(blockIdx.x - p.tiles) * THREADS + threadIdx.x, (long long)(gridDim.x - p.tiles) * THREADS);
     return;
   }
+  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < p.arrivedN; i += (long long)p.tiles * THREADS) p.arrived[i] = 0;
   const int digits = 1 << p.bits;
   const long long first = (long long)blockIdx.x * (THREADS * ROUNDS);
   unsigned key[ROUNDS];
@@ -378,6 +381,8 @@ struct Sums {
   int accumulate;
   float *dtable;
   float *head, *tail;          // [tiles][C]: the part of a tile's first (last) token, where that began (goes on) in another tile
+  uint2 *ends;                 // [tiles]: each tile's first and last token
+  unsigned *arrived;           // [slabs][tiles / 32], or null: see join_group
 };
 // The running sums of W columns.
 template <int W> struct Columns {
@@ -508,7 +513,34 @@ __device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const ui
     }
   }
 }
-template <class T, int W, int J> __global__ void __launch_bounds__(THREADS, 4) k_embedding_sums(const Sums p, const T *dout) {
+// A token that begins in one tile and goes on in others has its parts added up, in two steps so that one on most of the rows
+// does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token).  First 32 tiles (from a
+// multiple of 32 on) that all begin with a token from further in front become one part, in the place of the first: the last of
+// their warps adds them up, so that nothing is launched for it (224 k rows: 49.5 -> 45 us for the whole gradient).  Where there are
+// few tiles, the second step's CTA takes them faster by itself (50 k rows: 28 us against 32).
+__device__ __forceinline__ void join_group(const Sums &p, long long tile, unsigned key, int first, int columns) {
+  const int lane = threadIdx.x & 31;
+  const long long t0 = tile / 32 * 32, tiles = (p.n + p.tile - 1ll) / p.tile;
+  if (t0 == 0 || t0 + 32 > tiles || p.entries[t0 * p.tile - 1].x != key) return;
+  unsigned before = 0;
+  __syncwarp();
+  if (lane == 0) {
+    __threadfence();
+    before = atomicAdd(p.arrived + blockIdx.y * (tiles / 32) + tile / 32, 1u);
+    __threadfence();
+  }
+  __syncwarp();
+  if (__shfl_sync(~0u, before, 0) != 31) return;
+  float *at = p.head + t0 * p.C + first;
+  for (int c = lane; c < columns; c += 32) {
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 32; ++t) sum += __ldcg(at + (long long)t * p.C + c);
+    at[c] = sum;
+  }
+}
+// GROUPS: whether tiles are joined by 32 (the code for it, unused, costs narrow types registers: 50 k rows of 33 floats 28 -> 32 us).
+template <class T, int W, int J, bool GROUPS> __global__ void __launch_bounds__(THREADS, 4) k_embedding_sums(const Sums p, const T *dout) {
   __shared__ uint2 entries[WARPS][MAX_TILE + SUM_ROWS];
   __shared__ Items<W, J> items[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -529,15 +561,23 @@ template <class T, int W, int J> __global__ void __launch_bounds__(THREADS, 4) k
     if (r * 32 + lane < most) entry[r * 32 + lane] = e[r];
     count += __popc(__ballot_sync(~0u, e[r].x != none));
   }
-  if (count == 0) return;
   __syncwarp();
+  if (lane == 0 && blockIdx.y == 0) p.ends[tile] = make_uint2(e[0].x, entry[most - 1].x);
+  if (count == 0) return;
   const unsigned any = entry[count - 1].y;
   __syncwarp();
   if (lane < SUM_ROWS) entry[count + lane] = make_uint2(none, any);
   __syncwarp();
   warp_sums<T, W, J>(p, dout, entry, count, before, count == most ? next : none, items[warp], p.head + tile * p.C, p.tail + tile * p.C);
+  if constexpr (GROUPS) {
+    const unsigned key = entry[0].x; // (all the tile's, or the last tile's of 32: the others cannot be part of 32 that begin alike)
+    if (key == before && (entry[count - 1].x == key || (tile & 31) == 31)) {
+      const int column0 = blockIdx.y * 32 * W * J;
+      join_group(p, tile, key, column0, min(p.C - column0, 32 * W * J));
+    }
+  }
 }
-// The whole gradient of at most SMALL rows in one launch (203 rows of 32: 5.5 us on the GPU, where the eight launches of the
+// The whole gradient of at most SMALL rows in one launch (203 rows of 32: 5.5 us on the GPU, where the launches of the
 // general form take 22 us): the first CTAs (one a slab) sort the entries in shared memory and add them up; the others write the
 // zeros of the rows that no token names, each for a range of `range` rows.
 constexpr int SMALL_ROUNDS = 4, SMALL = THREADS * SMALL_ROUNDS, SMALL_DIGIT = 8, MOST_RANGE = 16384;
@@ -620,37 +660,17 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
     write_row<1>(p, last, column0 + x, sum);
   }
 }
-// A token that begins in one tile and goes on in others: its parts are added up, in two steps so that one on most of the rows
-// does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token; in two steps 9 us).
-// First 32 tiles (from a multiple of 32 on) that all begin with a token from further in front become one part, in the place
-// of the first: a warp for each.
-__device__ __forceinline__ unsigned first_token(const Sums &p, int tiles, long long t) { return t < tiles ? p.entries[t * p.tile].x : (unsigned)p.vocab; }
-__global__ void __launch_bounds__(THREADS) k_embedding_join32(const Sums p, int tiles) {
-  wait_for_prior_grids();
-  dependents_may_launch();
-  const int lane = threadIdx.x & 31;
-  const long long t0 = 32ll * (blockIdx.x * WARPS + (threadIdx.x >> 5));
-  if (t0 == 0 || t0 + 32 > tiles) return;
-  const unsigned k = p.entries[t0 * p.tile - 1].x;
-  if (k == (unsigned)p.vocab || !__all_sync(~0u, first_token(p, tiles, t0 + lane) == k)) return;
-  for (int c = lane; c < p.C; c += 32) {
-    float sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < 32; ++t) sum += p.head[(t0 + t) * p.C + c];
-    p.head[t0 * p.C + c] = sum;
-  }
-}
 // Then a warp looks at one tile after the other and adds up a token that begins in it and goes on in fewer than 32 more; a longer
-// one is left for the whole CTA, whose warps take every JOIN_WARPS-th part and add up what they have.  joined: whether
-// k_embedding_join32 ran (not where there are few tiles).
-constexpr int JOIN_THREADS = 512, JOIN_WARPS = JOIN_THREADS / 32, JOIN_COLUMNS = 4; // columns of a thread at once
-__global__ void __launch_bounds__(JOIN_THREADS) k_embedding_join(const Sums p, int tiles, int joined) {
+// one is left for the whole CTA, whose warps take every JOIN_WARPS-th part and add up what they have.
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_COLUMNS = 4; // columns of a thread at once
+__global__ void __launch_bounds__(JOIN_THREADS) k_embedding_join(const Sums p, int tiles) {
   __shared__ float share[JOIN_WARPS][32 * JOIN_COLUMNS];
   __shared__ int longOnes[JOIN_WARPS], found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned none = p.vocab;
   wait_for_prior_grids();
   dependents_may_launch();
+  const auto first_token = [&](long long t) { return t < tiles ? p.ends[t].x : none; };
   // columns c, c + 32, ... of parts begin, begin + step, ...: added to sum
   const auto add_parts = [&](float (&sum)[JOIN_COLUMNS], int c, int begin, int end, int step, auto row_of) {
 #pragma unroll 4
@@ -662,12 +682,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_embedding_join(const Sums p, i
   };
   for (int base = blockIdx.x * JOIN_WARPS; base < tiles; base += gridDim.x * JOIN_WARPS) {
     const int b = base + warp;
-    const long long first = (long long)b * p.tile, end = first + p.tile;
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
-    if (end < p.n) {
-      const unsigned k = p.entries[end - 1].x, before = first > 0 ? p.entries[first - 1].x : none;
-      const unsigned follows = first_token(p, tiles, (long long)b + 1 + lane); // the tokens that the next tiles begin with
+    if (b + 1 < tiles) {
+      const unsigned k = p.ends[b].y, before = b > 0 ? p.ends[b - 1].y : none;
+      const unsigned follows = first_token((long long)b + 1 + lane); // the tokens that the next tiles begin with
       const unsigned same = __ballot_sync(~0u, follows == k);
       if (k != none && (same & 1) && before != k) {
         if (same == ~0u) {
@@ -686,17 +705,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_embedding_join(const Sums p, i
     __syncthreads();
     for (int l = 0; l < found; ++l) {
       const int t0 = longOnes[l];
-      const unsigned k = p.entries[(long long)(t0 + 1) * p.tile].x;
+      const unsigned k = p.ends[t0].y;
       int last = t0 + 1, beyond = tiles; // the last tile that begins with k: `last` does, `beyond` does not
       while (beyond - last > 1) {
         const int step = (beyond - last + JOIN_THREADS - 1) / JOIN_THREADS;
-        const int with = __syncthreads_count(first_token(p, tiles, (long long)last + (long long)threadIdx.x * step) == k);
+        const int with = __syncthreads_count(first_token((long long)last + (long long)threadIdx.x * step) == k);
         last += (with - 1) * step;
         beyond = (int)min((long long)beyond, (long long)last + step);
       }
       ++last;
       // the parts: t0's tail, single tiles, 32 tiles at a time where they have been joined, single tiles
-      const int from = min(last, joined ? (t0 + 32) / 32 * 32 : last), to = max(from, last / 32 * 32);
+      const int from = min(last, p.arrived ? (t0 + 32) / 32 * 32 : last), to = max(from, last / 32 * 32);
       const int singles = from - t0, both = singles + (to - from) / 32, parts = both + max(0, last - to);
       const auto row_of = [&](int i) {
         const int t = i < singles ? t0 + i : i < both ? from + 32 * (i - singles) : to + i - both;
@@ -733,7 +752,7 @@ int pack_width(int type, const void *dout, long long stride, const float *dtable
 // Entries a warp sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than 16 warps each.
 int sum_tile(long long n) {
   int tile = MAX_TILE;
-  while (tile > MIN_TILE && n / tile < 16 * 148) tile /= 2;
+  while (tile > MIN_TILE && n < 16ll * 148 * tile) tile /= 2;
   return tile;
 }
 
@@ -742,7 +761,9 @@ constexpr int FEW_TILES = 64;
 int sort_rounds(long long n) { return n > (1 << 20) ? LARGE_ROUNDS : 4; } // large tiles: longer runs of a digit; small ones: work for every SM
 struct SortPlan {
   int tiles, passes, bits, digit;            // digit: bits a pass
-  size_t array, counts, totals, parts, total; // bytes
+  int sumTile;
+  long long sumTiles;
+  size_t array, counts, totals, parts, ends, arrived, total; // bytes
 };
 SortPlan plan_sort(long long n, int vocab, int C) {
   SortPlan p;
@@ -755,8 +776,12 @@ SortPlan plan_sort(long long n, int vocab, int C) {
   p.array = align_up(sizeof(uint2) * (size_t)n, 256);
   p.counts = align_up(sizeof(unsigned) * ((size_t)p.tiles << p.digit), 256);
   p.totals = align_up(sizeof(unsigned) << p.digit, 256);
-  p.parts = align_up(sizeof(float) * (size_t)((n + sum_tile(n) - 1) / sum_tile(n)) * (size_t)C, 256); // of each tile's first and last token
-  p.total = 2 * p.array + p.counts + p.totals + 2 * p.parts + 256;
+  p.sumTile = sum_tile(n);
+  p.sumTiles = (n + p.sumTile - 1) / p.sumTile;
+  p.parts = align_up(sizeof(float) * (size_t)p.sumTiles * (size_t)C, 256); // of each tile's first and last token
+  p.ends = align_up(sizeof(uint2) * (size_t)p.sumTiles, 256);
+  p.arrived = align_up(sizeof(unsigned) * (size_t)(p.sumTiles / 32) * (size_t)((C + 63) / 64), 256);
+  p.total = 2 * p.array + p.counts + p.totals + 2 * p.parts + p.ends + p.arrived + 256;
   return p;
 }
 template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
@@ -831,24 +856,26 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   Sums q = {};
   q.n = (int)n; q.vocab = vocab; q.C = C; q.stride = (unsigned)(dout_stride * type_bytes(dout_type));
   q.lanes = J > 1 ? 32 : vectors - (slabs - 1) * 32;
-  q.tile = sum_tile(n);
+  q.tile = sp.sumTile;
   q.scale = scale; q.accumulate = accumulate; q.dtable = d_dtable;
   q.head = (float *)(w + 2 * sp.array + sp.counts + sp.totals);
   q.tail = (float *)(w + 2 * sp.array + sp.counts + sp.totals + sp.parts);
-  // F<T, W, J> for dout's type, the width and the pieces
+  q.ends = (uint2 *)(w + 2 * sp.array + sp.counts + sp.totals + 2 * sp.parts);
+  // F(T, W, J) for dout's type, the width and the pieces
 #define SCN_SUMS(F, ...)                                                                                              \
   SCN_DISPATCH_TYPE(dout_type, T, {                                                                                   \
     constexpr int MOST = 16 / (int)sizeof(T);                                                                         \
-    if (W == MOST) SCN_CUDA_TRY(launch_dependent(F<T, MOST, 1>, __VA_ARGS__));                                        \
-    else if (W == MOST / 2) SCN_CUDA_TRY(launch_dependent(F<T, MOST / 2, 1>, __VA_ARGS__));                           \
-    else if (W == 2) SCN_CUDA_TRY(launch_dependent(F<T, 2, 1>, __VA_ARGS__));                                         \
-    else if (J == 1) SCN_CUDA_TRY(launch_dependent(F<T, 1, 1>, __VA_ARGS__));                                         \
-    else if (J == 2) SCN_CUDA_TRY(launch_dependent(F<T, 1, 2>, __VA_ARGS__));                                         \
-    else SCN_CUDA_TRY(launch_dependent(F<T, 1, 4>, __VA_ARGS__));                                                     \
+    if (W == MOST) SCN_CUDA_TRY(launch_dependent(F(T, MOST, 1), __VA_ARGS__));                                        \
+    else if (W == MOST / 2) SCN_CUDA_TRY(launch_dependent(F(T, MOST / 2, 1), __VA_ARGS__));                           \
+    else if (W == 2) SCN_CUDA_TRY(launch_dependent(F(T, 2, 1), __VA_ARGS__));                                         \
+    else if (J == 1) SCN_CUDA_TRY(launch_dependent(F(T, 1, 1), __VA_ARGS__));                                         \
+    else if (J == 2) SCN_CUDA_TRY(launch_dependent(F(T, 1, 2), __VA_ARGS__));                                         \
+    else SCN_CUDA_TRY(launch_dependent(F(T, 1, 4), __VA_ARGS__));                                                     \
   })
   if (n <= SMALL) {
     const int range = std::max(32, std::min(MOST_RANGE, (vocab + 4 * sm_count() - 1) / (4 * sm_count()))), clearing = accumulate ? 0 : (vocab + range - 1) / range;
-    SCN_SUMS(k_embedding_backward_small, dim3(1 + clearing, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout, d_tokens, sp.bits, range, d_errors);
+#define SCN_SMALL(T, W, J) (k_embedding_backward_small<T, W, J>)
+    SCN_SUMS(SCN_SMALL, dim3(1 + clearing, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout, d_tokens, sp.bits, range, d_errors);
     SCN_LAUNCH_CHECK("k_embedding_backward_small");
     return SCN_OK;
   }
@@ -858,6 +885,8 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
   p.counts = (unsigned *)(w + 2 * sp.array);
   p.totals = sp.tiles > FEW_TILES ? (unsigned *)(w + 2 * sp.array + sp.counts) : nullptr;
   p.errors = d_errors;
+  const int tiles = (int)sp.sumTiles;
+  if (tiles > 2048) q.arrived = (unsigned *)(w + 2 * sp.array + sp.counts + sp.totals + 2 * sp.parts + sp.ends);
   for (int k = 0; k < sp.passes; ++k) {
     p.tokens = k == 0 ? d_tokens : nullptr;
     p.in = array[(k + 1) & 1];
@@ -865,21 +894,20 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     p.shift = k * sp.digit;
     p.clear = k == 0 && !accumulate ? d_dtable : nullptr;
     p.clearN = (long long)vocab * C;
+    p.arrived = q.arrived;
+    p.arrivedN = k == 0 && q.arrived ? (long long)tiles / 32 * slabs : 0;
     const int rc = sort_rounds(n) == 4 ? sort_pass<4>(p, s) : sort_pass<LARGE_ROUNDS>(p, s);
     if (rc != SCN_OK) return rc;
   }
   q.entries = p.out;
-  const int tiles = (int)((n + q.tile - 1) / q.tile);
-  SCN_SUMS(k_embedding_sums, dim3((tiles + WARPS - 1) / WARPS, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout);
+#define SCN_TILES(T, W, J) (q.arrived ? k_embedding_sums<T, W, J, true> : k_embedding_sums<T, W, J, false>)
+  SCN_SUMS(SCN_TILES, dim3((tiles + WARPS - 1) / WARPS, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout);
 #undef SCN_SUMS
+#undef SCN_SMALL
+#undef SCN_TILES
   SCN_LAUNCH_CHECK("k_embedding_sums");
   if (tiles > 1) {
-    const int joined = tiles > 2048;
-    if (joined) {
-      SCN_CUDA_TRY(launch_dependent(k_embedding_join32, dim3((tiles / 32 + WARPS - 1) / WARPS), dim3(THREADS), 0, s, q, tiles));
-      SCN_LAUNCH_CHECK("k_embedding_join32");
-    }
-    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(std::min((tiles + JOIN_WARPS - 1) / JOIN_WARPS, 8 * sm_count())), dim3(JOIN_THREADS), 0, s, q, tiles, joined));
+    SCN_CUDA_TRY(launch_dependent(k_embedding_join, dim3(std::min((tiles + JOIN_WARPS - 1) / JOIN_WARPS, 8 * sm_count())), dim3(JOIN_THREADS), 0, s, q, tiles));
     SCN_LAUNCH_CHECK("k_embedding_join");
   }
   return SCN_OK;

@@ -291,3 +291,27 @@ def test_refusals_of_the_binding(abi):
                 lambda: abi.embedding_backward(dout, tok, table, workspace=torch.empty(1 << 20, device="cuda"))]:
         with pytest.raises(abi.ScnError):
             bad()
+
+
+@pytest.mark.parametrize("C", [1, 64, 100, 300])
+@pytest.mark.parametrize("n,starts", [
+    (4096, [0]), (4097, [0]), (6143, [0, 1]), (20000, [0]), (20000, [2048]), (20000, [2047]), (20000, [2049]), (20000, [2048, 4096]), (20000, [2047, 4095]),
+    (20000, [2049, 4097]), (20000, [1984, 4032]), (20000, [2112, 4160]), (20000, [100, 6000, 14000, 19999]), (20000, [0, 64, 128, 8000]), (70000, [5, 40000]),
+    (70000, [33000, 66000]), (700001, [0, 350000]), (700001, [65536, 131072]), (700001, [65535, 131073, 600000]),
+])
+@pytest.mark.parametrize("missing", [0, 3000])
+def test_long_tokens(abi, n, starts, missing, C):
+    """Tokens on thousands of rows, that begin at, before and behind the places where their parts are joined (64 to 256 rows a part, then
+    32 parts).  Whole numbers of at most 4: the sums of 700 k of them stay below 2^24, so they are exact in whatever order."""
+    gen = torch.Generator(device="cuda").manual_seed(n + C)
+    at = torch.arange(n, device="cuda")
+    tok = torch.bucketize(at, torch.tensor(starts, device="cuda"), right=True).int() * 3
+    if missing:
+        tok[-missing:] = -1
+    order = torch.randperm(n, device="cuda", generator=gen)
+    tok = tok[order].contiguous()
+    dout = torch.randint(-4, 5, (n, C), device="cuda", generator=gen).float()
+    V = 3 * len(starts) + 2
+    want = torch.zeros(V, C, dtype=torch.float64, device="cuda").index_add_(0, tok[tok >= 0].long(), dout[tok >= 0].double())
+    got = abi.embedding_backward(dout, tok, torch.full((V, C), 7.0, device="cuda"))
+    assert torch.equal(got.double(), want)
