@@ -214,20 +214,28 @@ __device__ __forceinline__ unsigned sum_before(unsigned own, unsigned *warpSum, 
   __syncthreads();
   return before + sum - own;
 }
-// One CTA for SCAN_DIGITS digits (so many counts of a tile fill a sector): counts[*][d] becomes its exclusive running sum over the
+// One CTA for SCAN_DIGITS digits (half a sector of each tile's counts, so that more SMs share the work): counts[*][d] becomes its exclusive running sum over the
 // tiles, totals[d] its sum.  A thread takes one digit of a run of the tiles: it adds them up, learns what the runs before hold,
-// and writes the running sums.
-constexpr int SCAN_DIGITS = 8, SCAN_THREADS = 1024, SCAN_RUNS = SCAN_THREADS / SCAN_DIGITS;
-__global__ void __launch_bounds__(SCAN_THREADS) k_radix_scan(const Pass p) {
+// and writes the running sums.  HELD: counts that stay in its registers in between, or 0 (reading them again
+// took 3.4 M rows' gradient 187 us in place of 180).
+constexpr int SCAN_DIGITS = 4, SCAN_THREADS = 1024, SCAN_RUNS = SCAN_THREADS / SCAN_DIGITS;
+template <int HELD> __global__ void __launch_bounds__(SCAN_THREADS) k_radix_scan(const Pass p) {
   __shared__ unsigned runSum[SCAN_RUNS][SCAN_DIGITS];
   wait_for_prior_grids();
   dependents_may_launch();
   const int digits = 1 << p.bits, d = threadIdx.x % SCAN_DIGITS, run = threadIdx.x / SCAN_DIGITS;
   const int each = (p.tiles + SCAN_RUNS - 1) / SCAN_RUNS, begin = min(run * each, p.tiles), end = min(begin + each, p.tiles);
   unsigned *column = p.counts + blockIdx.x * SCAN_DIGITS + d;
-  unsigned sum = 0;
+  unsigned sum = 0, held[HELD > 0 ? HELD : 1];
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) held[u] = begin + u < end ? column[(long long)(begin + u) * digits] : 0u;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) sum += held[u];
+  } else {
 #pragma unroll 8
-  for (int t = begin; t < end; ++t) sum += column[(long long)t * digits];
+    for (int t = begin; t < end; ++t) sum += column[(long long)t * digits];
+  }
   runSum[run][d] = sum;
   __syncthreads();
   if (threadIdx.x < 32 * SCAN_DIGITS) { // a warp a digit: running sums over the runs
@@ -247,12 +255,13 @@ __global__ void __launch_bounds__(SCAN_THREADS) k_radix_scan(const Pass p) {
   }
   __syncthreads();
   unsigned before = runSum[run][d];
-  for (int t0 = begin; t0 < end; t0 += 8) {
-    unsigned n[8];
+  constexpr int TURN = HELD > 0 ? HELD : 8;
+  for (int t0 = begin; t0 < end; t0 += TURN) {
+    unsigned n[TURN];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) n[u] = t0 + u < end ? column[(long long)(t0 + u) * digits] : 0u;
+    for (int u = 0; u < TURN; ++u) n[u] = HELD > 0 ? held[HELD > 0 ? u : 0] : t0 + u < end ? column[(long long)(t0 + u) * digits] : 0u;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < TURN; ++u) {
       if (t0 + u < end) column[(long long)(t0 + u) * digits] = before;
       before += n[u];
     }
@@ -788,7 +797,9 @@ template <int ROUNDS> int sort_pass(const Pass &p, cudaStream_t s) {
   const int digits = 1 << p.bits, clearing = p.clear ? 2 * sm_count() : 0;
   SCN_CUDA_TRY(launch_dependent(k_radix_count<ROUNDS>, dim3(p.tiles + clearing), dim3(THREADS), sizeof(unsigned) * digits, s, p));
   SCN_LAUNCH_CHECK("k_radix_count");
-  if (p.totals) SCN_CUDA_TRY(launch_dependent(k_radix_scan, dim3(digits / SCAN_DIGITS), dim3(SCAN_THREADS), 0, s, p));
+  const int each = (p.tiles + SCAN_RUNS - 1) / SCAN_RUNS;
+  const auto scan = each <= 2 ? k_radix_scan<2> : each <= 8 ? k_radix_scan<8> : each <= 24 ? k_radix_scan<24> : k_radix_scan<0>;
+  if (p.totals) SCN_CUDA_TRY(launch_dependent(scan, dim3(digits / SCAN_DIGITS), dim3(SCAN_THREADS), 0, s, p));
   if (p.totals) SCN_LAUNCH_CHECK("k_radix_scan");
   switch (p.bits) {
   case 6: SCN_CUDA_TRY(launch_dependent(k_radix_scatter<ROUNDS, 6>, dim3(p.tiles), dim3(THREADS), 0, s, p)); break;

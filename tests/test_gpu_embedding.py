@@ -315,3 +315,17 @@ def test_long_tokens(abi, n, starts, missing, C):
     want = torch.zeros(V, C, dtype=torch.float64, device="cuda").index_add_(0, tok[tok >= 0].long(), dout[tok >= 0].double())
     got = abi.embedding_backward(dout, tok, torch.full((V, C), 7.0, device="cuda"))
     assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("n", [4096 * 1024, 4096 * 1024 + 1, 4096 * 2048, 4096 * 2048 + 1, 20000003])
+def test_many_rows_of_one_value(abi, n):
+    """Sorts of thousands of tiles.  Whole numbers whose sums stay below 2^24: exact."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    tok = torch.randint(-5, 100000, (n,), device="cuda", generator=gen, dtype=torch.int32)
+    dout = torch.randint(-4, 5, (n, 1), device="cuda", generator=gen).to(torch.bfloat16)
+    want = torch.zeros(99990, 1, dtype=torch.float64, device="cuda")
+    ok = (tok >= 0) & (tok < 99990)
+    want.index_add_(0, tok[ok].long(), dout[ok].double())
+    errors = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = abi.embedding_backward(dout, tok, torch.empty(99990, 1, device="cuda"), errors=errors)
+    assert torch.equal(got.double(), want) and errors.item() != 0
