@@ -135,10 +135,17 @@ __device__ __forceinline__ float gradient_scale(const scn_adamw_scalars_t &h, co
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); } // of nothing that mul() gave
-// A sum that a product goes into, where both roundings count: one value at a time.  (A paired product and the paired sum behind it come
-// out as one fused operation, also where PTX names the rounding of each; the tests that count codes show it.)
-__device__ __forceinline__ float2 plus(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
-__device__ __forceinline__ float2 minus(float2 a, float2 b) { return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y)); }
+// A sum that a product goes into, where both roundings count.  (A paired product and the paired sum behind it come out as one fused
+// operation, also where PTX names the rounding of each; the tests that count codes show it.  So the sum is written as a fused operation
+// itself, a 1 + b with a 1 that only the launch knows: one rounding, and nothing left to fuse.  150 M values with decodes: 713 -> 708 us.  The 32-bit
+// step, which waits for memory, adds single values.)
+struct Ones {
+  float2 plus, minus; // 1 and -1
+};
+__device__ __forceinline__ float2 plus(const Ones &one, float2 a, float2 b) { return __ffma2_rn(a, one.plus, b); }
+struct Singly {};
+__device__ __forceinline__ float2 plus(Singly, float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 minus(const Ones &one, float2 a, float2 b) { return __ffma2_rn(b, one.minus, a); }
 __device__ __forceinline__ float root(float x) { // an ulp or so off; 0 below 2^-126
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -156,10 +163,10 @@ __device__ __forceinline__ float max_nan(float a, float b) { // a NaN stays one
 }
 // The moments.  Every operation is one rounding (no fused multiply-add), so that the 8-bit codes, which are compared
 // against these values, come out the same in any program that computes the formula in 32 bits.
-__device__ __forceinline__ void moments(const scn_adamw_scalars_t &h, float gs, float2 g, float2 &m, float2 &v) {
+template <class Sum> __device__ __forceinline__ void moments(const Sum &one, const scn_adamw_scalars_t &h, float gs, float2 g, float2 &m, float2 &v) {
   g = mul(g, both(gs));
-  m = plus(mul(m, both(h.beta1)), mul(g, both(h.one_minus_beta1)));
-  v = plus(mul(v, both(h.beta2)), mul(mul(g, g), both(h.one_minus_beta2)));
+  m = plus(one, mul(m, both(h.beta1)), mul(g, both(h.one_minus_beta1)));
+  v = plus(one, mul(v, both(h.beta2)), mul(mul(g, g), both(h.one_minus_beta2)));
 }
 // The parameter's step may use the hardware's approximate root and reciprocal (an ulp or two of 32 bits): unlike the states it
 // is compared with nothing.
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ Li
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
-        moments(h, gs, make_float2(g[k], g[k + 1]), m2, v2);
+        moments(Singly(), h, gs, make_float2(g[k], g[k + 1]), m2, v2);
         const float2 w2 = updated(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
         m[k] = m2.x; m[k + 1] = m2.y;
         v[k] = v2.x; v[k + 1] = v2.y;
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ Li
     for (int j = threadIdx.x; j < TURN && first + j < t.n; j += THREADS) {
       const long long i = first + j;
       float2 m = both(ms[i]), v = both(vs[i]);
-      moments(h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
+      moments(Singly(), h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
       const float w = updated(h, both(t.w[i]), m, v, t.decay, t.least).x;
       ms[i] = m.x; vs[i] = v.x; t.w[i] = w;
       if (t.w16) store_16(t.w16, t.w16type, i, w);
@@ -234,18 +241,18 @@ __device__ __forceinline__ float2 nearest(float2 r) { return add(add(r, both(838
 // whole number nearest to an approximate root is q or q + 1; which one, and what the dither decides, comes from differences
 // that are 0 or at least 2^-41 (u is no smaller than 2^-17), so a multiplication that saturates tells their signs.
 // (x - q^2 and 2 q + 1 are exact.)
-__device__ __forceinline__ float2 code_m(float2 x, float2 u) {
+__device__ __forceinline__ float2 code_m(const Ones &one, float2 x, float2 u) {
   float2 q = nearest(make_float2(root(x.x), root(x.y)));
-  q = minus(q, positive(__ffma2_rn(q, q, make_float2(-x.x, -x.y))));
+  q = minus(one, q, positive(__ffma2_rn(q, q, make_float2(-x.x, -x.y))));
   const float2 over = __ffma2_rn(q, make_float2(-q.x, -q.y), x), limit = mul(u, __ffma2_rn(q, both(2.f), both(1.f)));
-  return plus(q, positive(minus(over, limit)));
+  return plus(one, q, positive(minus(one, over, limit)));
 }
 __device__ __forceinline__ float2 fourth(float2 q) { q = mul(q, q); return mul(q, q); }
-__device__ __forceinline__ float2 code_v(float2 y, float2 u) {
+__device__ __forceinline__ float2 code_v(const Ones &one, float2 y, float2 u) {
   float2 q = nearest(make_float2(root(root(y.x)), root(root(y.y))));
-  q = minus(q, positive(minus(fourth(q), y)));
-  const float2 low = fourth(q), limit = mul(u, minus(fourth(add(q, both(1.f))), low));
-  return plus(q, positive(minus(minus(y, low), limit)));
+  q = minus(one, q, positive(minus(one, fourth(q), y)));
+  const float2 low = fourth(q), limit = mul(u, minus(one, fourth(add(q, both(1.f))), low));
+  return plus(one, q, positive(minus(one, minus(one, y, low), limit)));
 }
 // A 32-bit mix of a position and the seed: multiplications by odd numbers (the fractional bits of the square roots of 2, 3,
 // 5 and 7) between shifts that bring the high bits down.  Its two halves, the lower one with the upper one mixed in once more,
@@ -284,7 +291,7 @@ template <int K> __device__ __forceinline__ float2 decode_v(unsigned word, float
 constexpr unsigned NOT_FINITE = 0x7F800000u;
 // A block's share of everything, on its way to a warp while it works on the block before: the step issues instructions for
 // most of the time that its memory needs, so a warp cannot do without either.  150 M values with 16-bit gradients and a 16-bit
-// copy: 465 us, 5.2 TB/s of 16 bytes a value (79 % of a plain copy's rate; 81 % of the issue slots are taken).  Loads straight into
+// copy: 461 us, 5.2 TB/s of 16 bytes a value (79 % of a plain copy's rate; 81 % of the issue slots are taken).  Loads straight into
 // registers took 485 us with five CTAs an SM, 510 with four; the next block's loads into registers 515; one value in an
 // instruction 690; conversions and correctly rounded roots instead of the tricks below 2130.
 struct Incoming {
@@ -306,7 +313,7 @@ __device__ __forceinline__ void ask(const Tensor &t, long long block, int lane, 
   else copy_async<16>(in.v + (lane - 16) * 16, (const unsigned char *)t.v + i + (lane - 16) * 16);
 }
 template <int CAP>
-__global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
+__global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm, const Ones one) {
   __shared__ __align__(16) Incoming incoming[2][WARPS];
   const int own = owner(l, blockIdx.x);
   const Tensor &t = l.t[own];
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ 
     float topM = 0.f, topV = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      moments(h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
+      moments(one, h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
       const float2 to = updated(h, make_float2(w[2 * k], w[2 * k + 1]), m[k], v[k], t.decay, t.least);
       w[2 * k] = to.x; w[2 * k + 1] = to.y;
       if (!wide) { // (a NaN scale would reach the values behind the end)
@@ -395,8 +402,8 @@ __global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ 
       float2 um, uv;
       dither(at + 2 * k, key, um.x, uv.x);
       dither(at + 2 * k + 1, key, um.y, uv.y);
-      const float2 qm = code_m(make_float2(__fmul_rn(fabsf(m[k].x), im), __fmul_rn(fabsf(m[k].y), im)), add(um, both(DITHER)));
-      qv[k] = code_v(mul(v[k], both(iv)), add(uv, both(DITHER)));
+      const float2 qm = code_m(one, make_float2(__fmul_rn(fabsf(m[k].x), im), __fmul_rn(fabsf(m[k].y), im)), add(um, both(DITHER)));
+      qv[k] = code_v(one, mul(v[k], both(iv)), add(uv, both(DITHER)));
       product = mul(product, qv[k]);
       const float2 bytes = add(make_float2(copysignf(qm.x, m[k].x), copysignf(qm.y, m[k].y)), both(SIGNED)); // the bytes in the low bits again
       mb[2 * k] = __float_as_uint(bytes.x); mb[2 * k + 1] = __float_as_uint(bytes.y);
@@ -585,6 +592,7 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
     if (h->max_norm > 0 && !d_norm) return fail(SCN_ERR_INVALID, "AdamW: clipping needs the gradients' norm");
   }
   cudaStream_t s = (cudaStream_t)stream;
+  const Ones ones = {make_float2(1.f, 1.f), make_float2(-1.f, -1.f)};
   const auto eight = [](const scn_adamw_tensor_t &t) { return t.d_m_scale != nullptr; };
   int rc = for_lists(tensors, count, 1, [&](const scn_adamw_tensor_t &t) { return !eight(t); }, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_32<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
@@ -593,7 +601,7 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
   });
   if (rc != SCN_OK) return rc;
   return for_lists(tensors, count, 8, eight, [&](const auto &l) -> int {
-    SCN_CUDA_TRY(launch_dependent(k_adamw_8<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
+    SCN_CUDA_TRY(launch_dependent(k_adamw_8<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm, ones));
     SCN_LAUNCH_CHECK("k_adamw_8");
     return SCN_OK;
   });

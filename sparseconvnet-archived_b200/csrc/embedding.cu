@@ -139,7 +139,7 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
 // ------------------------------------------------------------------ stable radix sort of (token, row)
 // Digits of at most MAX_DIGIT bits, least significant first; per pass: digit counts of each tile, their running sums
 // over the tiles, and the scatter.  A tile is THREADS * ROUNDS consecutive entries, a warp of it 32 * ROUNDS consecutive ones.
-// 3.4 M rows, 18-bit keys: 83 us for both passes (counts 11 + 5, running sums 9 + 8, scatters 24 + 21, overlapped launches
+// 3.4 M rows, 18-bit keys: 75 us for both passes (counts 12 + 5, running sums 6 + 5, scatters 24 + 21, overlapped launches
 // included; the table's 33 MB of zeros are written beside the first counts).  It is bound by the latency of its short kernels
 // and the scatter by the instructions that rank entries within a warp; wider digits (10 bits) and larger tiles (15 rounds: 219 us for the
 // whole gradient, 8 rounds: 199, 4 rounds: 212) did not help.
