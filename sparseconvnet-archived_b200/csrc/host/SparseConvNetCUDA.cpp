@@ -220,7 +220,8 @@ void SparseConvNetCUDA::preprocessBatchOnDevice(SpatiallySparseBatch &batch) {
     cudaSafeCall(cudaStreamWaitEvent(memStream.stream, inputReady, 0));
     inputReady = nullptr;
   }
-  int *h = (int *)memStream.staging(sizeof(int) * (4 * nL + 1));
+  // (not in staging(): on a stream that holds other work the input's own upload from there has not run yet)
+  int *h = memStream.countsBack(4 * nL + 1);
   // The error word of the tensor-core kernels rides along with the counts: set by an earlier batch's kernels whose
   // results were never read through SoftmaxClassifier (the device-resident entry point), it is reported here.
   const int *tcWord = scn_conv_tc_error_word();
@@ -263,7 +264,7 @@ void SparseConvNetCUDA::preprocessBatchOnDevice(SpatiallySparseBatch &batch) {
     throw ScnException("a tensor-core kernel of an earlier batch gave up a time-limited wait (code " + std::to_string(code) +
                        "): that batch's results are not valid");
   }
-  std::vector<int> counts(h, h + 4 * nL); // staging is reused below
+  std::vector<int> counts(h, h + 4 * nL);
   if (hinted) { // a sample outgrew the shared-memory hint learnt from earlier batches: rebuild for the worst case
     bool overflow = false;
     for (int i = 0; i < nL; ++i) overflow = overflow || (layers[i]->changesGeometry && (counts[4 * i + 2] & SCN_DEV_ERR_CAPACITY));

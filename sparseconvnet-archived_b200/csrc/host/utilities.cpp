@@ -85,6 +85,7 @@ cudaMemStream::~cudaMemStream() {
   if (resultWords) cudaFree(resultWords);
   if (ownsStream && stream) cudaStreamDestroy(stream);
   if (pinnedMemory) cudaFreeHost(pinnedMemory);
+  if (countWords) cudaFreeHost(countWords);
 }
 void *cudaMemStream::deviceScratch(size_t bytes) {
   if (bytes > scratchBytes) {
@@ -126,6 +127,14 @@ void *cudaMemStream::staging(size_t bytes) {
     pinnedMemorySize = (int)want;
   }
   return pinnedMemory;
+}
+int *cudaMemStream::countsBack(size_t n) {
+  if (n > nCountWords) { // (idle: whoever used it has waited)
+    if (countWords) { cudaSafeCall(cudaFreeHost(countWords)); countWords = nullptr; nCountWords = 0; }
+    cudaSafeCall(cudaMallocHost((void **)&countWords, sizeof(int) * n));
+    nCountWords = n;
+  }
+  return countWords;
 }
 
 // utilities.cu:132-169.  file / linenumber name the caller in the error message.

@@ -63,6 +63,9 @@ public:
   explicit cudaMemStream(cudaStream_t external);
   ~cudaMemStream();
   void *staging(size_t bytes); // pinned buffer of at least `bytes`
+  // Pinned ints that the device's counts come back to while uploads out of staging() may still be queued: nothing is uploaded
+  // from here, and every use waits for its copy before it returns.
+  int *countsBack(size_t n);
   void *deviceScratch(size_t bytes); // device buffer of at least `bytes`; only work on `stream` may use it
   int *deviceResult();               // four device ints for a rule build whose counts nobody reads
   // Device block of the fused rule chain's resident build (scn_rules_chain_build_resident): nothing else writes it.
@@ -76,6 +79,8 @@ private:
   void *scratch = nullptr;
   size_t scratchBytes = 0;
   int *resultWords = nullptr;
+  int *countWords = nullptr;
+  size_t nCountWords = 0;
   void *chainBlock = nullptr;
   size_t chainBytes = 0;
   scn_chain_resident_t *chainResident = nullptr;

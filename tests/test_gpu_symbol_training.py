@@ -327,3 +327,48 @@ def test_dropped_features_stay(scn, abi, table, bits):
     dropped = np.setdiff1d(np.arange(64), kept)
     assert np.array_equal(W0[:, dropped], W1[:, dropped]) and np.array_equal(B0[dropped], B1[dropped])
     assert (W0[:, kept] != W1[:, kept]).mean() > 0.5
+
+
+@pytest.mark.parametrize("rows", ["many", "few"])
+@pytest.mark.parametrize("work", ["other kernels", "a forward pass of device arrays"])
+@pytest.mark.parametrize("call", ["forward_host_symbols", "forward_host", "train_batch_symbols", "train_batch"])
+def test_host_arrays_on_a_busy_stream(scn, abi, table, rows, work, call):
+    """Calls from pageable arrays while the stream still holds work that was there before, so that their uploads wait in the queue:
+    the results of the same call on an idle stream, bit for bit.  few: fewer rows than there are words in the layers' counts."""
+    net = build(scn, abi, abi.VLEAKYRELU)
+    net.set_symbols(table, 1.5)
+    S = net.inputSpatialSize
+    if rows == "many":
+        keys, off, syms, labels = batch(S, 2)
+    else:
+        k = np.arange(3, S * S, S * S // 9)[:8]
+        keys, off = np.concatenate([[-1], k[:4], [-1], k[4:]]).astype(np.int32), np.array([0, 5, 10], np.int32)
+        syms, labels = np.array([-1, 5, 6, 7, 8, -1, 9, 10, 11, 12], np.int32), np.array([1, 2], np.int32)
+        assert len(keys) < 4 * len(net.layers())
+    values = syms if call.endswith("symbols") else features_of(table, syms, 1.5)
+
+    def run():
+        if call.startswith("forward"):
+            return getattr(net, call)(keys, off, values)
+        probs, stats = getattr(net, call)(keys, off, values, labels, 0.0, 0.0)  # rate 0: the weights stay as they are
+        return probs, np.array([stats["nll"], stats["mistakes"]])
+
+    big = batch(S, 9, samples=400)
+    device = [torch.from_numpy(x).cuda() for x in (big[0], big[1], big[1][:-1], features_of(table, big[2], 1.5))]  # a sample's background row is its first
+    a, out = torch.ones(8192, 8192, device="cuda", dtype=torch.bfloat16), torch.empty(8192, 8192, device="cuda", dtype=torch.bfloat16)
+
+    def other_work(times):
+        for _ in range(times):
+            if work == "other kernels":
+                torch.matmul(a, a, out=out)
+            else:
+                net.forward_device(*device, max_sites=int(np.diff(big[1]).max()) - 1)
+
+    other_work(1)
+    run()  # (memory is allocated: nothing below waits for the GPU but the call itself)
+    torch.cuda.synchronize()
+    want = run()
+    other_work(60 if work == "other kernels" else 3)
+    got = run()
+    assert all(np.array_equal(x, y) for x, y in zip(got, want))
+    assert abi.conv_tc_take_error() == 0
