@@ -9,6 +9,7 @@ SymbolTable::SymbolTable(cudaMemStream &memStream, int nSymbols, int nFeatures, 
 void SymbolTable::forwards(SpatiallySparseBatchInterface &input) {
   const int rows = input.nSpatialSites;
   if ((int)input.symbols.size() != rows || input.nFeatures != nFeatures) throw ScnException("SymbolTable: one symbol per input row is needed");
+  if ((long long)rows * nFeatures > 0x7fffffffll) throw ScnException("SymbolTable: more than 2^31 features in one batch; use smaller batches");
   input.sub->features.copyToGPU();
   input.sub->features.resize(rows * nFeatures);
   scnSafeCall(scn_embedding_forward(table.dPtr(), SCN_F32, nSymbols, nFeatures, input.symbols.dPtr(), rows, scale, input.sub->features.dPtr(), SCN_F32,

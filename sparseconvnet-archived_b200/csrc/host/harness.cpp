@@ -116,6 +116,11 @@ void adoptDeviceInput(SparseConvNetCUDA &cnn, SpatiallySparseBatch &b, int batch
   in.backgroundRows.borrowDevice(const_cast<int *>(d_bg), batch);
   in.sub->features.borrowDevice(const_cast<float *>(d_features), rows * cnn.nInputFeatures);
 }
+// A batch's features are counted in 32 bits (a symbol or a key stands for nFeatures of them: few host bytes reach past that).
+void checkFeatureCount(int rows, int nFeatures) {
+  if (rows < 0) throw ScnException("the samples' offsets must not be negative");
+  if ((long long)rows * nFeatures > 0x7fffffffll) throw ScnException("more than 2^31 input features in one batch; use smaller batches");
+}
 // Interface 0 of the network's first pool slot filled from host arrays (pinned ones are copied from where they lie,
 // pageable ones through the stream's staging block); the features travel on a stream of their own.  symbols: one code a row
 // instead of features; the network's table turns them into features behind their copy.
@@ -123,6 +128,7 @@ SpatiallySparseBatch &uploadHostInput(scn_net *net, int batch, const int *keys, 
                                       const int *symbols = nullptr) {
   SparseConvNetCUDA &cnn = *net->cnn;
   if (batch < 1) throw ScnException("batch must be positive");
+  checkFeatureCount(off[batch], cnn.nInputFeatures);
   if (symbols) {
     if (!cnn.symbolTable) throw ScnException("no symbol table (scn_net_set_symbols)");
     for (int r = 0; r < off[batch]; ++r)
@@ -395,6 +401,7 @@ int scn_net_forward_host_begin(scn_net_t *net, int batch, const int *keys, const
     if (net->upCount == 2) throw ScnException("two batches are on their way already: take one with scn_net_forward_host_end first");
     scn_net::HostUpload &u = net->up[net->upHead];
     const int rows = off[batch], nF = cnn.nInputFeatures;
+    checkFeatureCount(rows, nF);
     int maxRows = 0;
     for (int s = 0; s < batch; ++s) maxRows = std::max(maxRows, off[s + 1] - off[s]);
     if (!cnn.layers.empty() && dynamic_cast<TerminalPoolingLayer *>(cnn.layers[0])) { // its rule width needs the exact count

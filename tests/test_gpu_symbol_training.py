@@ -372,3 +372,19 @@ def test_host_arrays_on_a_busy_stream(scn, abi, table, rows, work, call):
     got = run()
     assert all(np.array_equal(x, y) for x, y in zip(got, want))
     assert abi.conv_tc_take_error() == 0
+
+
+def test_batches_of_too_many_features(scn, abi):
+    """2^16 + 1 rows of 2^16 features: the count of the features, 2^32 + 2^16, would be 2^16 in 32 bits."""
+    wide, rows = 1 << 16, (1 << 16) + 1
+    net = scn.net.Net(2, wide, N_CLASSES, 1, 0)
+    net.addLeNetLayerMP(4, 1, 1, 2, 2, abi.VLEAKYRELU, 0.0, 1)
+    net.addSoftmaxLayer()
+    net.set_precision(abi.PREC_FP32)  # (no layer of 2^16 inputs has a tensor-core path)
+    net.set_symbols(np.ones((1, wide), np.float32))
+    keys, off, syms = np.arange(rows, dtype=np.int32), np.array([0, rows], np.int32), np.zeros(rows, np.int32)
+    for bad in [lambda: net.forward_host_symbols(keys, off, syms), lambda: net.train_batch_symbols(keys, off, syms, [0], 0.1)]:
+        with pytest.raises(abi.ScnError, match="smaller batches"):
+            bad()
+    probs, _ = net.forward_host_symbols(keys[:1], [0, 1], syms[:1])
+    assert np.isfinite(probs).all()
