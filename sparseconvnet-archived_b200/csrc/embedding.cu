@@ -608,8 +608,8 @@ __global__ void __launch_bounds__(THREADS) k_embedding_backward_small(const Sums
     for (int i = threadIdx.x; i < (rows + 31) / 32; i += THREADS) sh.present[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.n; i += THREADS) {
-      const int t = tokens[i] - first;
-      if (tokens[i] >= first && t < rows) atomicOr(&sh.present[t >> 5], 1u << (t & 31));
+      const int t = tokens[i];
+      if (t >= first && t - first < rows) atomicOr(&sh.present[(t - first) >> 5], 1u << ((t - first) & 31));
     }
     __syncthreads();
     for (int r = warp; r < rows; r += WARPS)
@@ -884,7 +884,8 @@ extern "C" int scn_embedding_backward(const int *d_tokens, long long n, const vo
     else SCN_CUDA_TRY(launch_dependent(F(T, 1, 4), __VA_ARGS__));                                                     \
   })
   if (n <= SMALL) {
-    const int range = std::max(32, std::min(MOST_RANGE, (vocab + 4 * sm_count() - 1) / (4 * sm_count()))), clearing = accumulate ? 0 : (vocab + range - 1) / range;
+    const long long share = (vocab - 1ll) / (4 * sm_count()) + 1; // (in 64 bits: vocab goes up to 2^31 - 1)
+    const int range = (int)std::max(32ll, std::min((long long)MOST_RANGE, share)), clearing = accumulate ? 0 : (int)((vocab - 1ll) / range + 1);
 #define SCN_SMALL(T, W, J) (k_embedding_backward_small<T, W, J>)
     SCN_SUMS(SCN_SMALL, dim3(1 + clearing, slabs), dim3(THREADS), 0, s, q, (const T *)d_dout, d_tokens, sp.bits, range, d_errors);
     SCN_LAUNCH_CHECK("k_embedding_backward_small");

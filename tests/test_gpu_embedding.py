@@ -329,3 +329,19 @@ def test_many_rows_of_one_value(abi, n):
     errors = torch.zeros(1, dtype=torch.int32, device="cuda")
     got = abi.embedding_backward(dout, tok, torch.empty(99990, 1, device="cuda"), errors=errors)
     assert torch.equal(got.double(), want) and errors.item() != 0
+
+
+@pytest.mark.parametrize("n", [5, 1024, 1025])
+@pytest.mark.parametrize("V", [2147467264, 2147467265, 2147483647])
+def test_gradient_of_the_largest_vocabularies(abi, n, V):
+    """As many tokens as 32 bits count, or nearly: few rows are summed in one launch that divides the table among its CTAs, more by the sort."""
+    tok = torch.randint(0, V, (n,), device="cuda", dtype=torch.int64).int()
+    tok[0], tok[1], tok[2], tok[3], tok[4] = V - 1, 0, -2147483648, V - 1, -1
+    dout = torch.randint(1, 5, (n, 1), device="cuda").float()
+    ok = tok >= 0
+    at, where = torch.unique(tok[ok], return_inverse=True)
+    want = torch.zeros(len(at), device="cuda").index_add_(0, where, dout[ok, 0])  # whole numbers: exact
+    dt = abi.embedding_backward(dout, tok, torch.full((V, 1), math.nan, device="cuda"))
+    assert torch.equal(dt[at.long(), 0], want) and dt.count_nonzero().item() == len(at)
+    abi.embedding_backward(dout, tok, dt, accumulate=True)
+    assert torch.equal(dt[at.long(), 0], 2 * want) and dt.count_nonzero().item() == len(at)
