@@ -123,13 +123,15 @@ __global__ void __launch_bounds__(FINISH) k_grad_norm_finish(const double *parti
 }
 
 // ------------------------------------------------------------------ step
-// What scales the gradients, or NaN if the norm is not finite: then nothing is changed.
+// What scales the gradients, or NaN if the norm is not finite: then nothing is changed.  Clipped it is grad_scale max_norm / (norm
+// |grad_scale|), whose factors can leave 32 bits where the result does not: then it is taken as max_norm / norm with grad_scale's sign.
 __device__ __forceinline__ float gradient_scale(const scn_adamw_scalars_t &h, const float *norm) {
   if (!norm) return h.grad_scale;
+  if (!isfinite(*norm)) return __int_as_float(0x7fffffff);
   const float total = *norm * fabsf(h.grad_scale);
-  if (!(total <= 3.402823466e38f)) return __int_as_float(0x7fffffff);
-  const float clip = h.max_norm > 0.f && total > h.max_norm ? __fdiv_rn(h.max_norm, total) : 1.f;
-  return __fmul_rn(h.grad_scale, clip);
+  if (!(h.max_norm > 0.f && total > h.max_norm)) return h.grad_scale;
+  const float clip = __fdiv_rn(h.max_norm, total);
+  return clip >= 0x1p-126f ? __fmul_rn(h.grad_scale, clip) : copysignf(__fdiv_rn(h.max_norm, *norm), h.grad_scale);
 }
 // Two values in one instruction each, as far as there is one: the 8-bit step is bound by the instructions it issues.
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }

@@ -535,3 +535,38 @@ def test_numbers_after_a_refused_step(abi):
         opt.step(0.1, 1)
         return w
     assert torch.equal(run(False), run(True))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size,gs,max_norm", [
+    (1e20, 5e18, 0.0), (1e30, 1e10, 1e-3), (1e30, -1e10, 1e-3), (1e8, 1e30, 1e-7), (1e-30, 1e38, 1.0), (1e15, 1e-30, 1.0), (1e37, 1.0, 1e-2)])
+def test_finite_norms_that_grad_scale_takes_out_of_32_bits(abi, bits, size, gs, max_norm):
+    """norm |grad_scale|, or max_norm over it, leaves 32 bits or all but does: the step is taken, with the gradients' norm scaled to
+    max_norm.  Only a norm that is itself not finite stops it."""
+    rng = np.random.default_rng(17)
+    n = 3000
+    x = rng.standard_normal(n)
+    g = torch.from_numpy((x / np.sqrt((x ** 2).sum()) * size).astype(f32)).cuda()
+    t = dict(w=torch.zeros(n, device="cuda"), g=g, **abi.adamw_states(n, "cuda", bits))
+    opt = abi.AdamW([t])
+    norm = opt.grad_norm()
+    assert math.isfinite(norm.item()) and abs(norm.item() / size - 1) < 1e-3
+    gs, max_norm = float(f32(gs)), float(f32(max_norm))
+    clipped = max_norm > 0 and norm.item() * abs(gs) > max_norm
+    scaled = g.double() * (math.copysign(max_norm / norm.item(), gs) if clipped else gs)
+    # the scale: three roundings (a product, a quotient, a product), or 2^-150 where it lies below the normal range; then the gradient's
+    # product (beta1 = 1/2 is exact)
+    err = 4.1 * U * scaled.abs() + g.double().abs() * 2.0 ** -150 + 2.0 ** -149
+    opt.step(1e-3, 1, beta1=0.5, beta2=0.0, grad_scale=gs, norm=norm, max_norm=max_norm)
+    m = 0.5 * scaled
+    if bits == 32:
+        assert ((t["m"].double() - m).abs() <= err).all()
+    elif max_norm == 0:  # squares past 32 bits: no code stands for them
+        assert t["m_scale"].isnan().all() and t["v_scale"].isnan().all()
+    else:  # a code that stands for at least a quarter of its block's largest value is at least 45: within a step of (2 q + 1) / q^2 < 0.05
+        got, large = abi.adamw_decode(t["m"], t["m_scale"]).double(), m.abs() > 0.25 * m.abs().max()
+        assert ((got - m).abs() <= 0.05 * m.abs())[large].all()
+    if max_norm > 0:  # beta2 = 0: v = g'^2, and the bias corrections leave g' / (|g'| + eps); roundings behind g' as in check_step, below 20 U
+        eps = float(f32(EPS))
+        hat = scaled / (scaled.abs() + eps)
+        assert ((t["w"].double() + float(f32(1e-3)) * hat).abs() <= 1e-3 * (24 * U * hat.abs() + err / (scaled.abs() + eps)) + 1e-44).all()
