@@ -25,7 +25,7 @@ struct Tensor {
   unsigned long long block; // blocks of BLOCK values in front of this tensor in the call's whole list
   float decay, least;
   short gtype, w16type;
-  int wide;            // every array is aligned for eight values at once
+  int wide;            // every array that the launch touches is aligned for eight values at once
 };
 template <int CAP> struct List {
   static constexpr int capacity = CAP;
@@ -488,13 +488,14 @@ const char *wrong_list(const scn_adamw_tensor_t *t, int count, bool step) {
     if ((uintptr_t)t[i].d_g & (type_bytes(t[i].g_type) - 1)) return "AdamW: misaligned pointer";
   return nullptr;
 }
-bool wide(const scn_adamw_tensor_t &t) {
+bool wide_gradient(const scn_adamw_tensor_t &t) { return !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)); }
+bool wide_step(const scn_adamw_tensor_t &t) {
   const uintptr_t states = (uintptr_t)t.d_m | (uintptr_t)t.d_v;
-  return !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_g & (8 * type_bytes(t.g_type) - 1)) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 15 : 31));
+  return wide_gradient(t) && !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 15 : 31));
 }
 // launch(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.  Where one turn a
 // chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes `most`: it finds its tensor once for all of them.
-template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Launch launch) {
+template <int CAP, class Take, class Wide, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Wide wide, Launch launch) {
   List<CAP> l;
   long long all = 0;
   for (int i = 0; i < count; ++i) all += take(t[i]) ? (t[i].n + TURN - 1) / TURN : 0;
@@ -520,10 +521,10 @@ template <int CAP, class Take, class Launch> int for_lists(const scn_adamw_tenso
   return l.count ? launch(l) : (int)SCN_OK;
 }
 // The parameters' bytes are copied at every launch: the smallest list that holds them all.
-template <class Take, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Launch launch) {
-  if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, most, take, launch);
-  if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, most, take, launch);
-  return for_lists<CAP_LARGE>(t, count, most, take, launch);
+template <class Take, class Wide, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Wide wide, Launch launch) {
+  if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, most, take, wide, launch);
+  if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, most, take, wide, launch);
+  return for_lists<CAP_LARGE>(t, count, most, take, wide, launch);
 }
 
 } // namespace
@@ -569,7 +570,7 @@ extern "C" int scn_grad_norm(const scn_adamw_tensor_t *tensors, int count, float
   int used = 0, launches = (count + CAP_LARGE - 1) / CAP_LARGE;
   if (launches > most) return fail(SCN_ERR_UNSUPPORTED, "AdamW: list too long");
   const int each = most / std::max(launches, 1); // a CTA a chunk as far as there are places for their sums
-  const int rc = for_lists(tensors, count, 4, [](const scn_adamw_tensor_t &) { return true; }, [&](const auto &l) -> int {
+  const int rc = for_lists(tensors, count, 4, [](const scn_adamw_tensor_t &) { return true; }, wide_gradient, [&](const auto &l) -> int {
     const int grid = std::min(l.chunks, each);
     SCN_CUDA_TRY(launch_dependent(k_grad_norm_partial<std::decay_t<decltype(l)>::capacity>, dim3(grid), dim3(THREADS), 0, s, l, partial + used));
     SCN_LAUNCH_CHECK("k_grad_norm_partial");
@@ -596,13 +597,13 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor_t *tensors, int count, cons
   cudaStream_t s = (cudaStream_t)stream;
   const Ones ones = {make_float2(1.f, 1.f), make_float2(-1.f, -1.f)};
   const auto eight = [](const scn_adamw_tensor_t &t) { return t.d_m_scale != nullptr; };
-  int rc = for_lists(tensors, count, 1, [&](const scn_adamw_tensor_t &t) { return !eight(t); }, [&](const auto &l) -> int {
+  int rc = for_lists(tensors, count, 1, [&](const scn_adamw_tensor_t &t) { return !eight(t); }, wide_step, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_32<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm));
     SCN_LAUNCH_CHECK("k_adamw_32");
     return SCN_OK;
   });
   if (rc != SCN_OK) return rc;
-  return for_lists(tensors, count, 8, eight, [&](const auto &l) -> int {
+  return for_lists(tensors, count, 8, eight, wide_step, [&](const auto &l) -> int {
     SCN_CUDA_TRY(launch_dependent(k_adamw_8<std::decay_t<decltype(l)>::capacity>, dim3(l.chunks), dim3(THREADS), 0, s, l, scalars, d_scalars, d_norm, ones));
     SCN_LAUNCH_CHECK("k_adamw_8");
     return SCN_OK;

@@ -570,3 +570,20 @@ def test_finite_norms_that_grad_scale_takes_out_of_32_bits(abi, bits, size, gs, 
         eps = float(f32(EPS))
         hat = scaled / (scaled.abs() + eps)
         assert ((t["w"].double() + float(f32(1e-3)) * hat).abs() <= 1e-3 * (24 * U * hat.abs() + err / (scaled.abs() + eps)) + 1e-44).all()
+
+
+def test_norm_depends_on_the_gradients_alone(abi):
+    """The norm reads d_g, g_type and n: whatever else an entry holds, the squares are added in the same order.  The values make another
+    order show: 1 + 2 (2^-12)^2 + (2^-24)^2 is (1 + 2^-24)^2, whose root lies halfway between two numbers of 32 bits; seven squares of
+    0.99 2^-53 vanish one by one beside the 1, but tip the balance once two of them are added up first."""
+    n = 2048
+    g = torch.zeros(n, device="cuda")
+    g[0], g[1:8], g[8:10], g[16] = 1.0, math.sqrt(0.99) * 2.0 ** -26.5, 2.0 ** -12, 2.0 ** -24
+    L, s = abi.lib(), torch.cuda.current_stream().cuda_stream
+    norm, ws = torch.empty(1, device="cuda"), torch.empty(L.scn_grad_norm_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    results = set()
+    for other in (dict(), dict(d_w=4), dict(d_m=1, d_v=3), dict(d_m_scale=4), dict(d_w16=2), dict(d_w=1, d_m=7, w16_type=9, weight_decay=math.nan)):
+        e = abi.AdamWTensor(d_g=g.data_ptr(), n=n, g_type=abi.F32, **other)  # (none of the other pointers is read)
+        abi.check(L.scn_grad_norm((abi.AdamWTensor * 1)(e), 1, norm.data_ptr(), ws.data_ptr(), ws.numel(), s))
+        results.add(norm.item())
+    assert len(results) == 1 and abs(results.pop() - 1) <= 2.0 ** -23
