@@ -377,6 +377,10 @@ void SparseConvNetCUDA::useSymbols(int nSymbols, float scale, const float *value
 }
 // Every layer's backwards in reverse order, then, where they leave it, the update.
 void SparseConvNetCUDA::learn(SpatiallySparseBatch &batch, float learningRate, float momentum) {
+  SpatiallySparseBatchInterface &in = batch.interfaces[0];
+  const bool symbols = symbolTable && in.symbols.size() > 0;
+  if (symbols && !in.backpropErrors) // (before any layer has learnt)
+    throw ScnException("a TRAINBATCH of symbols needs its input's gradient: set interfaces[0].backpropErrors before preprocessing");
   struct Deferring { // (a layer's backwards() called by itself still updates that layer)
     std::vector<SpatiallySparseLayer *> &layers;
     Deferring(std::vector<SpatiallySparseLayer *> &layers, bool on) : layers(layers) { set(on); }
@@ -387,8 +391,6 @@ void SparseConvNetCUDA::learn(SpatiallySparseBatch &batch, float learningRate, f
     }
   } deferring(layers, adamW != nullptr);
   for (int i = (int)layers.size() - 1; i >= 0; --i) layers[i]->backwards(batch, batch.interfaces[i], batch.interfaces[i + 1], learningRate, momentum);
-  SpatiallySparseBatchInterface &in = batch.interfaces[0];
-  const bool symbols = symbolTable && in.symbols.size() > 0;
   if (symbols) symbolTable->backwards(in);
   if (adamW) {
     std::vector<LearntParameter> list;

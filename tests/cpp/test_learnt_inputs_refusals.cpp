@@ -47,6 +47,20 @@ static SpatiallySparseBatch &fill(SparseConvNetCUDA &cnn, batchType type, bool e
   return b;
 }
 
+static std::vector<float> values(SparseConvNetCUDA &cnn, vectorCUDA<float> &v) {
+  cudaStreamSynchronize(cnn.memStream.stream);
+  std::vector<float> copy = v.hVector();
+  v.copyToGPU();
+  return copy;
+}
+// Everything that the network has learnt.
+static std::vector<std::vector<float>> learnt(SparseConvNetCUDA &cnn) {
+  std::vector<std::vector<float>> all = {values(cnn, cnn.symbolTable->table)};
+  for (auto l : cnn.layers)
+    if (auto n = dynamic_cast<NetworkInNetworkLayer *>(l)) { all.push_back(values(cnn, n->W)); all.push_back(values(cnn, n->B)); }
+  return all;
+}
+
 int main() {
   try {
     SparseConvNet net(2, nF, nClasses);
@@ -74,6 +88,23 @@ int main() {
       cnn.symbolTable->forwards(in);
       std::printf("OK too many features\n");
     }
+
+    // a training batch that forgot to ask for its input's gradient is refused before anything learns, under either optimiser, also where
+    // the gradient of an earlier batch is still there
+    std::ofstream nof, nog;
+    for (int optimiser = 0; optimiser < 2; ++optimiser) {
+      if (optimiser) cnn.useAdamW();
+      for (int times = 0; times < 2; ++times) {
+        const auto before = learnt(cnn);
+        bool refused = false;
+        try { cnn.processBatch(fill(cnn, TRAINBATCH, false), 0.01f, 0.f, nof, nog); } catch (const std::exception &e) { refused = true; }
+        CHECK(refused && learnt(cnn) == before && (!optimiser || cnn.adamW->step == times));
+        cnn.processBatch(fill(cnn, TRAINBATCH, true), 0.01f, 0.f, nof, nog);
+        const auto after = learnt(cnn);
+        for (size_t i = 0; i < after.size(); ++i) CHECK(after[i] != before[i]);
+      }
+    }
+    std::printf("OK no gradient\n");
   } catch (const std::exception &e) {
     std::printf("FAILED with exception: %s\n", e.what());
     return 1;
