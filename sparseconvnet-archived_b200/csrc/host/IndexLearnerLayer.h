@@ -22,6 +22,7 @@ public:
                  float momentum);
   void loadWeightsFromStream(std::ifstream &f, bool momentum);
   void putWeightsToStream(std::ofstream &f, bool momentum);
+  size_t weightFileBytes(bool momentum) override;
   int calculateInputSpatialSize(int outputSpatialSize);
   long long enqueueRules(SpatiallySparseBatch &batch, SpatiallySparseBatchInterface &input, SpatiallySparseBatchInterface &output,
                          long long rowsInBound, int *d_result);

@@ -676,6 +676,7 @@ void NetworkInNetworkLayer::putWeightsToStream(std::ofstream &f, bool momentum) 
   if (wOn) W.copyToGPU();
   if (bOn) B.copyToGPU();
 }
+size_t NetworkInNetworkLayer::weightFileBytes(bool momentum) { return sizeof(float) * ((size_t)W.size() + B.size()) * (momentum ? 2 : 1); }
 int NetworkInNetworkLayer::calculateInputSpatialSize(int outputSpatialSize) { return outputSpatialSize; }
 void replicateArray(float *src, float *dst, int nRows, int nColumns, cudaMemStream &memStream) {
   for (int r = 0; r < nRows; ++r)
@@ -704,6 +705,9 @@ void NetworkInNetworkPReLULayer::putWeightsToStream(std::ofstream &f, bool momen
   f.write((char *)b.data(), sizeof(float) * b.size());
   f.write((char *)s.data(), sizeof(float) * s.size());
   if (momentum) { std::vector<float> z(w.size() + b.size() + s.size(), 0.f); f.write((char *)z.data(), sizeof(float) * z.size()); }
+}
+size_t NetworkInNetworkPReLULayer::weightFileBytes(bool momentum) {
+  return NetworkInNetworkLayer::weightFileBytes(momentum) + sizeof(float) * PReLU.size() * (momentum ? 2 : 1);
 }
 
 // ------------------------------------------------------------------ applySigmoid / SoftmaxClassifier
@@ -1086,6 +1090,7 @@ void IndexLearnerLayer::putWeightsToStream(std::ofstream &f, bool) {
   f.write((char *)h.data(), sizeof(float) * h.size());
   if (on) W.copyToGPU();
 }
+size_t IndexLearnerLayer::weightFileBytes(bool) { return sizeof(float) * W.size(); }
 int IndexLearnerLayer::calculateInputSpatialSize(int outputSpatialSize) { return outputSpatialSize; }
 
 void IndexLearner(SpatiallySparseBatchInterface &input, SpatiallySparseBatch &batch, int nTop, cudaMemStream &memStream) {

@@ -12,6 +12,7 @@ public:
                              float dropout = 0, float alpha = 1);
   void loadWeightsFromStream(std::ifstream &f, bool momentum);
   void putWeightsToStream(std::ofstream &f, bool momentum);
+  size_t weightFileBytes(bool momentum) override;
   void learntParameters(std::vector<LearntParameter> &list) override;
 
 protected:

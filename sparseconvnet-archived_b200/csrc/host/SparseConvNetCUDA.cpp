@@ -617,9 +617,17 @@ void SparseConvNetCUDA::loadWeights(std::string baseName, int epoch, bool moment
   std::ifstream f(filename.c_str(), std::ios::in | std::ios::binary);
   if (!f) throw ScnException("Cannot find " + filename);
   std::cout << "Loading network parameters from " << filename << std::endl;
+  const bool withTable = symbolTable && firstNlayers >= (int)layers.size();
+  if (withTable) { // a file without the table is refused before any layer has taken its part
+    size_t need = sizeof(float) * (inputNormalizingConstants.size() + (size_t)symbolTable->table.size());
+    for (auto l : layers) need += l->weightFileBytes(momentum);
+    f.seekg(0, std::ios::end);
+    if (!f || (size_t)f.tellg() < need) throw ScnException("weight file ends early (a network of symbols needs its table's values behind everything else)");
+    f.seekg(0, std::ios::beg);
+  }
   for (int i = 0; i < std::min((int)layers.size(), firstNlayers); ++i) layers[i]->loadWeightsFromStream(f, momentum);
   if (!inputNormalizingConstants.empty()) f.read((char *)inputNormalizingConstants.data(), sizeof(float) * inputNormalizingConstants.size());
-  if (symbolTable && firstNlayers >= (int)layers.size()) {
+  if (withTable) {
     std::vector<float> &h = symbolTable->table.hVector();
     f.read((char *)h.data(), sizeof(float) * h.size());
     if (!f) throw ScnException("weight file ends early");

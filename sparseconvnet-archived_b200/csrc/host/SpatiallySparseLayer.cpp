@@ -11,4 +11,5 @@ void SpatiallySparseLayer::putWeightsToStream(std::ofstream &, bool) {}
 long long SpatiallySparseLayer::enqueueRules(SpatiallySparseBatch &, SpatiallySparseBatchInterface &, SpatiallySparseBatchInterface &,
                                              long long rowsInBound, int *) { return rowsInBound; }
 void SpatiallySparseLayer::finishRules(SpatiallySparseBatch &, SpatiallySparseBatchInterface &, SpatiallySparseBatchInterface &, const int *) {}
+size_t SpatiallySparseLayer::weightFileBytes(bool) { return 0; }
 void SpatiallySparseLayer::learntParameters(std::vector<LearntParameter> &) {}

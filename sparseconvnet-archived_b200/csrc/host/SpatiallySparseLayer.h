@@ -37,6 +37,8 @@ public:
   virtual void finishRules(SpatiallySparseBatch &batch, SpatiallySparseBatchInterface &input,
                            SpatiallySparseBatchInterface &output, const int *h_result);
   bool changesGeometry;
+  // Bytes of a weight file that loadWeightsFromStream() takes.
+  virtual size_t weightFileBytes(bool momentum);
   // The tensors that backwards() finds gradients for, for an optimiser over all layers (none: nothing to learn, or the layer
   // updates itself, as the index learner does).
   virtual void learntParameters(std::vector<LearntParameter> &list);

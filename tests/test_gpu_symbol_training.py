@@ -388,3 +388,28 @@ def test_batches_of_too_many_features(scn, abi):
             bad()
     probs, _ = net.forward_host_symbols(keys[:1], [0, 1], syms[:1])
     assert np.isfinite(probs).all()
+
+
+@pytest.mark.parametrize("act", ["VLEAKYRELU", "PRELU"])
+def test_weight_files_without_the_table(scn, abi, table, tmp_path, act):
+    """Such a file, or one that a byte has been cut off, is refused by a network of symbols before it changes anything."""
+    act = getattr(abi, act)
+    plain, net = build(scn, abi, act), build(scn, abi, act)
+    learnt = [i for i, L in enumerate(plain.layers()) if L["type"] == 2]
+    for i in learnt:
+        plain.set_weights(i, *[None if x is None else x + np.float32(1) for x in plain.get_weights(i)])
+    plain.save_weights(str(tmp_path / "w"), 1)
+    plain.set_symbols(table + np.float32(1))
+    plain.save_weights(str(tmp_path / "w"), 2)
+    whole = (tmp_path / "w_epoch-2.cnn").read_bytes()
+    (tmp_path / "w_epoch-3.cnn").write_bytes(whole[:-1])
+    net.set_symbols(table)
+    before = [net.get_weights(i) for i in learnt]
+    for epoch in (1, 3):
+        with pytest.raises(abi.ScnError, match="ends early"):
+            net.load_weights(str(tmp_path / "w"), epoch)
+        assert all(x is None or np.array_equal(x, y) for a, b in zip(before, learnt) for x, y in zip(a, net.get_weights(b)))
+        assert np.array_equal(net.get_symbols(), table)
+    net.load_weights(str(tmp_path / "w"), 2)
+    assert all(x is None or np.array_equal(x, y) for i in learnt for x, y in zip(plain.get_weights(i), net.get_weights(i)))
+    assert np.array_equal(net.get_symbols(), table + np.float32(1))
