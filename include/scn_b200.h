@@ -478,7 +478,7 @@ int scn_embedding_backward(const int *d_tokens, long long n, const void *d_dout,
  *     m  = beta1 m + (1 - beta1) g'
  *     v  = beta2 v + (1 - beta2) g' g'
  *     w  = max(w_min, w - lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay w))
- * in 32 bits; w_min = -INFINITY: no bound.  The root of a v below 2^-126 (gradients around 1e-18 and less) counts as 0. */
+ * in 32 bits; w_min = -INFINITY: no bound. */
 #define SCN_ADAMW_MAX_TENSORS 320
 #define SCN_ADAMW_BLOCK 256
 

@@ -153,6 +153,7 @@ __device__ __forceinline__ float root(float x) { // an ulp or so off; 0 below 2^
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float any_root(float x) { return x < 0x1p-64f ? root(x * 0x1p64f) * 0x1p-32f : root(x); } // below 2^-126 too
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -172,8 +173,13 @@ template <class Sum> __device__ __forceinline__ void moments(const Sum &one, con
 }
 // The parameter's step may use the hardware's approximate root and reciprocal (an ulp or two of 32 bits): unlike the states it
 // is compared with nothing.
-__device__ __forceinline__ float2 updated(const scn_adamw_scalars_t &h, float2 w, float2 m, float2 v, float decay, float least) {
-  const float2 den = __ffma2_rn(make_float2(root(v.x), root(v.y)), both(h.bias2), both(h.eps));
+// That root is 0 for v below 2^-126.  exact_roots: whether eps is so small beside 2^-63 bias2, the largest root lost, that it would
+// show; the values then take any_root.  (Asked once for eight values.  150 M values with 8-bit moments and decodes take 716 us with the
+// question, 713 without; 32-bit moments wait for memory and take no longer.)
+__device__ __forceinline__ bool exact_roots(const scn_adamw_scalars_t &h) { return !(h.eps >= 0x1p-39f * h.bias2); }
+template <bool EXACT> __device__ __forceinline__ float2 updated(const scn_adamw_scalars_t &h, float2 w, float2 m, float2 v, float decay, float least) {
+  const float2 r = EXACT ? make_float2(any_root(v.x), any_root(v.y)) : make_float2(root(v.x), root(v.y));
+  const float2 den = __ffma2_rn(r, both(h.bias2), both(h.eps));
   const float2 hat = mul(mul(m, both(h.bias1)), make_float2(reciprocal(den.x), reciprocal(den.y)));
   w = __ffma2_rn(both(-h.lr), __ffma2_rn(both(decay), w, hat), w);
   return make_float2(max_nan(w.x, least), max_nan(w.y, least));
@@ -191,6 +197,7 @@ __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ Li
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
+  const bool exactRoots = exact_roots(h);
   for (int turn = 0; turn < l.turns && first < t.n; ++turn, first += TURN) {
     if (t.wide && first + TURN <= t.n) {
       const long long i = first + threadIdx.x * 8;
@@ -199,15 +206,18 @@ __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ Li
       load8(ms + i, m);
       load8(vs + i, v);
       load8(t.w + i, w);
+      const auto update = [&](auto exact) {
 #pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
-        moments(Singly(), h, gs, make_float2(g[k], g[k + 1]), m2, v2);
-        const float2 w2 = updated(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
-        m[k] = m2.x; m[k + 1] = m2.y;
-        v[k] = v2.x; v[k + 1] = v2.y;
-        w[k] = w2.x; w[k + 1] = w2.y;
-      }
+        for (int k = 0; k < 8; k += 2) {
+          float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
+          moments(Singly(), h, gs, make_float2(g[k], g[k + 1]), m2, v2);
+          const float2 w2 = updated<exact>(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
+          m[k] = m2.x; m[k + 1] = m2.y;
+          v[k] = v2.x; v[k + 1] = v2.y;
+          w[k] = w2.x; w[k + 1] = w2.y;
+        }
+      };
+      if (exactRoots) update(std::true_type()); else update(std::false_type());
       store8(ms + i, m);
       store8(vs + i, v);
       store8(t.w + i, w);
@@ -218,7 +228,8 @@ __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ Li
       const long long i = first + j;
       float2 m = both(ms[i]), v = both(vs[i]);
       moments(Singly(), h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
-      const float w = updated(h, both(t.w[i]), m, v, t.decay, t.least).x;
+      const float2 w1 = both(t.w[i]);
+      const float w = (exactRoots ? updated<true>(h, w1, m, v, t.decay, t.least) : updated<false>(h, w1, m, v, t.decay, t.least)).x;
       ms[i] = m.x; vs[i] = v.x; t.w[i] = w;
       if (t.w16) store_16(t.w16, t.w16type, i, w);
     }
@@ -327,6 +338,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ 
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
+  const bool exactRoots = exact_roots(h);
   const auto whole = [&](long long b) { return t.wide && (b + 1) * BLOCK <= t.n; };
   if (whole(block)) ask(t, block, lane, incoming[0][warp]);
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -371,11 +383,17 @@ __global__ void __launch_bounds__(THREADS, 4) k_adamw_8(const __grid_constant__ 
       v[2 * k] = decode_v<0>(vw[k], sv); v[2 * k + 1] = decode_v<2>(vw[k], sv);
     }
     float topM = 0.f, topV = 0.f;
+    const auto update = [&](auto exact) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        moments(one, h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
+        const float2 to = updated<exact>(h, make_float2(w[2 * k], w[2 * k + 1]), m[k], v[k], t.decay, t.least);
+        w[2 * k] = to.x; w[2 * k + 1] = to.y;
+      }
+    };
+    if (exactRoots) update(std::true_type()); else update(std::false_type());
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      moments(one, h, gs, make_float2(g[2 * k], g[2 * k + 1]), m[k], v[k]);
-      const float2 to = updated(h, make_float2(w[2 * k], w[2 * k + 1]), m[k], v[k], t.decay, t.least);
-      w[2 * k] = to.x; w[2 * k + 1] = to.y;
       if (!wide) { // (a NaN scale would reach the values behind the end)
         if (i + 2 * k >= t.n) m[k].x = v[k].x = 0.f;
         if (i + 2 * k + 1 >= t.n) m[k].y = v[k].y = 0.f;

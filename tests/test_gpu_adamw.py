@@ -587,3 +587,28 @@ def test_norm_depends_on_the_gradients_alone(abi):
         abi.check(L.scn_grad_norm((abi.AdamWTensor * 1)(e), 1, norm.data_ptr(), ws.data_ptr(), ws.numel(), s))
         results.add(norm.item())
     assert len(results) == 1 and abs(results.pop() - 1) <= 2.0 ** -23
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("eps", [1.2e-38, 1e-30, 1e-20, 1e-15, 2e-12, 3e-12, 1e-8])
+def test_second_moments_below_the_normal_range(abi, bits, offset, eps):
+    """Gradients from 1e-23 to 1e-15: second moments from nothing over 2^-149 and 2^-126 up, beside an eps that hides their roots or is
+    dwarfed by them.  The moments in single 32-bit roundings, then the step from them in 64 bits."""
+    rng = np.random.default_rng(23)
+    n, lr, b1, b2 = 5000, 1e-3, 0.5, 0.5
+    t = make(abi, rng, [n], bits, offset=offset, decay=0.0)[0]
+    g = (rng.choice([-1, 1], n) * 10.0 ** rng.uniform(-23, -15, n)).astype(f32)
+    t["g"].copy_(torch.from_numpy(g))
+    for k in ("w", "m", "v", "m_scale", "v_scale"):
+        if t.get(k) is not None:
+            t[k].zero_()
+    abi.AdamW([t]).step(lr, 1, beta1=b1, beta2=b2, eps=eps)
+    m, v = np_moments(np.zeros(n, f32), np.zeros(n, f32), g, 1.0, b1, b2)
+    assert (v == 0).any() and ((v > 0) & (v < 2.0 ** -126)).any() and (v > 2.0 ** -126).any()
+    if bits == 32:
+        assert np.array_equal(t["m"].cpu().numpy(), m) and np.array_equal(t["v"].cpu().numpy(), v)
+    m, v, eps = m.astype(np.float64), v.astype(np.float64), float(f32(eps))
+    want = -float(f32(lr)) * 2.0 * m / (np.sqrt(v) * math.sqrt(2.0) + eps)
+    # behind the moments below 20 U (see check_step), one more where eps hides a root that is left out, lr's product and the result
+    assert (np.abs(t["w"].cpu().numpy().astype(np.float64) - want) <= 23 * U * np.abs(want) + 1e-44).all()
