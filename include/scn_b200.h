@@ -502,9 +502,9 @@ typedef struct {
 } scn_adamw_tensor_t;
 
 typedef struct {
-  double lr, beta1, beta2, eps; /* 0 <= beta < 1, eps >= 2^-126                                       */
+  double lr, beta1, beta2, eps; /* 0 <= beta < 1, eps >= 2^-126; lr and grad_scale finite in 32 bits too */
   double grad_scale;            /* 1 / batch size for the sums over a batch that the layers give, say */
-  double max_norm;              /* > 0: clip to this norm (needs d_norm); 0: no clipping              */
+  double max_norm;              /* at least 2^-149: clip to this norm (needs d_norm); 0: no clipping  */
   long long step;               /* t >= 1                                                             */
   unsigned seed;                /* of the 8-bit states' rounding: another one each step               */
 } scn_adamw_t;

@@ -554,9 +554,10 @@ extern "C" int scn_adamw_scalars(const scn_adamw_t *h, scn_adamw_scalars_t *out)
   clear_error();
   if (!h || !out) return fail(SCN_ERR_INVALID, "null pointer");
   if (!(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1)) return fail(SCN_ERR_INVALID, "AdamW: beta1 and beta2 must be in [0, 1)");
-  if (!std::isfinite(h->lr) || !std::isfinite(h->grad_scale)) return fail(SCN_ERR_INVALID, "AdamW: lr and grad_scale must be finite");
+  if (!std::isfinite((float)h->lr) || !std::isfinite((float)h->grad_scale)) return fail(SCN_ERR_INVALID, "AdamW: lr and grad_scale must be finite");
   if (!(std::isfinite(h->eps) && (float)h->eps >= 1.17549435e-38f)) return fail(SCN_ERR_INVALID, "AdamW: eps must be a positive normal 32-bit number");
   if (!(std::isfinite(h->max_norm) && h->max_norm >= 0)) return fail(SCN_ERR_INVALID, "AdamW: max_norm must be finite and not negative");
+  if (h->max_norm > 0 && (float)h->max_norm == 0.f) return fail(SCN_ERR_INVALID, "AdamW: max_norm is 0 in 32 bits, which would not clip at all");
   if (h->step < 1) return fail(SCN_ERR_INVALID, "AdamW: steps count from 1");
   out->lr = (float)h->lr;
   out->beta1 = (float)h->beta1;

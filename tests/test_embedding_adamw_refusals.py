@@ -183,3 +183,22 @@ def test_row_strides(a):
     for bad in [torch.empty(1, 4).expand(3, 4), torch.empty(4, 3).t(), torch.empty(3, 8)[:, ::2], torch.empty(3, 4, dtype=torch.float64), torch.empty(12)]:
         with pytest.raises(a.ScnError):
             a._row_stride(bad, 3, 4, "out")
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(lr=1e39), "finite"), (dict(lr=-1e39), "finite"), (dict(grad_scale=1e39), "finite"), (dict(grad_scale=-4e38), "finite"), (dict(max_norm=1e-46), "max_norm"),
+    (dict(max_norm=5e-324), "max_norm")])
+def test_numbers_that_32_bits_cannot_hold(a, change, text):
+    """The kernel reads 32-bit numbers: infinities in place of a rate or a scale, or a clip that turned into no clip, are refused."""
+    t, h = (a.AdamWTensor * 1)(entry(a)), parameters(a, **change)
+    refused(a, a.lib().scn_adamw_step(t, 1, ctypes.byref(h), None, P, None), INVALID, text)
+    out = a.AdamWScalars()
+    refused(a, a.lib().scn_adamw_scalars(ctypes.byref(h), ctypes.byref(out)), INVALID, text)
+
+
+@pytest.mark.parametrize("change", [dict(lr=3e38), dict(max_norm=1e300), dict(max_norm=1e-44), dict(eps=1e39), dict(lr=1e-50)])
+def test_numbers_at_the_ends_of_32_bits(a, change):
+    """Rounding these to 32 bits changes no step by more than roundings do."""
+    h, out = parameters(a, **change), a.AdamWScalars()
+    assert a.lib().scn_adamw_scalars(ctypes.byref(h), ctypes.byref(out)) == 0
+    assert out.max_norm > 0 or "max_norm" not in change
