@@ -4,6 +4,7 @@ torch is used only for device memory and streams: every function passes raw devi
 and torch's current stream to libscn_b200.so.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -53,6 +54,9 @@ class AdamWTensor(ctypes.Structure):
 class AdamWParameters(ctypes.Structure):
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
                 ("grad_scale", ctypes.c_double), ("max_norm", ctypes.c_double), ("step", c_ll), ("seed", ctypes.c_uint)]
+
+
+_PACK_PARAMETERS = struct.Struct("6dqI").pack_into  # all of the fields at once: half the time of one by one
 
 
 class AdamWScalars(ctypes.Structure):
@@ -724,7 +728,6 @@ class AdamW:
                 written = max(written, last)
         self.h = AdamWParameters()
         self._h = ctypes.byref(self.h)
-        self._set = None  # the numbers that h holds
         self._norm = torch.empty((), device=self.device)
         self._workspace_bytes = lib().scn_grad_norm_workspace_bytes()
         self._workspace = torch.empty(self._workspace_bytes, dtype=torch.uint8, device=self.device)
@@ -750,12 +753,11 @@ class AdamW:
         else:
             if lr is None or step is None:
                 raise ScnError("invalid argument: a step needs lr and its number")
-            numbers = (lr, beta1, beta2, eps, grad_scale, max_norm, step, step if seed is None else seed)
-            if numbers != self._set:
-                p, self._set = self.h, None
-                p.lr, p.beta1, p.beta2, p.eps, p.grad_scale, p.max_norm, p.step, p.seed = numbers[:7] + (numbers[7] & 0xFFFFFFFF,)
-                self._set = numbers
             h, sp = self._h, None
+            try:
+                _PACK_PARAMETERS(self.h, 0, lr, beta1, beta2, eps, grad_scale, max_norm, step, (step if seed is None else seed) & 0xFFFFFFFF)
+            except struct.error as e:
+                raise TypeError("AdamW step: %s" % e)
         if norm is None:
             np = None
         elif norm is self._norm:

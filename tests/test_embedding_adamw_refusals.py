@@ -202,3 +202,11 @@ def test_numbers_at_the_ends_of_32_bits(a, change):
     h, out = parameters(a, **change), a.AdamWScalars()
     assert a.lib().scn_adamw_scalars(ctypes.byref(h), ctypes.byref(out)) == 0
     assert out.max_norm > 0 or "max_norm" not in change
+
+
+def test_parameters_are_packed_in_the_order_of_their_fields(a):
+    values = dict(lr=1.5, beta1=0.25, beta2=0.5, eps=2.0, grad_scale=-3.0, max_norm=7.0, step=(1 << 40) + 3, seed=0xFFFFFFFF)
+    h = a.AdamWParameters()
+    a._PACK_PARAMETERS(h, 0, *values.values())
+    assert [f for f, _ in a.AdamWParameters._fields_] == list(values)
+    assert all(getattr(h, k) == v for k, v in values.items())

@@ -612,3 +612,14 @@ def test_second_moments_below_the_normal_range(abi, bits, offset, eps):
     want = -float(f32(lr)) * 2.0 * m / (np.sqrt(v) * math.sqrt(2.0) + eps)
     # behind the moments below 20 U (see check_step), one more where eps hides a root that is left out, lr's product and the result
     assert (np.abs(t["w"].cpu().numpy().astype(np.float64) - want) <= 23 * U * np.abs(want) + 1e-44).all()
+
+
+def test_every_step_takes_its_own_numbers(abi):
+    """Nothing is kept of the step before, also where the numbers are the same."""
+    w, g = torch.zeros(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = abi.AdamW([dict(w=w, g=g, **abi.adamw_states(300, "cuda", 32))])
+    opt.step(0.125, 1, eps=1e-12)
+    opt.h.lr = 7.0  # (what the C call last read)
+    opt.step(0.125, 1, eps=1e-12)
+    # step 1 twice: m = 0.1, then 0.19, v = 0.001, then 0.001999: lr times 1, then 1.9 / sqrt(1.999)
+    assert (w.double() + 0.125 * (1 + 1.9 / math.sqrt(1.999))).abs().max() < 1e-6
