@@ -191,48 +191,46 @@ template <int CAP>
 __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   const int at = owner(l, blockIdx.x);
   const Tensor &t = l.t[at];
-  long long first = (long long)((int)blockIdx.x - l.first[at]) * l.turns * TURN;
+  const long long first = (long long)((int)blockIdx.x - l.first[at]) * TURN; // (chunks of one turn)
   float *ms = (float *)t.m, *vs = (float *)t.v;
   wait_for_prior_grids();
   if (dh) h = *dh;
   const float gs = gradient_scale(h, norm);
   if (gs != gs) return;
   const bool exactRoots = exact_roots(h);
-  for (int turn = 0; turn < l.turns && first < t.n; ++turn, first += TURN) {
-    if (t.wide && first + TURN <= t.n) {
-      const long long i = first + threadIdx.x * 8;
-      float w[8], g[8], m[8], v[8];
-      load8_typed(t.g, t.gtype, i, g);
-      load8(ms + i, m);
-      load8(vs + i, v);
-      load8(t.w + i, w);
-      const auto update = [&](auto exact) {
+  if (t.wide && first + TURN <= t.n) {
+    const long long i = first + threadIdx.x * 8;
+    float w[8], g[8], m[8], v[8];
+    load8_typed(t.g, t.gtype, i, g);
+    load8(ms + i, m);
+    load8(vs + i, v);
+    load8(t.w + i, w);
+    const auto update = [&](auto exact) {
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
-          moments(Singly(), h, gs, make_float2(g[k], g[k + 1]), m2, v2);
-          const float2 w2 = updated<exact>(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
-          m[k] = m2.x; m[k + 1] = m2.y;
-          v[k] = v2.x; v[k + 1] = v2.y;
-          w[k] = w2.x; w[k + 1] = w2.y;
-        }
-      };
-      if (exactRoots) update(std::true_type()); else update(std::false_type());
-      store8(ms + i, m);
-      store8(vs + i, v);
-      store8(t.w + i, w);
-      if (t.w16) store8_typed(t.w16, t.w16type, i, w);
-      continue;
-    }
-    for (int j = threadIdx.x; j < TURN && first + j < t.n; j += THREADS) {
-      const long long i = first + j;
-      float2 m = both(ms[i]), v = both(vs[i]);
-      moments(Singly(), h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
-      const float2 w1 = both(t.w[i]);
-      const float w = (exactRoots ? updated<true>(h, w1, m, v, t.decay, t.least) : updated<false>(h, w1, m, v, t.decay, t.least)).x;
-      ms[i] = m.x; vs[i] = v.x; t.w[i] = w;
-      if (t.w16) store_16(t.w16, t.w16type, i, w);
-    }
+      for (int k = 0; k < 8; k += 2) {
+        float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
+        moments(Singly(), h, gs, make_float2(g[k], g[k + 1]), m2, v2);
+        const float2 w2 = updated<exact>(h, make_float2(w[k], w[k + 1]), m2, v2, t.decay, t.least);
+        m[k] = m2.x; m[k + 1] = m2.y;
+        v[k] = v2.x; v[k + 1] = v2.y;
+        w[k] = w2.x; w[k + 1] = w2.y;
+      }
+    };
+    if (exactRoots) update(std::true_type()); else update(std::false_type());
+    store8(ms + i, m);
+    store8(vs + i, v);
+    store8(t.w + i, w);
+    if (t.w16) store8_typed(t.w16, t.w16type, i, w);
+    return;
+  }
+  for (int j = threadIdx.x; j < TURN && first + j < t.n; j += THREADS) {
+    const long long i = first + j;
+    float2 m = both(ms[i]), v = both(vs[i]);
+    moments(Singly(), h, gs, both(load_typed(t.g, t.gtype, i)), m, v);
+    const float2 w1 = both(t.w[i]);
+    const float w = (exactRoots ? updated<true>(h, w1, m, v, t.decay, t.least) : updated<false>(h, w1, m, v, t.decay, t.least)).x;
+    ms[i] = m.x; vs[i] = v.x; t.w[i] = w;
+    if (t.w16) store_16(t.w16, t.w16type, i, w);
   }
 }
 

@@ -132,8 +132,9 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
   // 3.4 M rows of 64 floats, against 164 us with two)
   if (W == MOST) return launch(k_embedding_forward<T, O, MOST, 2>, 2);
   if (W == 1) return launch(k_embedding_forward<T, O, 1, 8>, 8);
-  if (W == MOST / 2) return launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
-  return launch(k_embedding_forward<T, O, 2, 8>, 8);
+  if constexpr (MOST == 8) // (a 16-bit table: 8, 4, 2, 1; floats: 4, 2, 1)
+    if (W == 2) return launch(k_embedding_forward<T, O, 2, 8>, 8);
+  return launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
 }
 
 // ------------------------------------------------------------------ stable radix sort of (token, row)
