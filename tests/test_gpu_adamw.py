@@ -623,3 +623,57 @@ def test_every_step_takes_its_own_numbers(abi):
     opt.step(0.125, 1, eps=1e-12)
     # step 1 twice: m = 0.1, then 0.19, v = 0.001, then 0.001999: lr times 1, then 1.9 / sqrt(1.999)
     assert (w.double() + 0.125 * (1 + 1.9 / math.sqrt(1.999))).abs().max() < 1e-6
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_large_list_of_several_tensors(abi, bits):
+    """Above some 30 M values a CTA takes several turns of a chunk (of the norm's too).  Tensors that end at a chunk's end, within one, one
+    value on either side, at an address that allows single values only, with and without a copy: every code, scale, moment and parameter, and the norm."""
+    chunk = 8 * 8 * BLOCK  # of 8-bit states
+    sizes = [20_000_003, chunk, 3 * chunk + 1, 5 * chunk - 1, 777, 6_000_001, 1, 8 * chunk + 12 * BLOCK, 5_000_000, 4 * chunk]
+    odd, types = {1, 5, 7}, [torch.bfloat16, torch.float32, torch.float16]
+    assert sum(sizes) > 100 * 148 * 8 * BLOCK
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    dither, ts, block = [], [], 0
+
+    def put(n, dtype, k):
+        return torch.zeros(n + 1, device="cuda", dtype=dtype)[1:] if k in odd else torch.zeros(n, device="cuda", dtype=dtype)
+
+    for k, n in enumerate(sizes):
+        t = dict(w=put(n, torch.float32, k), g=put(n, types[k % 3], k), weight_decay=0.0, w_min=-math.inf)
+        states = abi.adamw_states(n, "cuda", bits)
+        t.update(m=put(n, states["m"].dtype, k), v=put(n, states["v"].dtype, k), **{x: states[x] for x in states if x.endswith("scale")})
+        if k % 2:
+            t["w16"] = put(n, torch.bfloat16, k)
+        t["w"].normal_(generator=gen)
+        ts.append(t)
+        dither.append(block * BLOCK)
+        block += -(-n // BLOCK)
+    opt, one, full = abi.AdamW(ts), lambda x: float(f32(x)), 0xFFFFFFFF
+    moments = [[torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")] for n in sizes]
+    for step in (1, 2):
+        for t in ts:
+            n = len(t["g"])
+            t["g"].copy_(torch.randn(n, device="cuda", generator=gen) * torch.exp(2 * torch.randn(n, device="cuda", generator=gen)) * 1e-3)
+        before = snapshot(ts)
+        want = math.sqrt(sum((t["g"].double() ** 2).sum().item() for t in ts))
+        norm = opt.grad_norm()
+        assert abs(norm.item() - want) <= 1.001 * U * want
+        opt.step(1e-3, step)
+        check_step(before, ts, step=step)
+        for t, mv, start in zip(ts, moments, dither):
+            g, n = t["g"].float(), len(t["g"])
+            mv[0], mv[1] = mv[0] * one(B1) + g * one(1 - B1), mv[1] * one(B2) + (g * g) * one(1 - B2)
+            if bits == 32:
+                assert torch.equal(t["m"], mv[0]) and torch.equal(t["v"], mv[1])
+                continue
+            h = ((start + torch.arange(n, device="cuda")) * 0x6A09E667 + ((step * 0xBB67AE85) & full)) & full
+            h = ((h ^ (h >> 16)) * 0xBB67AE85) & full
+            h = ((h ^ (h >> 15)) * 0x3C6EF373) & full
+            h = h ^ (h >> 16)
+            pad = torch.nn.functional.pad
+            for i, (k, bits_of) in enumerate((("m", h & 0xFFFF), ("v", h >> 16))):
+                fill = (0, -n % BLOCK)
+                codes, scale = torch_encode(pad(mv[i], fill), pad((bits_of.float() + 0.5) * 2.0 ** -16, fill, value=0.5), k == "v")
+                assert torch.equal(t[k + "_scale"], scale) and torch.equal(t[k], codes[:n])
+                mv[i] = abi.adamw_decode(t[k], t[k + "_scale"])

@@ -345,3 +345,28 @@ def test_gradient_of_the_largest_vocabularies(abi, n, V):
     assert torch.equal(dt[at.long(), 0], want) and dt.count_nonzero().item() == len(at)
     abi.embedding_backward(dout, tok, dt, accumulate=True)
     assert torch.equal(dt[at.long(), 0], 2 * want) and dt.count_nonzero().item() == len(at)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("C,extra,first", LAYOUTS[:10] + [(48, 1, 1), (65, 0, 0), (130, 0, 0)])
+def test_gradient_of_many_tiles(abi, dtype, accumulate, C, extra, first):
+    """Some thousands of tiles, so that tokens on 32 of them and more are joined by the tiles' own warps: every width of access and number
+    of columns a thread, with a token on a third of the rows, some on a few tiles, and many on a few rows.  Whole numbers whose sums stay
+    below 2^24: exact in whatever order."""
+    n, V = 300007, 5003
+    gen = torch.Generator(device="cuda").manual_seed(C + extra)
+    u = torch.rand(n, device="cuda", generator=gen)
+    tok = torch.randint(0, V, (n,), device="cuda", generator=gen, dtype=torch.int32)
+    tok[u < 0.6] = (torch.randint(0, 9, (n,), device="cuda", generator=gen, dtype=torch.int32) * 500 + 7)[u < 0.6]
+    tok[u < 0.33] = V // 3
+    tok[u > 0.99] = -1
+    dout, whole = strided(n, C, extra, first, dtype)
+    dout.copy_(torch.randint(-4, 5, (n, C), device="cuda", generator=gen))
+    before = torch.randint(-9, 10, (V, C), device="cuda", generator=gen).float()
+    ok = tok >= 0
+    want = torch.zeros(V, C, dtype=torch.float64, device="cuda").index_add_(0, tok[ok].long(), dout.double()[ok])
+    if accumulate:
+        want += before
+    dt = before.clone() if accumulate else torch.full((V, C), math.nan, device="cuda")
+    assert torch.equal(abi.embedding_backward(dout, tok, dt, accumulate=accumulate).double(), want)
