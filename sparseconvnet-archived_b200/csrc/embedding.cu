@@ -75,8 +75,8 @@ template <class T, class O, int W, int ROWS> __global__ void __launch_bounds__(T
   }
 }
 // The same value by value, for widths, strides and addresses that allow no more: a warp takes ROWS rows and 32 * COLS columns at
-// once, so that about as many bytes are on their way.  224 k rows of 96 from a 16-bit table into rows of 99 floats: 26 us (a
-// plain fill of as many bytes takes 14.5 us); groups of 48 threads with two turns a row took 39 us.
+// once.  224 k rows of 96 from a 16-bit table into rows of 99 floats: 26 us (a plain fill of as many bytes takes 14.5 us);
+// groups of 48 threads with two turns a row took 39 us.
 template <class T, class O, int ROWS, int COLS> __global__ void __launch_bounds__(THREADS) k_embedding_forward_single(const Lookup p) {
   const int lane = threadIdx.x & 31;
   const unsigned i = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * ROWS;
@@ -118,8 +118,10 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
   while (W > 1 && !(p.C % W == 0 && (uintptr_t)p.table % (W * sizeof(T)) == 0 && ((uintptr_t)p.out | (uintptr_t)p.stride) % std::min<size_t>(16, W * sizeof(O)) == 0)) W /= 2;
   if (W == 1 && p.C > 16) {
     const auto single = [&](auto kernel, unsigned rows) { return launch_dependent(kernel, dim3((p.n + WARPS * rows - 1) / (WARPS * rows)), dim3(THREADS), 0, s, p); };
+    // Rows of up to 32 values sixteen at a time, of up to 96 three, longer ones two, so that few lanes idle in a row's last columns.  224 k rows
+    // three values apart, us with (16, 1), (3, 3), (2, 4): 20 columns 8.7, 13.1, 16.1; 32: 10.3, 13.1, 16.2; 48: 20.7, 15.8, 17.8; 64: 27.3, 18.6, 19.5;
+    // 96: 41.5, 26.5, 26.2; 128: 53.8, 37.9, 33.1; 515: 243, 141, 124.  (8, 2) is no better than (3, 3) anywhere: 48: 16.1; 64: 19.7.
     if (p.C <= 32) return single(k_embedding_forward_single<T, O, 16, 1>, 16);
-    if (p.C <= 64) return single(k_embedding_forward_single<T, O, 8, 2>, 8);
     if (p.C <= 96) return single(k_embedding_forward_single<T, O, 3, 3>, 3);
     return single(k_embedding_forward_single<T, O, 2, 4>, 2);
   }
@@ -128,13 +130,13 @@ template <class T, class O> cudaError_t launch_forward(const Lookup &p, cudaStre
     const unsigned grid = std::min((p.n + groups * rows - 1) / (groups * rows), 64u * sm_count());
     return launch_dependent(kernel, dim3(grid), dim3(THREADS), 0, s, p, lanes, groups);
   };
-  // narrow accesses: more rows at once, for as many bytes on their way (four rows of 16 bytes at once took longer: 197 us for
-  // 3.4 M rows of 64 floats, against 164 us with two)
+  // Two rows at once, four of half-width accesses.  us with two, four and eight rows: 3.4 M rows of 64 floats (16 bytes an access) 160, 188, 252; of
+  // 30 (8 bytes) 119, 115, 192; of 15 (4 bytes) 99, 118, 168; 1 M rows of 98 16-bit values (4 bytes) 87, 88, 113.
+  if (W == MOST / 2) return launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
   if (W == MOST) return launch(k_embedding_forward<T, O, MOST, 2>, 2);
-  if (W == 1) return launch(k_embedding_forward<T, O, 1, 8>, 8);
   if constexpr (MOST == 8) // (a 16-bit table: 8, 4, 2, 1; floats: 4, 2, 1)
-    if (W == 2) return launch(k_embedding_forward<T, O, 2, 8>, 8);
-  return launch(k_embedding_forward<T, O, MOST / 2, 4>, 4);
+    if (W == 2) return launch(k_embedding_forward<T, O, 2, 2>, 2);
+  return launch(k_embedding_forward<T, O, 1, 2>, 2);
 }
 
 // ------------------------------------------------------------------ stable radix sort of (token, row)
