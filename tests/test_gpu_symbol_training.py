@@ -413,3 +413,28 @@ def test_weight_files_without_the_table(scn, abi, table, tmp_path, act):
     net.load_weights(str(tmp_path / "w"), 2)
     assert all(x is None or np.array_equal(x, y) for i in learnt for x, y in zip(plain.get_weights(i), net.get_weights(i)))
     assert np.array_equal(net.get_symbols(), table + np.float32(1))
+
+
+def test_dropped_features_follow_their_moments_and_decay(scn, abi, table):
+    """As documented: a batch that drops features gives their weights gradients of zero, so that the moments of earlier batches and the
+    weight decay go on moving them.  Step 1 keeps all features: m = 0.1 g and v = 0.001 g^2, the move is the rate times the sign of g (and
+    decay).  Step 2 with g = 0: m = 0.09 g, v = 0.000999 g^2, a move by (0.09 / 0.19) / sqrt(0.000999 / 0.001999) of the rate, whatever g."""
+    net = build(scn, abi, abi.VLEAKYRELU, dropout=0.5)
+    at = [i for i, L in enumerate(net.layers()) if L["type"] == 2][1]
+    net.set_symbols(table)
+    keys, off, syms, labels = batch(net.inputSpatialSize, 5)
+    lr, decay = 1e-3, 0.25
+    net.use_adamw(eps=1e-20, weight_decay=decay)
+    W = [net.get_weights(at)[0].astype(np.float64)]
+    dropped = np.arange(1, 64, 2)
+    for present in (np.arange(64), np.arange(0, 64, 2)):
+        net.set_dropout_features(at, present)
+        net.train_batch_symbols(keys, off, syms, labels, lr)
+        W.append(net.get_weights(at)[0].astype(np.float64))
+    first, second = (W[1] - W[0] + lr * decay * W[0])[:, dropped] / lr, (W[2] - W[1] + lr * decay * W[1])[:, dropped] / lr
+    learnt = np.abs(first) > 0.5  # (a weight without a gradient has only decayed)
+    assert learnt.mean() > 0.5
+    want = np.sign(first) * (0.09 / 0.19) / np.sqrt(0.000999 / 0.001999)
+    # each weight is rounded to 32 bits (U of it, over the rate), the step below 30 U, the rates and betas given in 32 bits
+    assert (np.abs(second - want)[learnt] <= 2 * U * np.abs(W[1][:, dropped]).max() / lr + 40 * U + 1e-5).all()
+    assert np.abs(second[~learnt]).max(initial=0.0) <= 2 * U * np.abs(W[1]).max() / lr + 1e-5
