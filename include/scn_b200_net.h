@@ -99,11 +99,14 @@ int scn_net_use_adamw(scn_net_t *net, float beta1, float beta2, float eps, float
 /* Inputs whose rows carry a code instead of features: a table h_table [n_symbols x nInputFeatures] turns symbol s into the
  * features scale * table[s] (scn_embedding_forward; a negative symbol, a background row's say, into zeros), and training
  * batches of symbols learn it as well (scn_embedding_backward).  Call it before scn_net_use_adamw if it replaces a table.
- * Weight files then hold the table behind everything else. */
+ * Weight files then hold the table behind everything else (one without it is refused before anything is loaded).  Symbols reach a
+ * network through the two calls below and, in C++, through interfaces[0].symbols: data sets, scn_net_forward_host_begin / _end, the
+ * device-resident and the exchange calls take features. */
 int scn_net_set_symbols(scn_net_t *net, int n_symbols, float scale, const float *h_table);
 /* The table as it is now and its gradient of the last training batch (either may be NULL). */
 int scn_net_get_symbols(scn_net_t *net, float *h_table, float *h_gradient);
-/* scn_net_forward_host and scn_net_train_batch with h_symbols[rows], each below n_symbols, in place of the features. */
+/* scn_net_forward_host and scn_net_train_batch with h_symbols[rows], each below n_symbols, in place of the features.  (As for those:
+ * rows x nInputFeatures below 2^31.) */
 int scn_net_forward_host_symbols(scn_net_t *net, int batch, const int *h_keys, const int *h_off, const int *h_symbols, float *h_probs,
                                  int *h_predictions);
 int scn_net_train_batch_symbols(scn_net_t *net, int batch, const int *h_keys, const int *h_off, const int *h_symbols, const int *h_labels,

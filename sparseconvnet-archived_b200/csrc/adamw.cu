@@ -73,8 +73,9 @@ __device__ __forceinline__ void store_16(void *p, int type, long long i, float v
 
 // ------------------------------------------------------------------ norm
 // Squares are added up in 64 bits: nothing overflows, and the result does not depend on how many CTAs there are by more than
-// its last rounding.  A CTA a chunk leaves its sum, one CTA adds them up in a fixed order.  2.8 M values: 5.4 + 2.5 us, 30 M: 25 us
-// (4.9 TB/s).
+// its last rounding.  A CTA a chunk leaves its sum, one CTA adds them up in a fixed order.  2.8 M values, from memory: 9 + 2 us (launches
+// overlap); 30 M values of 32 bits 34 us, 3.5 TB/s, of 16 bits 29 us: half the bytes are hardly faster, so it is the conversions and sums in 64 bits
+// that bound it there.
 template <int CAP> __global__ void __launch_bounds__(THREADS) k_grad_norm_partial(const __grid_constant__ List<CAP> l, double *partial) {
   wait_for_prior_grids();
   double sum = 0;
@@ -186,7 +187,7 @@ template <bool EXACT> __device__ __forceinline__ float2 updated(const scn_adamw_
 }
 // A CTA takes one chunk, a thread eight values a turn: everything it reads is on its way before the first is used.  150 M values
 // with 16-bit gradients and a 16-bit copy (28 bytes a value): 615 us, 6.8 TB/s, 104 % of a plain copy's rate; one value a thread at
-// a time took 1455 us, four turns a CTA 634 us.  2.8 M values, from memory: 18 us (4.3 TB/s): two waves of CTAs, mostly their latency.
+// a time took 1455 us, four turns a CTA 634 us.  2.8 M values, from memory: 16 us (4.9 TB/s): two waves of CTAs, mostly their latency.
 template <int CAP>
 __global__ void __launch_bounds__(THREADS) k_adamw_32(const __grid_constant__ List<CAP> l, scn_adamw_scalars_t h, const scn_adamw_scalars_t *dh, const float *norm) {
   const int at = owner(l, blockIdx.x);
@@ -302,7 +303,8 @@ template <int K> __device__ __forceinline__ float2 decode_v(unsigned word, float
 constexpr unsigned NOT_FINITE = 0x7F800000u;
 // A block's share of everything, on its way to a warp while it works on the block before: the step issues instructions for
 // most of the time that its memory needs, so a warp cannot do without either.  150 M values with 16-bit gradients and a 16-bit
-// copy: 461 us, 5.2 TB/s of 16 bytes a value (79 % of a plain copy's rate; 81 % of the issue slots are taken).  Loads straight into
+// copy: 460 us, 5.2 TB/s of 16 bytes a value (80 % of a plain copy's rate; 80 % of the issue slots are taken); up to 500 us once the power cap
+// has brought the clock from 1965 to some 1850 MHz.  Loads straight into
 // registers took 485 us with five CTAs an SM, 510 with four; the next block's loads into registers 515; one value in an
 // instruction 690; conversions and correctly rounded roots instead of the tricks below 2130.
 struct Incoming {
@@ -510,7 +512,8 @@ bool wide_step(const scn_adamw_tensor_t &t) {
   return wide_gradient(t) && !((uintptr_t)t.d_w & 31) && !((uintptr_t)t.d_w16 & 15) && !(states & (t.d_m_scale ? 15 : 31));
 }
 // launch(list) for the tensors that `take` accepts, CAP at a time; blocks are counted over the whole list.  Where one turn a
-// chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes `most`: it finds its tensor once for all of them.
+// chunk gives more CTAs than an SM holds in a dozen waves, a CTA takes `most`: it finds its tensor once for all of them.  (150 M values: norm and
+// 32-bit step 687 us with four turns in the norm, 717 with one; 8-bit step with decodes 770 us with one turn, 720 with four, 715 with eight, 720 with 16.)
 template <int CAP, class Take, class Wide, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Wide wide, Launch launch) {
   List<CAP> l;
   long long all = 0;
@@ -536,7 +539,8 @@ template <int CAP, class Take, class Wide, class Launch> int for_lists(const scn
   }
   return l.count ? launch(l) : (int)SCN_OK;
 }
-// The parameters' bytes are copied at every launch: the smallest list that holds them all.
+// The parameters' bytes are copied at every launch: the smallest list that holds them all.  (A step over 12 tensors: 5.3 us, with the medium list 5.5, with
+// the large one 7.1.)
 template <class Take, class Wide, class Launch> int for_lists(const scn_adamw_tensor_t *t, int count, int most, Take take, Wide wide, Launch launch) {
   if (count <= CAP_SMALL) return for_lists<CAP_SMALL>(t, count, most, take, wide, launch);
   if (count <= CAP_MEDIUM) return for_lists<CAP_MEDIUM>(t, count, most, take, wide, launch);

@@ -13,7 +13,8 @@ constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_LANES = 64;
 // out[i][c] = scale * table[tokens[i]][c]; a zero row for a token outside [0, vocab).  Groups of `lanes` threads take a row, W
 // columns a thread at a time, ROWS rows at once so that as many table rows are on their way, with the tokens of the next turn
 // already asked for; the output, which is not read again here, is stored so that it leaves the caches to the table.
-// 3.4 M rows of 64 floats from a table of 65536: 160 us, 5.6 TB/s of the 889 MB it cannot do without (85 % of a plain copy's rate).
+// 3.4 M rows of 64 floats from a table of 65536: 160 us, 5.6 TB/s of the 889 MB it cannot do without (85 % of a plain copy's rate); 169 us
+// once the power cap has brought the clock from 1965 to some 1800 MHz.
 // Rows that end or begin inside a 32-byte sector next to bytes that nobody writes cost the memory a read of the sector each:
 // the same rows 16 bytes apart take 350 us, 32 bytes apart 162 us.
 struct Lookup {
@@ -381,7 +382,7 @@ template <int ROUNDS, int BITS> __global__ void __launch_bounds__(THREADS) k_rad
 // others, and each table row is written once.  Warps wait for no other warp: a CTA whose warps met at its end would stand
 // idle while its last rows arrive (that cost 22 of 129 us).  3.4 M rows of 64 16-bit values, 131072 tokens, the k-th in
 // frequency about 1 / k: 97 us, 4.8 TB/s of the 463 MB read and written; reading rows of 128 bytes in that order and adding them up
-// takes 76 us at best.  Tiles of 2048 entries a CTA took 120 us, a ring of asynchronous copies in front of the registers 130 us,
+// takes 78 us at best.  Tiles of 2048 entries a CTA took 120 us, a ring of asynchronous copies in front of the registers 130 us,
 // rows interleaved over a warp's groups with a sum over the warp at each change of token 156 us.
 constexpr int SUM_ROWS = 8, MAX_TILE = 256, MIN_TILE = 64; // rows a thread asks for at once
 struct Sums {
@@ -529,7 +530,9 @@ __device__ __forceinline__ void warp_sums(const Sums &p, const T *dout, const ui
 // does not keep a single CTA busy (one CTA for each token: 62 us for a third of 224 k rows on one token).  First 32 tiles (from a
 // multiple of 32 on) that all begin with a token from further in front become one part, in the place of the first: the last of
 // their warps adds them up, so that nothing is launched for it (224 k rows: 49.5 -> 45 us for the whole gradient).  Where there are
-// few tiles, the second step's CTA takes them faster by itself (50 k rows: 28 us against 32).
+// 2048 tiles or fewer, the second step's CTA takes them by itself: faster where no token is hot (rows of 33 floats added on: 50 k rows 28 us against 33,
+// 100 k 33 against 35, 160 k, 2500 tiles, 40 against 41), slower with a third of the rows on one (96 floats: 50 k rows 35 against 31, 100 k 47
+// against 37, 160 k 60 against 39, 224 k 73 against 44).
 __device__ __forceinline__ void join_group(const Sums &p, long long tile, unsigned key, int first, int columns) {
   const int lane = threadIdx.x & 31;
   const long long t0 = tile / 32 * 32, tiles = (p.n + p.tile - 1ll) / p.tile;
@@ -761,7 +764,8 @@ int pack_width(int type, const void *dout, long long stride, const float *dtable
     if (C % W == 0 && stride % W == 0 && (uintptr_t)dout % (W * size) == 0 && (uintptr_t)dtable % (4 * std::min(W, 4)) == 0) return W;
   return 1;
 }
-// Entries a warp sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than 16 warps each.
+// Entries a warp sums: MAX_TILE, fewer (a power of two) where that would leave SMs with less than 16 warps each.  us with 64, 128, 256: 50 k rows of
+// 33 floats 28, 32, 44; 224 k of 96 44, 63, 70; 700 k of 96 94, 91, 83; 3.4 M 16-bit rows of 64 207, 189, 182.
 int sum_tile(long long n) {
   int tile = MAX_TILE;
   while (tile > MIN_TILE && n < 16ll * 148 * tile) tile /= 2;
@@ -769,8 +773,12 @@ int sum_tile(long long n) {
 }
 
 constexpr int LARGE_ROUNDS = 8, LEAST_DIGIT = 6;
+// Up to so many tiles every scatter adds the tiles' counts up itself, which saves a launch: 5 k rows 23 us, 28 with k_radix_scan; 98 tiles 47 us with
+// it, 52 without.
 constexpr int FEW_TILES = 64;
-int sort_rounds(long long n) { return n > (1 << 20) ? LARGE_ROUNDS : 4; } // large tiles: longer runs of a digit; small ones: work for every SM
+// Large tiles: longer runs of a digit; small ones: work for every SM.  us with small and large ones: 100 k rows 47, 49; 1 M 87, 89; 1.5 M 114, 113;
+// 3.4 M 195, 182.
+int sort_rounds(long long n) { return n > (1 << 20) ? LARGE_ROUNDS : 4; }
 struct SortPlan {
   int tiles, passes, bits, digit;            // digit: bits a pass
   int sumTile;
