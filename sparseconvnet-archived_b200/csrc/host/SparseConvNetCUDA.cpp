@@ -617,6 +617,7 @@ void SparseConvNetCUDA::loadWeights(std::string baseName, int epoch, bool moment
   std::ifstream f(filename.c_str(), std::ios::in | std::ios::binary);
   if (!f) throw ScnException("Cannot find " + filename);
   std::cout << "Loading network parameters from " << filename << std::endl;
+  cudaSafeCall(cudaStreamSynchronize(memStream.stream)); // the vectors' own copies wait for blocking streams only; a caller's may not be one
   const bool withTable = symbolTable && firstNlayers >= (int)layers.size();
   if (withTable) { // a file without the table is refused before any layer has taken its part
     size_t need = sizeof(float) * (inputNormalizingConstants.size() + (size_t)symbolTable->table.size());
@@ -637,10 +638,10 @@ void SparseConvNetCUDA::saveWeights(std::string baseName, int epoch, bool moment
   std::string filename = baseName + "_epoch-" + std::to_string(epoch) + ".cnn";
   std::ofstream f(filename.c_str(), std::ios::binary);
   if (!f) throw ScnException("Cannot write " + filename);
+  cudaSafeCall(cudaStreamSynchronize(memStream.stream)); // (as in loadWeights: the last step's update may still be running)
   for (auto l : layers) l->putWeightsToStream(f, momentum);
   if (!inputNormalizingConstants.empty()) f.write((char *)inputNormalizingConstants.data(), sizeof(float) * inputNormalizingConstants.size());
   if (symbolTable) {
-    cudaSafeCall(cudaStreamSynchronize(memStream.stream));
     vectorCUDA<float> &t = symbolTable->table;
     const bool on = t.onGPU;
     f.write((char *)t.hVector().data(), sizeof(float) * t.hVector().size());

@@ -329,6 +329,7 @@ int scn_net_set_weights(scn_net_t *net, int layer, const float *W, const float *
   return guarded([&] {
     auto n = dynamic_cast<NetworkInNetworkLayer *>(net->cnn->layers.at(layer));
     if (!n) throw ScnException("layer has no weights");
+    cudaSafeCall(cudaStreamSynchronize(net->cnn->memStream.stream)); // a forward pass of device arrays may still read the old ones
     std::vector<float> &w = n->W.hVector(), &b = n->B.hVector();
     std::memcpy(w.data(), W, sizeof(float) * w.size());
     std::memcpy(b.data(), B, sizeof(float) * b.size());
