@@ -463,7 +463,8 @@ int scn_embedding_forward(const void *d_table, int table_type, int vocab, int C,
  * it the sums are added onto what is there (magnitudes below 2^-126, there or in the result, may count as zero) and
  * rows without a token are left as they are.  Negative tokens and tokens at or above vocab (these set
  * SCN_DEV_ERR_KEY in *d_errors if not NULL) contribute nothing.
- *   d_dout      n rows of C (at most 4194240) values of dout_type, dout_stride (>= C) values apart
+ *   d_dout      n rows of C (at most 4194240) values of dout_type, dout_stride (>= C) values apart; not overlapping
+ *               the table's gradient
  *   d_workspace scn_embedding_backward_workspace_bytes(n, vocab, C) bytes (0: bad sizes), 16-byte aligned, nothing kept
  *               in it between calls; calls that can overlap on the GPU need a workspace each. */
 size_t scn_embedding_backward_workspace_bytes(long long n, int vocab, int C);
